@@ -391,6 +391,35 @@ int ymx_bn_act_backward(const void *u, const void *dy, const float *scale, const
                         void *stream);
 int ymx_bn_backward_apply(const void *dz, const void *u, const float *a, const float *b, const float *c, void *du,
                           long long n_pix, int C, int dtype, void *stream);
+
+/* ---- group normalisation with activation, dropout and shortcut (no counterpart in the reference) ----
+ * x [B][n_pix][C] dense, G groups of C / G neighbouring channels, statistics of every (sample,
+ * group) over its pixels and channels (biased variance):
+ *   h = (x - mean) / sqrt(var + eps),  t = gamma h + beta
+ *   y = keep * act(t) / (1 - rate) + residual            (residual may be NULL)
+ * stats [B][G] receives the pairs (mean, 1 / sqrt(var + eps)) that the backward pass takes.
+ * rate 0: no dropout, state may be NULL.  0 < rate < 1: state points to two 64-bit words on the
+ * device, (seed, call); element i of the map (linear index) is kept iff word i % 4 of
+ * Philox4x32-10 with counter (i / 4, call) and key seed is >= floor(rate * 2^32).  The mask is not
+ * stored: the backward pass is given the same rate and the same two words.
+ *   dx, dgamma, dbeta = gradients for dy = d loss / d y; the shortcut's gradient is dy itself.
+ * gamma, beta, stats, dgamma, dbeta are fp32; x, residual, y, dy, dx have the type dtype.  Sums are
+ * fp32 in a fixed order (reproducible).  workspace: ymx_group_norm_workspace_bytes(B, n_pix, C, G)
+ * bytes, 16-byte aligned, nothing of it is kept between calls. */
+size_t ymx_group_norm_workspace_bytes(long long B, long long n_pix, int C, int G);
+int ymx_group_norm_forward(const void *x, const float *gamma, const float *beta, const void *residual, void *y, float *stats,
+                           long long B, long long n_pix, int C, int G, int act, float eps, int dtype, double rate,
+                           const void *state, void *workspace, size_t ws_bytes, void *stream);
+int ymx_group_norm_backward(const void *x, const void *dy, const float *gamma, const float *beta, const float *stats, void *dx,
+                            float *dgamma, float *dbeta, long long B, long long n_pix, int C, int G, int act, int dtype,
+                            double rate, const void *state, void *workspace, size_t ws_bytes, void *stream);
+
+/* ---- dropout (no counterpart in the reference) ----------------------------------------------
+ *   y = keep * x / (1 - rate) + residual                 (residual may be NULL; 0 <= rate < 1)
+ * over n elements, keep as above; a dropped element is 0 whatever x holds.  The gradient is the
+ * same call on dy without residual. */
+int ymx_dropout(const void *x, const void *residual, void *y, long long n, int dtype, double rate, const void *state,
+                void *stream);
 int ymx_act_backward(const void *z, const void *dy, void *dz, long long n, int act, int dtype, void *stream);
 /* ymx_act_backward and ymx_bias_grad in one pass over dense [n_pix, C] rows (bf16, act 1 or 2,
  * C / 8 a power of two up to 256; ..._workspace_bytes returns 0 for anything else). */

@@ -16,7 +16,8 @@ F32, BF16 = 0, 1
 ACT_NONE, ACT_LEAKY, ACT_MISH = 0, 1, 2
 ACT_CODES = {None: ACT_NONE, "leaky": ACT_LEAKY, "mish": ACT_MISH}
 
-_vp, _i, _f, _sz, _ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_longlong
+_vp, _i, _f, _sz, _ll, _d = (ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_longlong,
+                                 ctypes.c_double)
 
 
 class ymx_op(ctypes.Structure):
@@ -44,6 +45,10 @@ SIGNATURES = {
     "ymx_bn_act_forward": (_i, [_vp, _vp, _vp, _vp, _vp, _ll, _i, _i, _i, _vp]),
     "ymx_bn_act_backward": (_i, [_vp, _vp, _vp, _vp, _vp, _ll, _i, _i, _i, _vp, _vp, _sz, _vp]),
     "ymx_bn_backward_apply": (_i, [_vp] * 6 + [_ll, _i, _i, _vp]),
+    "ymx_group_norm_workspace_bytes": (_sz, [_ll, _ll, _i, _i]),
+    "ymx_group_norm_forward": (_i, [_vp] * 6 + [_ll, _ll, _i, _i, _i, _f, _i, _d, _vp, _vp, _sz, _vp]),
+    "ymx_group_norm_backward": (_i, [_vp] * 8 + [_ll, _ll, _i, _i, _i, _i, _d, _vp, _vp, _sz, _vp]),
+    "ymx_dropout": (_i, [_vp, _vp, _vp, _ll, _i, _d, _vp, _vp]),
     "ymx_pack_weights_pair": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
     "ymx_pack_weights_dgrad_s2": (_i, [_vp, _vp, _i, _i, _i, _i, _vp]),
     "ymx_conv2d_dgrad_s2": (_i, [_vp, _vp, _vp] + [_i] * 7 + [_vp]),

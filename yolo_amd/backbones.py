@@ -32,7 +32,9 @@ class Darknet53(nn.Module):
     scale_2 [B,S/16,S/16,512], scale_3 [B,S/32,S/32,1024]).  Layers use the
     YOLOConv defaults: bias + Mish, no batch norm (backbones.py:10-42 override
     nothing).  kwargs: name, dtype (compute type; default follows the input, with
-    an fp32 image accepted by a bf16 network's first layer), seed (parameter init).
+    an fp32 image accepted by a bf16 network's first layer), seed (parameter init),
+    groupNormalization (number of groups, every convolution) and dropout (rate, on every
+    residual branch while back-propagation is recorded), as YOLOConv's.
     """
 
     def __init__(self, **kwargs):
@@ -40,25 +42,29 @@ class Darknet53(nn.Module):
         self.name = kwargs.pop("name", None)
         dtype = kwargs.pop("dtype", None)
         seed = kwargs.pop("seed", None)
+        d = dict(dtype=dtype, groupNormalization=kwargs.pop("groupNormalization", 0))
+        rate = kwargs.pop("dropout", 0.0)
         if kwargs:
             raise TypeError("Darknet53: unexpected keyword arguments %s" % sorted(kwargs))
-        d = dict(dtype=dtype)
+
+        def block(f1, f2, i):               # residual block i of 23: a dropout sequence of its own
+            return ResidialBlock(f1, f2, dropout=rate, dropout_seed=None if seed is None else seed + i, **d)
 
         s1 = [YOLOConv((3, 3, 32), **d), YOLOConv((3, 3, 64), downsample=True, **d)]
-        for _ in range(1):
-            s1.append(ResidialBlock(32, 64, **d))
+        for i in range(1):
+            s1.append(block(32, 64, i))
         s1.append(YOLOConv((3, 3, 128), downsample=True, **d))
-        for _ in range(2):
-            s1.append(ResidialBlock(64, 128, **d))
+        for i in range(2):
+            s1.append(block(64, 128, 1 + i))
         s1.append(YOLOConv((3, 3, 256), downsample=True, **d))
-        for _ in range(8):
-            s1.append(ResidialBlock(128, 256, **d))
+        for i in range(8):
+            s1.append(block(128, 256, 3 + i))
         s2 = [YOLOConv((3, 3, 512), downsample=True, **d)]
-        for _ in range(8):
-            s2.append(ResidialBlock(256, 512, **d))
+        for i in range(8):
+            s2.append(block(256, 512, 11 + i))
         s3 = [YOLOConv((3, 3, 1024), downsample=True, **d)]
-        for _ in range(4):
-            s3.append(ResidialBlock(512, 1024, **d))
+        for i in range(4):
+            s3.append(block(512, 1024, 19 + i))
         self.layer_stack_1 = nn.ModuleList(s1)
         self.layer_stack_2 = nn.ModuleList(s2)
         self.layer_stack_3 = nn.ModuleList(s3)

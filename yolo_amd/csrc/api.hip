@@ -867,6 +867,68 @@ int ymx_bn_backward_apply(const void *dz, const void *u, const float *a, const f
     return launch_bn_bwd_apply(dz, u, a, b, c, du, n_pix, C, dtype, (hipStream_t)stream);
 }
 
+// Shared checks of the group-norm entry points; fills the geometry and the dropout fields of a.
+static int gn_args(const char *what, GnArgs &a, long long B, long long n_pix, int C, int G, int act, int dtype, double rate,
+                   const void *state, const void *ws, size_t ws_bytes) {
+    if (B <= 0 || n_pix <= 0 || C <= 0 || G <= 0) return fail(YMX_EARG, "%s: non-positive size", what);
+    if (C % G) return fail(YMX_EARG, "%s: %d channels do not split into %d groups", what, C, G);
+    if (act != YMX_ACT_NONE && act != YMX_ACT_LEAKY && act != YMX_ACT_MISH) return fail(YMX_EARG, "%s: activation code %d", what, act);
+    if (dtype != YMX_F32 && dtype != YMX_BF16) return fail(YMX_EARG, "%s: dtype %d", what, dtype);
+    if (!(rate >= 0.0 && rate < 1.0)) return fail(YMX_EARG, "%s: dropout rate %g (0 <= rate < 1)", what, rate);
+    if (rate > 0.0 && (!state || ((uintptr_t)state & 7))) return fail(YMX_EARG, "%s: dropout needs a state of two 64-bit words", what);
+    // pixel indexes are 32-bit in the kernels, and so are workgroup numbers; offsets are 64-bit
+    if (n_pix > (1ll << 30) || B > (1ll << 20) || B * G > (1ll << 30) || (long long)C * B > (1ll << 33))
+        return fail(YMX_EUNSUPPORTED, "%s: %lld samples of %lld pixels and %d channels", what, B, n_pix, C);
+    const size_t need = group_norm_workspace_bytes((int)B, (int)n_pix, C, G);
+    if (!aligned16(ws)) return fail(YMX_EARG, "%s: the workspace must be 16-byte aligned", what);
+    if (ws_bytes < need) return fail(YMX_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, ws_bytes, need);
+    a.B = (int)B; a.P = (int)n_pix; a.C = C; a.G = G; a.D = C / G;
+    a.act = act; a.dtype = dtype;
+    a.state = rate > 0.0 ? (const unsigned *)state : nullptr;
+    a.threshold = (unsigned)(rate * 4294967296.0);
+    a.keep_scale = (float)(1.0 / (1.0 - rate));
+    return YMX_OK;
+}
+
+size_t ymx_group_norm_workspace_bytes(long long B, long long n_pix, int C, int G) {
+    if (B <= 0 || n_pix <= 0 || C <= 0 || G <= 0 || B > (1ll << 20) || n_pix > (1ll << 30)) return 0;
+    return group_norm_workspace_bytes((int)B, (int)n_pix, C, G);
+}
+
+int ymx_group_norm_forward(const void *x, const float *gamma, const float *beta, const void *residual, void *y, float *stats,
+                           long long B, long long n_pix, int C, int G, int act, float eps, int dtype, double rate,
+                           const void *state, void *workspace, size_t ws_bytes, void *stream) {
+    if (!x || !gamma || !beta || !y || !stats || !workspace) return fail(YMX_EARG, "group_norm_forward: null pointer");
+    if (!(eps > 0.0f)) return fail(YMX_EARG, "group_norm_forward: epsilon %g", (double)eps);
+    GnArgs a = {};
+    if (const int rc = gn_args("group_norm_forward", a, B, n_pix, C, G, act, dtype, rate, state, workspace, ws_bytes)) return rc;
+    a.x = x; a.gamma = gamma; a.beta = beta; a.res = residual; a.y = y; a.stats = stats; a.eps = eps;
+    return launch_group_norm_forward(a, workspace, (hipStream_t)stream);
+}
+
+int ymx_group_norm_backward(const void *x, const void *dy, const float *gamma, const float *beta, const float *stats, void *dx,
+                            float *dgamma, float *dbeta, long long B, long long n_pix, int C, int G, int act, int dtype,
+                            double rate, const void *state, void *workspace, size_t ws_bytes, void *stream) {
+    if (!x || !dy || !gamma || !beta || !stats || !dx || !dgamma || !dbeta || !workspace)
+        return fail(YMX_EARG, "group_norm_backward: null pointer");
+    GnArgs a = {};
+    if (const int rc = gn_args("group_norm_backward", a, B, n_pix, C, G, act, dtype, rate, state, workspace, ws_bytes)) return rc;
+    a.x = x; a.dy = dy; a.gamma = gamma; a.beta = beta; a.stats = (float *)stats; a.dx = dx; a.dgamma = dgamma; a.dbeta = dbeta;
+    return launch_group_norm_backward(a, workspace, (hipStream_t)stream);
+}
+
+int ymx_dropout(const void *x, const void *residual, void *y, long long n, int dtype, double rate, const void *state,
+                void *stream) {
+    if (!x || !y || !state) return fail(YMX_EARG, "dropout: null pointer");
+    if (n < 0) return fail(YMX_EARG, "dropout: negative size");
+    if (dtype != YMX_F32 && dtype != YMX_BF16) return fail(YMX_EARG, "dropout: dtype %d", dtype);
+    if (!(rate >= 0.0 && rate < 1.0)) return fail(YMX_EARG, "dropout: rate %g (0 <= rate < 1)", rate);
+    if ((uintptr_t)state & 7) return fail(YMX_EARG, "dropout: the state must be 8-byte aligned");
+    if (n == 0) return YMX_OK;
+    return launch_dropout(x, residual, y, n, dtype, (unsigned)(rate * 4294967296.0), (float)(1.0 / (1.0 - rate)),
+                          (const unsigned *)state, (hipStream_t)stream);
+}
+
 int ymx_bbox_iou(const float *b1, const float *b2, float *out, long long n, int giou, void *stream) {
     if (!b1 || !b2 || !out) return fail(YMX_EARG, "bbox_iou: null pointer");
     if (n < 0) return fail(YMX_EARG, "bbox_iou: negative count");

@@ -106,6 +106,25 @@ template <int ACT> __device__ __forceinline__ float act_c(float v) {
     if constexpr (ACT == YMX_ACT_LEAKY) return v > 0.0f ? v : 0.1f * v;
     return v;
 }
+__device__ __forceinline__ float mish_grad_f(float z) {
+    // d/dz [z * tanh(softplus(z))] with e = exp(z):
+    //   tanh(softplus(z)) = n / d,  n = e (e + 2),  d = n + 2
+    //   derivative = e * w / d^2,   w = 4 (z + 1) + e (4 z + 6 + e (4 + e))
+    // one exponential and one reciprocal (1 ulp each), the rest multiply-adds; -> 1 for large z
+    // (taken as 1 beyond 20, where e^4z would leave the fp32 range), -> 0 for very negative z
+#pragma clang fp contract(fast)
+    const float zc = fminf(z, 20.0f);
+    const float e = __builtin_amdgcn_exp2f(zc * 1.44269504088896f);
+    const float w = 4.0f * zc + 4.0f + e * (4.0f * zc + 6.0f + e * (4.0f + e));
+    const float d = e * (e + 2.0f) + 2.0f;
+    const float g = e * w * __builtin_amdgcn_rcpf(d * d);
+    return z > 20.0f ? 1.0f : g;
+}
+template <int ACT> __device__ __forceinline__ float act_grad_c(float z) {
+    if constexpr (ACT == YMX_ACT_MISH) return mish_grad_f(z);
+    if constexpr (ACT == YMX_ACT_LEAKY) return z > 0.0f ? 1.0f : 0.1f;
+    return 1.0f;
+}
 // act(v * sc + sh) for a pair (the affine step is one packed fma, as in affine_f).
 __device__ __forceinline__ f32x2_t affine2(f32x2_t v, f32x2_t sc, f32x2_t sh) { return __builtin_elementwise_fma(v, sc, sh); }
 template <int ACT> __device__ __forceinline__ f32x2_t act2(f32x2_t x) {
@@ -277,6 +296,24 @@ int launch_bn_reduce(const void *u, const void *dy, void *dz, const float *scale
                      int dtype, float *sums, void *ws, hipStream_t s);
 int launch_bn_bwd_apply(const void *dz, const void *u, const float *a, const float *b, const float *c, void *du, long long P, int C,
                         int dtype, hipStream_t s);
+struct GnArgs {
+    const void *x, *res, *dy;        // [B][P][C] dense; res: shortcut added after activation and dropout, or null
+    void *y, *dx;
+    const float *gamma, *beta;
+    float *stats;                    // [B][G] pairs (mean, 1 / sqrt(var + eps))
+    float *dgamma, *dbeta;
+    int B, P, C, G, D;               // samples, pixels per sample, channels, groups, channels per group
+    int act, dtype;
+    float eps;
+    const unsigned *state;           // dropout: (seed, call) on the device, see philox.h; null = none
+    unsigned threshold;
+    float keep_scale;
+};
+size_t group_norm_workspace_bytes(int B, int P, int C, int G);
+int launch_group_norm_forward(const GnArgs &a, void *ws, hipStream_t s);
+int launch_group_norm_backward(const GnArgs &a, void *ws, hipStream_t s);
+int launch_dropout(const void *x, const void *res, void *y, long long n, int dtype, unsigned threshold, float keep_scale,
+                   const unsigned *state, hipStream_t s);
 size_t conv_wgrad_workspace_bytes(int k, int Cin, int Cout, long long P);
 size_t conv_wgrad_s2_workspace_bytes(int B, int H, int W, int Cin, int Cout);
 int launch_conv_wgrad(const void *x, int x_ld, const void *dz, int dz_ld, float *dw, int B, int H, int W, int Cin, int Cout, int k,

@@ -83,6 +83,79 @@ class BatchNormalization(nn.Module):
         return affine_act(x, scale, shift, _lib.ACT_NONE)
 
 
+class Dropout(nn.Module):
+    """Dropout whose mask is computed from (seed, call number) and never stored (the interface of
+    Keras' Dropout: active with training=True, kept values divided by 1 - rate).
+
+    state holds the two numbers on the device; every active call takes the next call number, so a
+    step captured into a HIP graph draws another mask at each replay, and a checkpoint of the
+    module resumes the sequence.  seed: default one drawn from torch's CPU generator; layers with
+    the same seed draw the same masks, and so do the ranks of a data-parallel job that build the
+    model from the same generator state.
+    """
+
+    def __init__(self, rate, seed=None):
+        super().__init__()
+        self.rate = _training._check_rate(rate, "Dropout")
+        if seed is None:
+            seed = int(torch.randint(0, 2 ** 62, (1,)))
+        self.register_buffer("state", torch.tensor([int(seed), 0], dtype=torch.int64))
+
+    def draw(self):
+        """The state of the next call: (seed, call number), a tensor of its own."""
+        used = self.state.clone()
+        self.state[1:].add_(1)
+        return used
+
+    def forward(self, x, training=False):
+        if not training or self.rate == 0.0:
+            return x
+        return _training.dropout(x, self.rate, self.draw())
+
+
+class GroupNormalization(nn.Module):
+    """Group norm over the last axis of [B, ..., C] (the interface of Keras' GroupNormalization):
+    statistics of every sample and group of C / groups neighbouring channels, in training and
+    inference alike.  trainable = False freezes gamma and beta.  Differentiable with training=True
+    and inside yolo_amd.training.backprop()."""
+
+    def __init__(self, groups=32, num_features=None, epsilon=BN_EPSILON):
+        super().__init__()
+        self.groups = int(groups)
+        if self.groups <= 0:
+            raise ValueError("GroupNormalization: %d groups" % self.groups)
+        self.epsilon = epsilon
+        self.trainable = True
+        self.num_features = None
+        if num_features is not None:
+            self.build(num_features)
+
+    def build(self, num_features):
+        if num_features % self.groups:
+            raise ValueError("GroupNormalization: %d channels do not split into %d groups" % (num_features, self.groups))
+        self.num_features = num_features
+        self.gamma = nn.Parameter(torch.ones(num_features))
+        self.beta = nn.Parameter(torch.zeros(num_features))
+
+    def apply_act(self, u, act=_lib.ACT_NONE, shortcut=None, drop=None, training=True):
+        """Normalisation, activation code, dropout (a Dropout layer; training only) and shortcut in one
+        operator."""
+        gamma, beta = (self.gamma, self.beta) if self.trainable else (self.gamma.detach(), self.beta.detach())
+        name = {v: k for k, v in _lib.ACT_CODES.items()}[act]
+        rate = drop.rate if (drop is not None and training) else 0.0
+        state = drop.draw() if rate > 0.0 else None
+        if training:
+            return _training.group_norm_act(u, gamma, beta, self.groups, name, shortcut, self.epsilon, rate, state)
+        with torch.no_grad():
+            return _training.group_norm_act(u, gamma, beta, self.groups, name, shortcut, self.epsilon)
+
+    def forward(self, x, training=False):
+        if self.num_features is None:
+            self.build(x.shape[-1])
+            self.to(x.device)
+        return self.apply_act(x, training=bool(training) or _training.enabled())
+
+
 class Mish(nn.Module):
     """x * tanh(softplus(x)) (layers.py:17-22)."""
 
@@ -154,7 +227,9 @@ class YOLOConv(nn.Module):
     this class (or pass in_channels= / call build()).
 
     Extra keyword arguments: name (kept), dtype (torch.float32 or torch.bfloat16: the
-    compute type; default = the input's type), in_channels.
+    compute type; default = the input's type), in_channels, groupNormalization (number of
+    groups: GroupNormalization in the place of batch normalisation), dropout (rate, after the
+    activation and before the shortcut, while back-propagation is recorded) and dropout_seed.
     """
 
     def __init__(self, filters_shape, downsample=False, batchNormalization=False, activation="mish", **kwargs):
@@ -163,6 +238,9 @@ class YOLOConv(nn.Module):
         self.compute_dtype = kwargs.pop("dtype", None)
         in_channels = kwargs.pop("in_channels", None)
         kwargs.pop("trainable", None)
+        groups = int(kwargs.pop("groupNormalization", 0) or 0)
+        rate = _training._check_rate(kwargs.pop("dropout", 0.0) or 0.0, "YOLOConv")
+        dropout_seed = kwargs.pop("dropout_seed", None)
         if kwargs:
             raise TypeError("YOLOConv: unexpected keyword arguments %s" % sorted(kwargs))
         if len(filters_shape) != 3 or filters_shape[0] != filters_shape[1]:
@@ -171,6 +249,10 @@ class YOLOConv(nn.Module):
         self.filters = int(filters_shape[-1])
         self.downsample = bool(downsample)
         self.batch_normalization = bool(batchNormalization)
+        self.group_normalization = groups > 0
+        if groups < 0 or (self.group_normalization and self.batch_normalization):
+            raise ValueError("YOLOConv: groupNormalization is a number of groups and excludes batchNormalization")
+        self.normalized = self.batch_normalization or self.group_normalization       # linear convolution without bias
         self.act_fn = None
         if activation:
             if callable(activation):
@@ -184,7 +266,11 @@ class YOLOConv(nn.Module):
                 raise ValueError("Activation should either be a function or one of \"leaky\" or \"mish\".")
         else:
             self.act_code = _lib.ACT_NONE
+        if self.act_fn is not None and (self.group_normalization or rate > 0.0):
+            raise ValueError("YOLOConv: groupNormalization and dropout take \"leaky\", \"mish\" or no activation")
         self.bn = BatchNormalization(self.filters) if self.batch_normalization else None
+        self.gn = GroupNormalization(groups, self.filters) if self.group_normalization else None
+        self.drop = Dropout(rate, dropout_seed) if rate > 0.0 else None
         self.in_channels = None
         self._packed = {}
         if in_channels is not None:
@@ -195,7 +281,7 @@ class YOLOConv(nn.Module):
         k = self.kernel_size
         self.in_channels = int(in_channels)
         self.kernel = nn.Parameter(torch.randn(k, k, self.in_channels, self.filters, generator=generator) * 0.01)
-        if not self.batch_normalization:
+        if not self.normalized:
             self.bias = nn.Parameter(torch.zeros(self.filters))
         self._packed = {}
         return self
@@ -209,6 +295,8 @@ class YOLOConv(nn.Module):
             if self.batch_normalization:
                 self.bn.gamma.copy_(p["gamma"]); self.bn.beta.copy_(p["beta"])
                 self.bn.moving_mean.copy_(p["mean"]); self.bn.moving_variance.copy_(p["var"])
+            elif self.group_normalization:
+                self.gn.gamma.copy_(p["gamma"]); self.gn.beta.copy_(p["beta"])
             else:
                 self.bias.copy_(p["bias"])
         self._packed = {}
@@ -217,7 +305,7 @@ class YOLOConv(nn.Module):
         """(weights packed for libymx, scale or None, shift) for a compute dtype."""
         dev = self.kernel.device
         key = (dtype, dev, self.kernel._version,
-               self.bias._version if not self.batch_normalization else
+               self.bias._version if not self.normalized else None if self.group_normalization else
                (self.bn.gamma._version, self.bn.beta._version, self.bn.moving_mean._version,
                 self.bn.moving_variance._version))
         hit = self._packed.get("entry")
@@ -232,6 +320,8 @@ class YOLOConv(nn.Module):
         _lib.launch("ymx_pack_weights", wp, _lib.ptr(src), _lib.ptr(wp), k, cin, cout, code)
         if self.batch_normalization:
             scale, shift = self.bn.folded()
+        elif self.group_normalization:
+            scale = shift = None
         else:
             scale, shift = None, self.bias.detach().float().contiguous()
         entry = (wp, scale, shift, src)      # src kept alive until the pack kernel has run
@@ -245,7 +335,7 @@ class YOLOConv(nn.Module):
         Layers whose input channels do not take the MFMA kernels (the first: 3) have no
         input-gradient pack; stride-2 layers get the 2x2 depth-to-space form
         (ymx_conv2d_dgrad_s2)."""
-        bn = self.batch_normalization              # the convolution is then linear: no bias, normalisation follows
+        bn = self.normalized                       # the convolution is then linear: no bias, normalisation follows
         dev = self.kernel.device
         key = (dtype, dev, self.kernel._version, None if bn else self.bias._version)
         hit = self._packed.get("train")
@@ -280,7 +370,7 @@ class YOLOConv(nn.Module):
         return (h + 1 - k) // 2 + 1, (w + 1 - k) // 2 + 1
 
     # -- forward ----------------------------------------------------------------
-    def forward(self, x, residual=None, out_dtype=None, out=None, _grad_link=None):
+    def forward(self, x, residual=None, out_dtype=None, out=None, _grad_link=None, _linear=False):
         """x NHWC -> NHWC.  residual (same shape as the output) is added after the
         activation inside the kernel; out_dtype overrides the output element type; out, if
         given, receives the result: a [B,H',W',Cout] view whose pixels may be spaced wider than
@@ -298,6 +388,11 @@ class YOLOConv(nn.Module):
             y = _training.conv_block(self, x, residual, _grad_link)
             return y if out_dtype in (None, y.dtype) else y.to(out_dtype)
         cdt = self.compute_dtype or x.dtype
+        if self.group_normalization and not _linear:
+            y = self.gn.apply_act(self.forward(x, _linear=True), self.act_code, residual, training=False)
+            y = y if out_dtype in (None, y.dtype) else y.to(out_dtype)
+            return y if out is None else out.copy_(y)
+        act_code = _lib.ACT_NONE if _linear else self.act_code
         code = _lib.dtype_code(cdt)
         k, cin, cout = self.kernel_size, self.in_channels, self.filters
         mfma = (cin % 8 == 0) if code == _lib.BF16 else (cin % 4 == 0)
@@ -326,7 +421,7 @@ class YOLOConv(nn.Module):
             if residual.dtype != want:
                 residual = residual.to(want)
         _lib.launch("ymx_conv2d_fused_ex", x, _lib.ptr(x), _lib.ptr(wp), _lib.ptr(scale), _lib.ptr(shift), _lib.ptr(residual) if fuse_res else None,
-            _lib.ptr(y), b, h, w, cin, cout, k, 2 if self.downsample else 1, self.act_code, code,
+            _lib.ptr(y), b, h, w, cin, cout, k, 2 if self.downsample else 1, act_code, code,
             _lib.dtype_code(x.dtype), _lib.dtype_code(odt), 0, 0, y_ld)
         if self.act_fn is not None:
             y = self.act_fn(y)
@@ -339,16 +434,19 @@ class ResidialBlock(nn.Module):
     """x + conv3x3(conv1x1(x)); the add follows the second activation (layers.py:92-106).
 
     The spelling is the reference's.  The add is fused into the 3x3 conv's epilogue.
+    kwargs: dtype, groupNormalization (both convolutions), dropout and dropout_seed (the second
+    one, before the shortcut add), as YOLOConv's.
     """
 
     def __init__(self, filter_num1, filter_num2, activation="mish", **kwargs):
         super().__init__()
-        dtype = kwargs.pop("dtype", None)
+        d = dict(dtype=kwargs.pop("dtype", None), groupNormalization=kwargs.pop("groupNormalization", 0))
+        drop = dict(dropout=kwargs.pop("dropout", 0.0), dropout_seed=kwargs.pop("dropout_seed", None))
         if kwargs:
             raise TypeError("ResidialBlock: unexpected keyword arguments %s" % sorted(kwargs))
         self.layer_stack = nn.ModuleList([
-            YOLOConv(filters_shape=(1, 1, filter_num1), activation=activation, dtype=dtype),
-            YOLOConv(filters_shape=(3, 3, filter_num2), activation=activation, dtype=dtype),
+            YOLOConv(filters_shape=(1, 1, filter_num1), activation=activation, **d),
+            YOLOConv(filters_shape=(3, 3, filter_num2), activation=activation, **d, **drop),
         ])
 
     def forward(self, x, out=None):

@@ -26,7 +26,10 @@ Outside the context (the default) the layers run the fused inference kernels and
 graph.  A YOLOConv with batch normalisation (layers.py:65-68) runs as a linear convolution
 followed by ``batch_norm_act``: batch statistics, gamma / beta, activation and shortcut, with
 the moving statistics updated as Keras does (frozen layers, ``trainable = False``, keep
-normalising with the moving statistics, layers.py:11-15).
+normalising with the moving statistics, layers.py:11-15).  One with group normalisation is
+followed by ``group_norm_act`` instead: statistics of every (sample, group of channels), hence
+the same in training and inference and independent of the batch, with dropout in the same
+pass; ``dropout`` alone follows any other block.
 """
 import threading
 
@@ -169,7 +172,7 @@ class _ConvBlock(torch.autograd.Function):
             raise ValueError("yolo_amd.training: back-propagation is provided for bfloat16 networks")
         k, cin, cout = layer.kernel_size, layer.in_channels, layer.filters
         stride = 2 if layer.downsample else 1
-        act = _lib.ACT_NONE if layer.batch_normalization else layer.act_code      # normalisation and activation follow separately
+        act = _lib.ACT_NONE if layer.normalized else layer.act_code      # normalisation and activation follow separately
         ctx.act = act
         x_dtype_in = x.dtype
         x = x.contiguous()
@@ -332,9 +335,19 @@ def conv_block(layer, x, shortcut=None, link=None):
     ``backprop()``).  link: the GradLink of the ResidialBlock the layer belongs to."""
     if layer.act_fn is not None:
         raise ValueError("yolo_amd.training: callable activations are not differentiated")
+    if layer.group_normalization:
+        u = _ConvBlock.apply(x, layer.kernel, None, None, layer, None)            # linear, no bias
+        return layer.gn.apply_act(u, layer.act_code, shortcut, layer.drop)        # dropout and shortcut in the same pass
+    drop = layer.drop is not None and layer.drop.rate > 0.0
     if layer.batch_normalization:
         u = _ConvBlock.apply(x, layer.kernel, None, None, layer, None)            # linear, no bias (layers.py:61)
-        return batch_norm_act(layer.bn, u, layer.act_code, shortcut)
+        y = batch_norm_act(layer.bn, u, layer.act_code, None if drop else shortcut)
+    elif drop:
+        y = _ConvBlock.apply(x, layer.kernel, layer.bias, None, layer, link if shortcut is None else None)
+    if drop:
+        return dropout(y, layer.drop.rate, layer.drop.draw(), shortcut)
+    if layer.batch_normalization:
+        return y
     return _ConvBlock.apply(x, layer.kernel, layer.bias, shortcut, layer, link)
 
 
@@ -469,3 +482,168 @@ class _SppConcat(torch.autograd.Function):
 def spp_concat(x):
     _lib.require_gpu(x)
     return _SppConcat.apply(x)
+
+
+# ---- group normalisation and dropout ------------------------------------------------------------
+def _activation_code(activation, who):
+    if not activation:
+        return _lib.ACT_NONE
+    if activation not in _lib.ACT_CODES:
+        raise ValueError("%s: activation %r (\"leaky\", \"mish\" or None)" % (who, activation))
+    return _lib.ACT_CODES[activation]
+
+
+def _check_rate(rate, who):
+    rate = float(rate)
+    if not 0.0 <= rate < 1.0:
+        raise ValueError("%s: dropout rate %g (0 <= rate < 1)" % (who, rate))
+    return rate
+
+
+def _check_dropout(x, rate, state, who):
+    rate = _check_rate(rate, who)
+    if rate > 0.0:
+        if not torch.is_tensor(state) or state.dtype != torch.int64 or tuple(state.shape) != (2,) or not state.is_contiguous():
+            raise ValueError("%s: state must be an int64 tensor (seed, call number)" % who)
+        if state.device != x.device:
+            raise ValueError("%s: state on %s, input on %s" % (who, state.device, x.device))
+    return rate
+
+
+def _check_shortcut(x, shortcut, who):
+    if shortcut is not None and (shortcut.shape != x.shape or shortcut.device != x.device):
+        raise ValueError("%s: shortcut %s on %s does not match %s on %s" % (who, tuple(shortcut.shape), shortcut.device,
+                                                                              tuple(x.shape), x.device))
+
+
+def _records(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _group_norm_forward(x, gamma, beta, shortcut, groups, act, epsilon, rate, state):
+    """(y, contiguous x, gamma and beta as the kernels take them, statistics)"""
+    x = x.contiguous()
+    b, c = x.shape[0], x.shape[-1]
+    gamma, beta = gamma.float().contiguous(), beta.float().contiguous()
+    sc = None if shortcut is None else shortcut.to(x.dtype).contiguous()
+    y = torch.empty_like(x)
+    stats = torch.empty((b, groups, 2), device=x.device, dtype=torch.float32)
+    if x.numel():
+        pix = x.numel() // (b * c)
+        nb = _lib.lib().ymx_group_norm_workspace_bytes(b, pix, c, groups)
+        ws = torch.empty((nb,), device=x.device, dtype=torch.uint8)
+        _lib.launch("ymx_group_norm_forward", x, _lib.ptr(x), _lib.ptr(gamma), _lib.ptr(beta), _lib.ptr(sc), _lib.ptr(y), _lib.ptr(stats),
+                    b, pix, c, groups, act, epsilon, _lib.dtype_code(x.dtype), rate, _lib.ptr(state), _lib.ptr(ws), nb)
+    return y, x, gamma, beta, stats
+
+
+class _GroupNormAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gamma, beta, shortcut, groups, act, epsilon, rate, state):
+        y, xc, ga, be, stats = _group_norm_forward(x, gamma, beta, shortcut, groups, act, epsilon, rate, state)
+        ctx.save_for_backward(xc, ga, be, stats, state)
+        ctx.args = (groups, act, rate)
+        ctx.dtypes = (gamma.dtype, beta.dtype, None if shortcut is None else shortcut.dtype)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, gamma, beta, stats, state = ctx.saved_tensors
+        groups, act, rate = ctx.args
+        b, c = x.shape[0], x.shape[-1]
+        dy = dy.to(x.dtype).contiguous()
+        dx = dgamma = dbeta = None
+        if any(ctx.needs_input_grad[:3]):
+            dx = torch.empty_like(x)
+            if x.numel():
+                dgamma, dbeta = (torch.empty((c,), device=x.device, dtype=torch.float32) for _ in range(2))
+                pix = x.numel() // (b * c)
+                nb = _lib.lib().ymx_group_norm_workspace_bytes(b, pix, c, groups)
+                ws = torch.empty((nb,), device=x.device, dtype=torch.uint8)
+                _lib.launch("ymx_group_norm_backward", x, _lib.ptr(x), _lib.ptr(dy), _lib.ptr(gamma), _lib.ptr(beta), _lib.ptr(stats), _lib.ptr(dx),
+                            _lib.ptr(dgamma), _lib.ptr(dbeta), b, pix, c, groups, act, _lib.dtype_code(x.dtype), rate,
+                            _lib.ptr(state), _lib.ptr(ws), nb)
+            else:
+                dgamma, dbeta = (torch.zeros((c,), device=x.device, dtype=torch.float32) for _ in range(2))
+            dgamma = dgamma.to(ctx.dtypes[0]) if ctx.needs_input_grad[1] else None
+            dbeta = dbeta.to(ctx.dtypes[1]) if ctx.needs_input_grad[2] else None
+        dsc = dy.to(ctx.dtypes[2]) if ctx.needs_input_grad[3] else None
+        return (dx if ctx.needs_input_grad[0] else None), dgamma, dbeta, dsc, None, None, None, None, None
+
+
+def group_norm_act(x, gamma, beta, groups, activation=None, shortcut=None, epsilon=1e-3, rate=0.0, state=None):
+    """``dropout(act(gamma * (x - mean) / sqrt(var + epsilon) + beta)) + shortcut`` over x [B, ..., C] (a
+    GPU tensor, bfloat16 or float32), the statistics of every (sample, group of C / groups
+    neighbouring channels) over its pixels.  gamma, beta: [C].  activation: "mish", "leaky" or None.
+    rate, state: dropout before the shortcut, see ``dropout``.  Differentiable in x, gamma, beta and
+    shortcut (once; the gradients of gamma and beta are summed in fp32); with gradients disabled, or if
+    none of them requires one, no graph is recorded."""
+    _lib.require_gpu(x, gamma, beta, shortcut)
+    code = _activation_code(activation, "group_norm_act")
+    if x.dim() < 2:
+        raise ValueError("group_norm_act: expected [B, ..., C], got shape %s" % (tuple(x.shape),))
+    _lib.dtype_code(x.dtype)
+    c, groups = x.shape[-1], int(groups)
+    if groups <= 0 or c % groups:
+        raise ValueError("group_norm_act: %d channels do not split into %d groups" % (c, groups))
+    for name, t in (("gamma", gamma), ("beta", beta)):
+        if tuple(t.shape) != (c,) or t.device != x.device:
+            raise ValueError("group_norm_act: %s %s on %s, expected (%d,) on %s" % (name, tuple(t.shape), t.device, c, x.device))
+    if not epsilon > 0:
+        raise ValueError("group_norm_act: epsilon %g" % epsilon)
+    _check_shortcut(x, shortcut, "group_norm_act")
+    rate = _check_dropout(x, rate, state, "group_norm_act")
+    state = state if rate > 0.0 else None
+    if _records(x, gamma, beta, shortcut):
+        return _GroupNormAct.apply(x, gamma, beta, shortcut, groups, code, float(epsilon), rate, state)
+    with torch.no_grad():
+        return _group_norm_forward(x, gamma, beta, shortcut, groups, code, float(epsilon), rate, state)[0]
+
+
+def _dropout_launch(x, shortcut, rate, state):
+    x = x.contiguous()
+    y = torch.empty_like(x)
+    sc = None if shortcut is None else shortcut.to(x.dtype).contiguous()
+    _lib.launch("ymx_dropout", x, _lib.ptr(x), _lib.ptr(sc), _lib.ptr(y), x.numel(), _lib.dtype_code(x.dtype), rate, _lib.ptr(state))
+    return y
+
+
+class _DropoutFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, shortcut, rate, state):
+        ctx.save_for_backward(state)
+        ctx.rate = rate
+        ctx.x_dtype = x.dtype
+        ctx.shortcut_dtype = None if shortcut is None else shortcut.dtype
+        return _dropout_launch(x, shortcut, rate, state)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        (state,) = ctx.saved_tensors
+        dy = dy.to(ctx.x_dtype)
+        dx = _dropout_launch(dy, None, ctx.rate, state) if (ctx.needs_input_grad[0] and dy.numel()) else \
+            (torch.empty_like(dy) if ctx.needs_input_grad[0] else None)
+        return dx, (dy.to(ctx.shortcut_dtype) if ctx.needs_input_grad[1] else None), None, None
+
+
+def dropout(x, rate, state, shortcut=None):
+    """``keep * x / (1 - rate) + shortcut`` over a GPU tensor (bfloat16 or float32) of any shape.
+    state: int64 tensor (seed, call number) on x's device; element i (row-major) is kept iff word
+    i % 4 of Philox4x32-10 with counter (i // 4, call) and key seed is >= floor(rate * 2**32), so
+    equal states give equal masks and the backward pass computes the mask again from the state: leave
+    its values alone until then (autograd notices an in-place change), and give every call of a step
+    another call number (layers.Dropout does).  Differentiable in x and shortcut."""
+    _lib.require_gpu(x, shortcut)
+    _lib.dtype_code(x.dtype)
+    _check_shortcut(x, shortcut, "dropout")
+    rate = _check_dropout(x, rate, state, "dropout")
+    if rate == 0.0:
+        return x if shortcut is None else x + shortcut.to(x.dtype)
+    if x.numel() == 0:
+        return x.clone()
+    if _records(x, shortcut):
+        return _DropoutFn.apply(x, shortcut, rate, state)
+    with torch.no_grad():
+        return _dropout_launch(x, shortcut, rate, state)
