@@ -28,7 +28,8 @@ extern "C" {
 
 #define YMX_VERSION 100
 
-enum { YMX_F32 = 0, YMX_BF16 = 1, YMX_U8 = 2 /* image entry points only */ };
+enum { YMX_F32 = 0, YMX_BF16 = 1, YMX_U8 = 2 /* image entry points only */,
+       YMX_F8E4M3 = 3 /* block-scaled 8-bit floating point: packed kernels and quantised maps */ };
 enum { YMX_ACT_NONE = 0, YMX_ACT_LEAKY = 1, YMX_ACT_MISH = 2 };
 enum {
     YMX_OK = 0,
@@ -115,6 +116,24 @@ int ymx_conv2d_fused_ex(const void *x, const void *w, const void *scale, const v
                         const void *residual, void *y, int B, int H, int W, int Cin, int Cout,
                         int k, int stride, int act, int dtype, int x_dtype, int out_dtype,
                         int x_ld, int res_ld, int y_ld, void *stream);
+
+/* ---- convolution blocks in 8-bit floating point (no counterpart in the reference) -------------
+ * The convolution entry points above with dtype = x_dtype = YMX_F8E4M3: x is a quantised map, w a
+ * kernel packed by ymx_pack_weights(..., YMX_F8E4M3), k is 1 or 3, Cin a multiple of 16; scale,
+ * shift and act as above, y and residual have the type out_dtype (fp32 or bf16; both 0-dense or
+ * with pixel strides), products are accumulated in fp32.  ymx_packed_weight_bytes gives the size.
+ *
+ * Values are e4m3 numbers times 2^k, one k for each block of up to 128 input channels: of one
+ * pixel of a map, of one tap and one output channel of a kernel.  k is the smallest integer
+ * >= -126 with |largest finite value of the block| <= 448 * 2^k (0 for a block of zeros); values
+ * are rounded to nearest even; NaN and infinities become NaN.
+ *
+ * A quantised map of n_pix pixels is one buffer of ymx_quantized_bytes(n_pix, C) bytes: the e4m3
+ * bytes [n_pix][C], padding to a multiple of 256 bytes, then [n_pix][S] exponent bytes k + 127, of
+ * which the first ceil(C / 128) are set, S = that number rounded up to 4.  x of
+ * ymx_quantize_blocks is fp32 or bf16 with pixel stride x_ld (elements, a multiple of 8; 0 = dense). */
+size_t ymx_quantized_bytes(long long n_pix, int C);
+int ymx_quantize_blocks(const void *x, void *q, long long n_pix, int C, int dtype, int x_ld, void *stream);
 
 /* ---- upsample + concat ------------------------------------------------------
  * Replaces Upsample.call (layers.py:37-39: tf.image.resize bilinear x2, half-pixel

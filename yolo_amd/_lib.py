@@ -12,7 +12,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # one next to this file
 LIB_PATH = os.environ.get("YMX_LIBRARY") or os.path.join(_HERE, "libymx.so")
 
-F32, BF16 = 0, 1
+F32, BF16, F8E4M3 = 0, 1, 3
 ACT_NONE, ACT_LEAKY, ACT_MISH = 0, 1, 2
 ACT_CODES = {None: ACT_NONE, "leaky": ACT_LEAKY, "mish": ACT_MISH}
 
@@ -45,6 +45,8 @@ SIGNATURES = {
     "ymx_bn_act_forward": (_i, [_vp, _vp, _vp, _vp, _vp, _ll, _i, _i, _i, _vp]),
     "ymx_bn_act_backward": (_i, [_vp, _vp, _vp, _vp, _vp, _ll, _i, _i, _i, _vp, _vp, _sz, _vp]),
     "ymx_bn_backward_apply": (_i, [_vp] * 6 + [_ll, _i, _i, _vp]),
+    "ymx_quantized_bytes": (_sz, [_ll, _i]),
+    "ymx_quantize_blocks": (_i, [_vp, _vp, _ll, _i, _i, _i, _vp]),
     "ymx_group_norm_workspace_bytes": (_sz, [_ll, _ll, _i, _i]),
     "ymx_group_norm_forward": (_i, [_vp] * 6 + [_ll, _ll, _i, _i, _i, _f, _i, _d, _vp, _vp, _sz, _vp]),
     "ymx_group_norm_backward": (_i, [_vp] * 8 + [_ll, _ll, _i, _i, _i, _i, _d, _vp, _vp, _sz, _vp]),

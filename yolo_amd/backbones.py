@@ -182,7 +182,7 @@ class CSPDarknet53(nn.Module):
         c1 = flat_convs(main)[-1].filters
         c2 = flat_convs(skip)[-1].filters
         probe = flat_convs(main)[-1]
-        dt = probe.compute_dtype or x_main.dtype
+        dt = probe.map_dtype(x_main)
         b, h, w = x_main.shape[0], x_main.shape[1], x_main.shape[2]
         if _training.enabled():
             # recorded for back-propagation: the branches' gradients are the two channel slices of the concat's

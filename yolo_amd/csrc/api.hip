@@ -95,7 +95,7 @@ static int conv_impl(const void *x, const void *w, const void *scale, const void
     if (stride != 1 && stride != 2) return fail(YMX_EUNSUPPORTED, "conv2d: stride %d (1 or 2)", stride);
     if (act != YMX_ACT_NONE && act != YMX_ACT_LEAKY && act != YMX_ACT_MISH)
         return fail(YMX_EARG, "conv2d: activation code %d", act);
-    if (dtype != YMX_F32 && dtype != YMX_BF16) return fail(YMX_EARG, "conv2d: dtype %d", dtype);
+    if (dtype != YMX_F32 && dtype != YMX_BF16 && dtype != YMX_F8E4M3) return fail(YMX_EARG, "conv2d: dtype %d", dtype);
     ConvArgs a;
     memset(&a, 0, sizeof(a));
     a.x = x; a.w = w; a.res = residual; a.y = y;
@@ -137,6 +137,20 @@ static int conv_impl(const void *x, const void *w, const void *scale, const void
     set_fastdiv((unsigned)k, a.k_m, a.k_s);
     a.act = act;
     a.dtype = dtype; a.x_dtype = x_dtype; a.out_dtype = out_dtype;
+    if (dtype == YMX_F8E4M3) {
+        // x is a quantised map (ymx_quantize_blocks), the residual has the output's type
+        if (x_dtype != YMX_F8E4M3) return fail(YMX_EARG, "conv2d: an 8-bit kernel takes a quantised map");
+        if (out_dtype != YMX_F32 && out_dtype != YMX_BF16) return fail(YMX_EARG, "conv2d: output dtype %d", out_dtype);
+        if (z || d2s) return fail(YMX_EUNSUPPORTED, "conv2d: 8-bit kernels are for inference");
+        if (Cin % 16 || (k != 1 && k != 3)) return fail(YMX_EUNSUPPORTED, "conv2d: 8-bit kernels take input channels in multiples of 16 and 1x1 or 3x3 windows (%d, %d)", Cin, k);
+        if (a.x_ld != Cin) return fail(YMX_EARG, "conv2d: a quantised map is dense");
+        if (!aligned16(x) || !aligned16(w)) return fail(YMX_EARG, "conv2d: x and w must be 16-byte aligned");
+        const uintptr_t mis = out_dtype == YMX_BF16 ? 1 : 3;
+        if (((uintptr_t)y & mis) || ((uintptr_t)residual & mis)) return fail(YMX_EARG, "conv2d: y/residual not aligned to their elements");
+        if (label) { *label = "f8"; return YMX_OK; }
+        return launch_conv_f8(a, (long long)B * H * W, s);
+    }
+    if (x_dtype == YMX_F8E4M3) return fail(YMX_EARG, "conv2d: a quantised map needs an 8-bit kernel");
     if (z) {
         if (dtype != YMX_BF16 || out_dtype != YMX_BF16 || act == YMX_ACT_NONE || a.y_ld != Cout || !aligned16(z))
             return fail(YMX_EARG, "conv2d: the second output needs bf16, an activation, dense y and a 16-byte aligned z");
@@ -279,6 +293,7 @@ const char *ymx_last_error(void) { return g_err.c_str(); }
 
 size_t ymx_packed_weight_bytes(int k, int Cin, int Cout, int dtype) {
     if (k <= 0 || Cin <= 0 || Cout <= 0) return 0;
+    if (dtype == YMX_F8E4M3) return Cin % 16 || (k != 1 && k != 3) ? 0 : packed_f8_bytes(k, Cin, Cout);
     if (!conv_uses_mfma(Cin, dtype)) return (size_t)k * k * Cin * Cout * 4;
     return (size_t)packed_rows(Cout) * packed_kw(k, Cin) * (dtype == YMX_BF16 ? 2 : 4);
 }
@@ -286,8 +301,27 @@ size_t ymx_packed_weight_bytes(int k, int Cin, int Cout, int dtype) {
 int ymx_pack_weights(const float *w_hwio, void *w_packed, int k, int Cin, int Cout, int dtype, void *stream) {
     if (!w_hwio || !w_packed) return fail(YMX_EARG, "pack_weights: null pointer");
     if (k <= 0 || Cin <= 0 || Cout <= 0) return fail(YMX_EARG, "pack_weights: non-positive size");
+    if (dtype == YMX_F8E4M3) {
+        if (Cin % 16 || (k != 1 && k != 3)) return fail(YMX_EUNSUPPORTED, "pack_weights: 8-bit kernels take input channels in multiples of 16 and 1x1 or 3x3 windows (%d, %d)", Cin, k);
+        if (!aligned16(w_packed)) return fail(YMX_EARG, "pack_weights: the packed kernel must be 16-byte aligned");
+        return launch_pack_f8(w_hwio, w_packed, k, Cin, Cout, (hipStream_t)stream);
+    }
     if (dtype != YMX_F32 && dtype != YMX_BF16) return fail(YMX_EARG, "pack_weights: dtype %d", dtype);
     return launch_pack_weights(w_hwio, w_packed, k, Cin, Cout, dtype, (hipStream_t)stream);
+}
+
+size_t ymx_quantized_bytes(long long n_pix, int C) { return (n_pix > 0 && C > 0) ? quant_bytes(n_pix, C) : 0; }
+
+int ymx_quantize_blocks(const void *x, void *q, long long n_pix, int C, int dtype, int x_ld, void *stream) {
+    if (!x || !q) return fail(YMX_EARG, "quantize_blocks: null pointer");
+    if (n_pix <= 0 || C <= 0) return fail(YMX_EARG, "quantize_blocks: non-positive size");
+    if (dtype != YMX_F32 && dtype != YMX_BF16) return fail(YMX_EARG, "quantize_blocks: dtype %d", dtype);
+    if (C % 16) return fail(YMX_EUNSUPPORTED, "quantize_blocks: %d channels (multiples of 16)", C);
+    const int ld = x_ld > 0 ? x_ld : C;
+    if (ld < C || ld % 8) return fail(YMX_EARG, "quantize_blocks: pixel stride %d (at least C, a multiple of 8)", ld);
+    if (!aligned16(x) || !aligned16(q)) return fail(YMX_EARG, "quantize_blocks: 16-byte alignment");
+    if (n_pix > 0x7fffffffLL) return fail(YMX_EUNSUPPORTED, "quantize_blocks: more than 2^31 pixels");
+    return launch_quantize(x, ld, q, n_pix, C, dtype, (hipStream_t)stream);
 }
 
 int ymx_pack_weights_dgrad(const float *w_hwio, void *w_packed, int k, int Cin, int Cout, int dz_channels, int dtype,
@@ -333,7 +367,7 @@ int ymx_conv2d_fused(const void *x, const void *w, const void *scale, const void
 int ymx_conv2d_fused_ex(const void *x, const void *w, const void *scale, const void *shift, const void *residual,
                         void *y, int B, int H, int W, int Cin, int Cout, int k, int stride, int act, int dtype,
                         int x_dtype, int out_dtype, int x_ld, int res_ld, int y_ld, void *stream) {
-    if ((x_dtype != YMX_F32 && x_dtype != YMX_BF16) || (out_dtype != YMX_F32 && out_dtype != YMX_BF16))
+    if ((x_dtype != YMX_F32 && x_dtype != YMX_BF16 && x_dtype != YMX_F8E4M3) || (out_dtype != YMX_F32 && out_dtype != YMX_BF16))
         return fail(YMX_EARG, "conv2d: x_dtype %d / out_dtype %d", x_dtype, out_dtype);
     return conv_impl(x, w, scale, shift, residual, y, B, H, W, Cin, Cout, k, stride, act, dtype, x_dtype, out_dtype,
                      x_ld, res_ld, y_ld, (hipStream_t)stream);

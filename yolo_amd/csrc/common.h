@@ -267,6 +267,12 @@ int launch_conv_resblock(const void *x, int x_ld, const void *w1, const float *s
 int launch_conv_resblock128(const void *x, int x_ld, const void *w1, const float *scale1, const float *shift1, const void *w2,
                             const float *scale2, const float *shift2, void *y, int y_ld, int B, int H, int W, int act, hipStream_t s);
 int launch_conv_direct(const ConvArgs &a, hipStream_t s);
+// 8-bit block-scaled convolutions (conv_blockscaled.hip)
+size_t quant_bytes(long long n_pix, int C);
+int launch_quantize(const void *x, int x_ld, void *q, long long n_pix, int C, int dtype, hipStream_t s);
+size_t packed_f8_bytes(int k, int Cin, int Cout);
+int launch_pack_f8(const float *w_hwio, void *packed, int k, int Cin, int Cout, hipStream_t s);
+int launch_conv_f8(const ConvArgs &a, long long in_pix, hipStream_t s);
 int launch_pack_weights(const float *w_hwio, void *w_packed, int k, int Cin, int Cout, int dtype,
                         hipStream_t s, int src_cout = 0);
 int launch_pack_weights_pair(const float *w_hwio, void *w_fwd, void *w_bwd, int k, int Cin, int Cout, int dz_channels, int stride,

@@ -39,6 +39,56 @@ def affine_act(x, scale, shift, act):
     return y
 
 
+class BlockQuantized(object):
+    """A map [..., C] held as e4m3 numbers with one power of two for each block of 128 channels of a
+    pixel: what an 8-bit YOLOConv multiplies (quantize_blocks makes it; YOLOConv does so itself
+    for a plain tensor).  buffer: one uint8 tensor laid out as ymx_quantize_blocks documents;
+    values / exponents: views of it (float8_e4m3fn [..., C]; uint8 [..., ceil(C / 128)], k + 127)."""
+
+    def __init__(self, buffer, shape):
+        self.buffer = buffer
+        self.shape = torch.Size(shape)
+
+    @property
+    def device(self):
+        return self.buffer.device
+
+    @property
+    def values(self):
+        return self.buffer[:self.shape.numel()].view(torch.float8_e4m3fn).view(self.shape)
+
+    @property
+    def exponents(self):
+        n = self.shape.numel()
+        nb = -(-self.shape[-1] // 128)
+        tail = self.buffer[-(-n // 256) * 256:]
+        return tail.view(self.shape[:-1] + (-(-nb // 4) * 4,))[..., :nb]
+
+    def dequantize(self, dtype=torch.float32):
+        """The values the bytes stand for."""
+        k = self.exponents.to(torch.int32) - 127
+        k = k.repeat_interleave(128, dim=-1)[..., :self.shape[-1]]
+        return torch.ldexp(self.values.float(), k).to(dtype)
+
+
+def quantize_blocks(x):
+    """BlockQuantized of a GPU tensor [..., C], bfloat16 or float32, C a multiple of 16: for each block
+    of up to 128 channels of a pixel the smallest k (>= -126) with |largest finite value| <= 448 * 2**k, values
+    rounded to the nearest e4m3 number times 2**k; NaN and infinities become NaN."""
+    _lib.require_gpu(x)
+    code = _lib.dtype_code(x.dtype)
+    c = x.shape[-1] if x.dim() else 0
+    if c == 0 or c % 16 or x.numel() == 0:
+        raise ValueError("quantize_blocks: expected a non-empty [..., C] with C a multiple of 16, got shape %s" % (tuple(x.shape),))
+    x = x.contiguous()
+    if x.data_ptr() % 16:
+        x = x.clone()
+    pix = x.numel() // c
+    buf = torch.empty((_lib.lib().ymx_quantized_bytes(pix, c),), device=x.device, dtype=torch.uint8)
+    _lib.launch("ymx_quantize_blocks", x, _lib.ptr(x), _lib.ptr(buf), pix, c, code, 0)
+    return BlockQuantized(buf, x.shape)
+
+
 class BatchNormalization(nn.Module):
     """Batch norm over the last axis (layers.py:4-15).
 
@@ -227,7 +277,10 @@ class YOLOConv(nn.Module):
     this class (or pass in_channels= / call build()).
 
     Extra keyword arguments: name (kept), dtype (torch.float32 or torch.bfloat16: the
-    compute type; default = the input's type), in_channels, groupNormalization (number of
+    compute type; default = the input's type; torch.float8_e4m3fn: products of 8-bit numbers with
+    a power of two for each block of 128 input channels, inference only, 1x1 and 3x3 windows, maps
+    stored in bfloat16 between the layers; a layer whose input channels are no multiple of 16, the
+    first one, computes in bfloat16), in_channels, groupNormalization (number of
     groups: GroupNormalization in the place of batch normalisation), dropout (rate, after the
     activation and before the shortcut, while back-propagation is recorded) and dropout_seed.
     """
@@ -253,6 +306,8 @@ class YOLOConv(nn.Module):
         if groups < 0 or (self.group_normalization and self.batch_normalization):
             raise ValueError("YOLOConv: groupNormalization is a number of groups and excludes batchNormalization")
         self.normalized = self.batch_normalization or self.group_normalization       # linear convolution without bias
+        if self.compute_dtype == torch.float8_e4m3fn and self.kernel_size not in (1, 3):
+            raise ValueError("YOLOConv: 8-bit layers have 1x1 or 3x3 windows, got %d" % self.kernel_size)
         self.act_fn = None
         if activation:
             if callable(activation):
@@ -312,7 +367,7 @@ class YOLOConv(nn.Module):
         if hit is not None and hit[0] == key:
             return hit[1]
         _lib.require_gpu(self.kernel)
-        code = _lib.dtype_code(dtype)
+        code = _lib.F8E4M3 if dtype == torch.float8_e4m3fn else _lib.dtype_code(dtype)
         k, cin, cout = self.kernel_size, self.in_channels, self.filters
         nbytes = _lib.lib().ymx_packed_weight_bytes(k, cin, cout, code)
         wp = torch.empty(nbytes, dtype=torch.uint8, device=dev)
@@ -362,6 +417,52 @@ class YOLOConv(nn.Module):
         self._packed["train"] = (key, entry)
         return entry
 
+    def is_8bit(self):
+        return self.compute_dtype == torch.float8_e4m3fn and self.in_channels % 16 == 0
+
+    def map_dtype(self, x):
+        """Element type of the layer's output map for the input x."""
+        if self.compute_dtype == torch.float8_e4m3fn:
+            return torch.bfloat16
+        return self.compute_dtype or x.dtype
+
+    def _forward_8bit(self, x, residual, out_dtype, out, act_code):
+        q = x if isinstance(x, BlockQuantized) else quantize_blocks(x)
+        b, h, w, cin = q.shape
+        k, cout = self.kernel_size, self.filters
+        oh, ow = self.output_hw(h, w)
+        odt = out_dtype or torch.bfloat16
+        wp, scale, shift, _ = self.packed(torch.float8_e4m3fn)
+        y_ld = 0
+        if out is not None:
+            y_ld = self._check_out(out, b, oh, ow, odt, q.device)
+            y = out
+        else:
+            y = torch.empty((b, oh, ow, cout), device=q.device, dtype=odt)
+        if residual is not None:
+            residual = _as_nhwc(residual)
+            if residual.shape != y.shape:
+                raise ValueError("YOLOConv: residual shape %s != output shape %s" % (tuple(residual.shape), tuple(y.shape)))
+        fused = residual if self.act_fn is None else None
+        if fused is not None and fused.dtype != odt:
+            fused = fused.to(odt)
+        _lib.launch("ymx_conv2d_fused_ex", q, _lib.ptr(q.buffer), _lib.ptr(wp), _lib.ptr(scale), _lib.ptr(shift), _lib.ptr(fused),
+                    _lib.ptr(y), b, h, w, cin, cout, k, 2 if self.downsample else 1, act_code, _lib.F8E4M3, _lib.F8E4M3,
+                    _lib.dtype_code(odt), 0, 0, y_ld)
+        if self.act_fn is not None:
+            y = self.act_fn(y)
+            if residual is not None:
+                y = residual + y
+        return y
+
+    def _check_out(self, out, b, oh, ow, odt, device):
+        if self.act_fn is not None:
+            raise ValueError("YOLOConv: out= is not supported with a callable activation")
+        if (tuple(out.shape) != (b, oh, ow, self.filters) or out.dtype != odt or out.device != device or out.stride(3) != 1 or
+                out.stride(1) != ow * out.stride(2) or out.stride(0) != oh * ow * out.stride(2)):
+            raise ValueError("YOLOConv: out must be a [%d,%d,%d,%d] %s view with dense pixels" % (b, oh, ow, self.filters, odt))
+        return out.stride(2)
+
     # -- geometry ---------------------------------------------------------------
     def output_hw(self, h, w):
         if not self.downsample:
@@ -375,7 +476,10 @@ class YOLOConv(nn.Module):
         activation inside the kernel; out_dtype overrides the output element type; out, if
         given, receives the result: a [B,H',W',Cout] view whose pixels may be spaced wider than
         Cout (a channel slice of a larger NHWC buffer: how a concat is written in place)."""
-        x = _as_nhwc(x)
+        if not isinstance(x, BlockQuantized):
+            x = _as_nhwc(x)
+        elif len(x.shape) != 4 or self.compute_dtype != torch.float8_e4m3fn or _training.enabled():
+            raise ValueError("YOLOConv: a quantised map [B,H,W,C] is for inference with dtype=torch.float8_e4m3fn")
         if self.in_channels is None:
             self.build(x.shape[-1])
             self.to(x.device)
@@ -387,12 +491,14 @@ class YOLOConv(nn.Module):
                 raise ValueError("YOLOConv: out= is not supported while back-propagation is recorded")
             y = _training.conv_block(self, x, residual, _grad_link)
             return y if out_dtype in (None, y.dtype) else y.to(out_dtype)
-        cdt = self.compute_dtype or x.dtype
         if self.group_normalization and not _linear:
             y = self.gn.apply_act(self.forward(x, _linear=True), self.act_code, residual, training=False)
             y = y if out_dtype in (None, y.dtype) else y.to(out_dtype)
             return y if out is None else out.copy_(y)
         act_code = _lib.ACT_NONE if _linear else self.act_code
+        if self.is_8bit():
+            return self._forward_8bit(x, residual, out_dtype, out, act_code)
+        cdt = self.map_dtype(x)
         code = _lib.dtype_code(cdt)
         k, cin, cout = self.kernel_size, self.in_channels, self.filters
         mfma = (cin % 8 == 0) if code == _lib.BF16 else (cin % 4 == 0)
@@ -404,12 +510,7 @@ class YOLOConv(nn.Module):
         oh, ow = self.output_hw(h, w)
         y_ld = 0
         if out is not None:
-            if self.act_fn is not None:
-                raise ValueError("YOLOConv: out= is not supported with a callable activation")
-            if (tuple(out.shape) != (b, oh, ow, cout) or out.dtype != odt or out.device != x.device or out.stride(3) != 1 or
-                    out.stride(1) != ow * out.stride(2) or out.stride(0) != oh * ow * out.stride(2)):
-                raise ValueError("YOLOConv: out must be a [%d,%d,%d,%d] %s view with dense pixels" % (b, oh, ow, cout, odt))
-            y, y_ld = out, out.stride(2)
+            y, y_ld = out, self._check_out(out, b, oh, ow, odt, x.device)
         else:
             y = _empty_like_nhwc(x, cout, oh, ow, dtype=odt)
         fuse_res = residual is not None and self.act_fn is None
