@@ -80,9 +80,8 @@ __device__ __forceinline__ float mish_f(float x) {
     const float n = e * (e + 2.0f);
     return x * (n * __builtin_amdgcn_rcpf(n + 2.0f));
 }
-// Two values at once: the multiplies and adds become packed fp32 instructions (v_pk_mul_f32,
-// v_pk_add_f32: two IEEE-exact results per issue slot), the exponential and the reciprocal
-// stay scalar.  Bit-identical to mish_f on each element.
+// Two values at once (the library is built without packed fp32 instructions, so a pair is two
+// scalar operations).  Bit-identical to mish_f on each element.
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f32x2_t mish2_f(f32x2_t x) {
 #pragma clang fp contract(off)
@@ -125,7 +124,7 @@ template <int ACT> __device__ __forceinline__ float act_grad_c(float z) {
     if constexpr (ACT == YMX_ACT_LEAKY) return z > 0.0f ? 1.0f : 0.1f;
     return 1.0f;
 }
-// act(v * sc + sh) for a pair (the affine step is one packed fma, as in affine_f).
+// act(v * sc + sh) for a pair (the affine step is one fma each, as in affine_f).
 __device__ __forceinline__ f32x2_t affine2(f32x2_t v, f32x2_t sc, f32x2_t sh) { return __builtin_elementwise_fma(v, sc, sh); }
 template <int ACT> __device__ __forceinline__ f32x2_t act2(f32x2_t x) {
     if constexpr (ACT == YMX_ACT_MISH) return mish2_f(x);

@@ -254,8 +254,7 @@ conv_first_rows_kernel(const ConvArgs a, const int chunks_per_row, const int nch
             d0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a2[0], b2, d0, 0, 0, 0);
             d1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a2[1], b2, d1, 0, 0, 0);
             if (ow < a.OW) {
-                // two values per step: the activation's multiplies and adds are packed fp32
-                // instructions (this layer is bound by its 354 M Mish evaluations, not by memory)
+                // two values per step (this layer is bound by its 354 M Mish evaluations, not by memory)
                 float v[8];
 #pragma unroll
                 for (int r = 0; r < 4; r += 2) {

@@ -27,7 +27,7 @@ typedef __attribute__((ext_vector_type(4))) unsigned int epi_u32x4_t;
 typedef __bf16 epi_bf16x2_t __attribute__((ext_vector_type(2)));
 
 // Two IEEE additions (no contraction with whatever produced the operands) and one packed
-// round-to-nearest-even conversion of a pair: v_pk_add_f32 and v_cvt_pk_bf16_f32.
+// round-to-nearest-even conversion of a pair (v_cvt_pk_bf16_f32).
 __device__ __forceinline__ f32x2_t epi_add2(f32x2_t a, f32x2_t b) {
 #pragma clang fp contract(off)
     return a + b;
@@ -155,8 +155,7 @@ __device__ __forceinline__ void epi_run(const ConvArgs &a, f32x4_t (&acc)[NI][NJ
 #pragma unroll
                 for (int r = 0; r < 8; ++r) v[r] = nxt[r];
                 if (n + 1 < NPASS) read_row(px + PPI, nxt);     // next pass's row is in flight during this one's math
-                // pairs of neighbouring channels stay pairs from the affine step to the packed
-                // conversion, so that no instruction is spent on re-pairing them
+                // pairs of neighbouring channels stay pairs from the affine step to the packed conversion
                 f32x2_t o[4];
                 uint32_t zq[4];
 #pragma unroll
