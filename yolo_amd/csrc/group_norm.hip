@@ -145,20 +145,25 @@ __global__ void __launch_bounds__(1024) gn_stats_join_kernel(const GnArgs a, con
     if (threadIdx.x == 0) ((float2 *)a.stats)[blockIdx.x] = float2{mean, 1.0f / sqrtf(var + a.eps)};
 }
 
-// The numbers of a thread's V channels: h = (x - mean) r, t = gamma h + beta.
+// The numbers of a thread's V channels: d = x - mean first (exact next to the mean, so that a map without
+// spread gives beta itself), then h = d r and t = d (gamma r) + beta.
 template <int V> struct GnChannels {
-    float mean[V], r[V], ga[V], be[V];
-    __device__ __forceinline__ GnChannels(const GnArgs &a, int b, int c0) {
+    float mean[V], r[V], ta[V], be[V];
+    __device__ __forceinline__ void set(int i, float m, float rstd, float gamma, float beta) {
+        mean[i] = m;
+        r[i] = rstd;
+        ta[i] = gamma * rstd;
+        be[i] = beta;
+    }
+    __device__ __forceinline__ void load(const GnArgs &a, int b, int c0) {
         const float2 *__restrict__ st = (const float2 *)a.stats + (size_t)b * a.G;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const float2 m = st[(c0 + i) / a.D];
-            mean[i] = m.x;
-            r[i] = m.y;
-            ga[i] = a.gamma[c0 + i];
-            be[i] = a.beta[c0 + i];
+            set(i, m.x, m.y, a.gamma[c0 + i], a.beta[c0 + i]);
         }
     }
+    __device__ __forceinline__ float t(int i, float x) const { return __builtin_fmaf(x - mean[i], ta[i], be[i]); }
 };
 
 // Pass 2, forward.
@@ -167,7 +172,8 @@ __global__ void __launch_bounds__(256) gn_apply_kernel(const GnArgs a, const GnW
     const GnPos<V> g(a, w);
     if (!g.on) return;
     typedef vec_io<T, V> IO;
-    const GnChannels<V> ch(a, g.b, g.c0);
+    GnChannels<V> ch;
+    ch.load(a, g.b, g.c0);
     const size_t base = (size_t)g.b * a.P * a.C + g.c0;
     const T *__restrict__ x = (const T *)a.x + base, *__restrict__ res = (const T *)a.res + base;
     T *__restrict__ y = (T *)a.y + base;
@@ -189,8 +195,7 @@ __global__ void __launch_bounds__(256) gn_apply_kernel(const GnArgs a, const GnW
                    if constexpr (DROP) drop_keep<V>(drop, key, base + (size_t)p * a.C, keep);
 #pragma unroll
                    for (int i = 0; i < V; ++i) {
-                       const float h = (v[i] - ch.mean[i]) * ch.r[i];
-                       v[i] = act_c<ACT>(__builtin_fmaf(ch.ga[i], h, ch.be[i]));
+                       v[i] = act_c<ACT>(ch.t(i, v[i]));
                        if constexpr (DROP) v[i] = keep[i] ? v[i] * drop.keep_scale : 0.0f;
                    }
                    if (has_res) {
@@ -202,20 +207,31 @@ __global__ void __launch_bounds__(256) gn_apply_kernel(const GnArgs a, const GnW
                });
 }
 
-// dt and h of one vector of a map and its gradient.
+// dt of one vector of a map and its gradient.
 template <int V, int ACT, bool DROP>
 __device__ __forceinline__ void gn_dt(const GnChannels<V> &ch, const DropArgs &drop, const uint4 &key, unsigned long long i0,
-                                      const float (&x)[V], const float (&dy)[V], float (&dt)[V], float (&h)[V]) {
+                                      const float (&x)[V], const float (&dy)[V], float (&dt)[V]) {
     bool keep[V];
     if constexpr (DROP) drop_keep<V>(drop, key, i0, keep);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        h[i] = (x[i] - ch.mean[i]) * ch.r[i];
         float d = dy[i];
         if constexpr (DROP) d = keep[i] ? d * drop.keep_scale : 0.0f;
-        dt[i] = d * act_grad_c<ACT>(__builtin_fmaf(ch.ga[i], h[i], ch.be[i]));
+        dt[i] = d * act_grad_c<ACT>(ch.t(i, x[i]));
     }
 }
+
+// dx of V values: r (gamma dt - (m1 + h m2)) = ta dt + d b + c with the group's m1 = S1 / N, m2 = S2 / N.
+template <int V> struct GnGradient {
+    float b[V], c[V];
+    __device__ __forceinline__ void set(const GnChannels<V> &ch, int i, float m1, float m2) {
+        b[i] = -ch.r[i] * ch.r[i] * m2;
+        c[i] = -ch.r[i] * m1;
+    }
+    __device__ __forceinline__ float dx(const GnChannels<V> &ch, int i, float x, float dt) const {
+        return __builtin_fmaf(ch.ta[i], dt, __builtin_fmaf(x - ch.mean[i], b[i], c[i]));
+    }
+};
 
 // Pass 1, backward: part[(b nchunk + chunk) C + c] = (sum dt, sum dt h) of the chunk's pixels.
 template <typename T, int V, int ACT, bool DROP>
@@ -225,7 +241,8 @@ __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const GnArgs a, const 
     typedef vec_io<T, V> IO;
     const int W = w.cvb * V;
     if (g.on) {
-        const GnChannels<V> ch(a, g.b, g.c0);
+        GnChannels<V> ch;
+        ch.load(a, g.b, g.c0);
         const size_t base = (size_t)g.b * a.P * a.C + g.c0;
         const T *__restrict__ x = (const T *)a.x + base, *__restrict__ dy = (const T *)a.dy + base;
         const DropArgs drop = {a.state, a.threshold, a.keep_scale};
@@ -237,18 +254,18 @@ __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const GnArgs a, const 
         struct Row { typename IO::raw x, d; };
         gn_rows<2>(g.p, g.p1, w.R, [&](int p) { return Row{IO::load(x + (size_t)p * a.C), IO::load(dy + (size_t)p * a.C)}; },
                    [&](int p, const Row &q) {
-                       float v[V], d[V], dt[V], h[V];
+                       float v[V], d[V], dt[V];
                        IO::unpack(q.x, v);
                        IO::unpack(q.d, d);
-                       gn_dt<V, ACT, DROP>(ch, drop, key, base + (size_t)p * a.C, v, d, dt, h);
+                       gn_dt<V, ACT, DROP>(ch, drop, key, base + (size_t)p * a.C, v, d, dt);
 #pragma unroll
                        for (int i = 0; i < V; ++i) {
                            s1[i] += dt[i];
-                           s2[i] += dt[i] * h[i];
+                           s2[i] += dt[i] * (v[i] - ch.mean[i]);
                        }
                    });
 #pragma unroll
-        for (int i = 0; i < V; ++i) red[g.r * W + g.cv * V + i] = float2{s1[i], s2[i]};
+        for (int i = 0; i < V; ++i) red[g.r * W + g.cv * V + i] = float2{s1[i], s2[i] * ch.r[i]};
     }
     __syncthreads();
     for (int c = threadIdx.x; c < W && g.zb * W + c < a.C; c += 256) {
@@ -262,17 +279,18 @@ __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const GnArgs a, const 
     }
 }
 
-// Workgroups 0 .. B G - 1: gsum[b][g] = (S1, S2) / N.  The others, 32 channels each: dbeta and dgamma,
-// the B nchunk pairs of a channel added by 8 row lanes and those in order.
-__global__ void __launch_bounds__(256) gn_bwd_join_kernel(const GnArgs a, const GnWork w, const float2 *__restrict__ part,
-                                                          float2 *__restrict__ gsum) {
-    __shared__ float2 red[256];
-    if ((int)blockIdx.x < a.B * a.G) {
+// Workgroups 0 .. nsum - 1 (one per sample and group, or none): gsum[b][g] = (S1, S2) / N.  The others, 16
+// channels each: dbeta and dgamma, a channel's B nchunk pairs added by 64 row lanes (four chains each) and
+// those by a tree.
+__global__ void __launch_bounds__(1024) gn_bwd_join_kernel(const GnArgs a, const GnWork w, const float2 *__restrict__ part,
+                                                           float2 *__restrict__ gsum, int nsum) {
+    __shared__ float2 red[16 * 65];
+    if ((int)blockIdx.x < nsum) {
         const int b = blockIdx.x / a.G, g = blockIdx.x % a.G;
         const float2 *__restrict__ q = part + (size_t)b * w.nchunk * a.C + g * a.D;
         const int items = w.nchunk * a.D;
         float s1 = 0.0f, s2 = 0.0f;
-        for (int i = threadIdx.x; i < items; i += 256) {
+        for (int i = threadIdx.x; i < items; i += 1024) {
             const int k = i / a.D, c = i - k * a.D;
             const float2 v = q[(size_t)k * a.C + c];
             const float ga = a.gamma[g * a.D + c];
@@ -284,25 +302,37 @@ __global__ void __launch_bounds__(256) gn_bwd_join_kernel(const GnArgs a, const 
         const float inv = 1.0f / ((float)a.P * (float)a.D);
         if (threadIdx.x == 0) gsum[blockIdx.x] = float2{s1 * inv, s2 * inv};
     } else {
-        const int c = ((int)blockIdx.x - a.B * a.G) * 32 + (threadIdx.x & 31), row = threadIdx.x >> 5;
-        float2 s = {0.0f, 0.0f};
+        const int cl = threadIdx.x & 15, row = threadIdx.x >> 4, c = ((int)blockIdx.x - nsum) * 16 + cl;
+        float2 s[4] = {};
         if (c < a.C) {
             const int rows = a.B * w.nchunk;
-            for (int i = row; i < rows; i += 8) {
+            int i = row;
+            for (; i + 192 < rows; i += 256) {
+                float2 v[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) v[u] = part[(size_t)(i + 64 * u) * a.C + c];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) { s[u].x += v[u].x; s[u].y += v[u].y; }
+            }
+            for (; i < rows; i += 64) {
                 const float2 v = part[(size_t)i * a.C + c];
-                s.x += v.x;
-                s.y += v.y;
+                s[0].x += v.x;
+                s[0].y += v.y;
             }
         }
-        red[threadIdx.x] = s;
+        red[cl * 65 + row] = float2{(s[0].x + s[1].x) + (s[2].x + s[3].x), (s[0].y + s[1].y) + (s[2].y + s[3].y)};
         __syncthreads();
-        if (row == 0 && c < a.C) {
-            for (int i = 1; i < 8; ++i) {
-                s.x += red[i * 32 + threadIdx.x].x;
-                s.y += red[i * 32 + threadIdx.x].y;
-            }
-            a.dbeta[c] = s.x;
-            a.dgamma[c] = s.y;
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;          // wave k adds channel k's 64 lanes
+        float2 t = red[wave * 65 + lane];
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            t.x += __shfl_xor(t.x, o);
+            t.y += __shfl_xor(t.y, o);
+        }
+        const int cw = ((int)blockIdx.x - nsum) * 16 + wave;
+        if (lane == 0 && cw < a.C) {
+            a.dbeta[cw] = t.x;
+            a.dgamma[cw] = t.y;
         }
     }
 }
@@ -313,13 +343,13 @@ __global__ void __launch_bounds__(256) gn_bwd_apply_kernel(const GnArgs a, const
     const GnPos<V> g(a, w);
     if (!g.on) return;
     typedef vec_io<T, V> IO;
-    const GnChannels<V> ch(a, g.b, g.c0);
-    float m1[V], m2[V];
+    GnChannels<V> ch;
+    GnGradient<V> gr;
+    ch.load(a, g.b, g.c0);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const float2 m = gsum[(size_t)g.b * a.G + (g.c0 + i) / a.D];
-        m1[i] = m.x;
-        m2[i] = m.y;
+        gr.set(ch, i, m.x, m.y);
     }
     const size_t base = (size_t)g.b * a.P * a.C + g.c0;
     const T *__restrict__ x = (const T *)a.x + base, *__restrict__ dy = (const T *)a.dy + base;
@@ -330,14 +360,205 @@ __global__ void __launch_bounds__(256) gn_bwd_apply_kernel(const GnArgs a, const
     struct Row { typename IO::raw x, d; };
     gn_rows<2>(g.p, g.p1, w.R, [&](int p) { return Row{IO::load(x + (size_t)p * a.C), IO::load(dy + (size_t)p * a.C)}; },
                [&](int p, const Row &q) {
-                   float v[V], d[V], dt[V], h[V];
+                   float v[V], d[V], dt[V];
                    IO::unpack(q.x, v);
                    IO::unpack(q.d, d);
-                   gn_dt<V, ACT, DROP>(ch, drop, key, base + (size_t)p * a.C, v, d, dt, h);
+                   gn_dt<V, ACT, DROP>(ch, drop, key, base + (size_t)p * a.C, v, d, dt);
 #pragma unroll
-                   for (int i = 0; i < V; ++i) v[i] = ch.r[i] * (ch.ga[i] * dt[i] - (m1[i] + h[i] * m2[i]));
+                   for (int i = 0; i < V; ++i) v[i] = gr.dx(ch, i, v[i], dt[i]);
                    IO::store(dx + (size_t)p * a.C, v);
                });
+}
+
+// ---- one pass: the pixels of a sample's channel slab stay in registers ------------------------------
+// A workgroup of 512 threads owns sv V neighbouring channels (whole groups) of one sample: thread (row, cv) holds
+// the vectors of pixels row, row + R, ..., R = 512 / sv, so the map is read once, the statistics are taken in two
+// steps (mean, then squares about it) from registers, and one launch does what the chunked form needs three for.
+// sv is a power of two up to 64 and D one up to 64, so sums over rows are lane exchanges and one LDS step.
+struct GnSlab { int sv, nslab; };
+
+// sum[i] (channel cv V + i of this thread) -> totals over the workgroup's rows; tot[c] for thread c < sv V.
+template <int V> __device__ __forceinline__ float gn_slab_total(const float (&v)[V], int sv, float *red) {
+    float s[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[i] = v[i];
+    for (int o = sv; o < 64; o <<= 1)
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[i] += __shfl_xor(s[i], o);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, W = sv * V;
+    __syncthreads();                                             // (the scratch may still be read)
+    if (lane < sv)
+#pragma unroll
+        for (int i = 0; i < V; ++i) red[wave * W + lane * V + i] = s[i];
+    __syncthreads();
+    float t = 0.0f;
+    if ((int)threadIdx.x < W)
+        for (int w = 0; w < 8; ++w) t += red[w * W + threadIdx.x];
+    return t;
+}
+// Sum over the D neighbouring threads of a group.
+__device__ __forceinline__ float gn_group_sum(float t, int D) {
+    for (int o = 1; o < D; o <<= 1) t += __shfl_xor(t, o);
+    return t;
+}
+
+template <typename T, int V, int NV, int ACT, bool DROP>
+__global__ void __launch_bounds__(512) gn_slab_kernel(const GnArgs a, const GnSlab w) {
+    extern __shared__ float red[];                               // [8][sv V] partial sums, then [sv V] of a channel's group
+    typedef vec_io<T, V> IO;
+    const int W = w.sv * V, cv = threadIdx.x % w.sv, row = threadIdx.x / w.sv, R = 512 / w.sv;
+    const int id = xcd_remap(blockIdx.x, gridDim.x), slab = id % w.nslab, b = id / w.nslab;
+    const size_t base = (size_t)b * a.P * a.C + slab * W + cv * V;
+    const T *__restrict__ x = (const T *)a.x + base, *__restrict__ res = (const T *)a.res + base;
+    T *__restrict__ y = (T *)a.y + base;
+    float *grp = red + 8 * W;
+    typename IO::raw q[NV];
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+        if (row + n * R < a.P) q[n] = IO::load(x + (size_t)(row + n * R) * a.C);
+    const float inv_n = 1.0f / ((float)a.P * (float)a.D);
+    float s[V], mean[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[i] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+        float v[V];
+        IO::unpack(q[n], v);
+        if (row + n * R < a.P)
+#pragma unroll
+            for (int i = 0; i < V; ++i) s[i] += v[i];
+    }
+    float t = gn_group_sum(gn_slab_total<V>(s, w.sv, red), a.D) * inv_n;
+    if ((int)threadIdx.x < W) grp[threadIdx.x] = t;
+    const float m_keep = t;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        mean[i] = grp[cv * V + i];
+        s[i] = 0.0f;
+    }
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+        float v[V];
+        IO::unpack(q[n], v);
+        if (row + n * R < a.P)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float d = v[i] - mean[i];
+                s[i] += d * d;
+            }
+    }
+    t = gn_group_sum(gn_slab_total<V>(s, w.sv, red), a.D) * inv_n;
+    t = 1.0f / sqrtf(t + a.eps);
+    if ((int)threadIdx.x < W) {
+        grp[threadIdx.x] = t;
+        if (threadIdx.x % a.D == 0) ((float2 *)a.stats)[(size_t)b * a.G + (slab * W + threadIdx.x) / a.D] = float2{m_keep, t};
+    }
+    __syncthreads();
+    GnChannels<V> ch;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int c = cv * V + i;
+        ch.set(i, mean[i], grp[c], a.gamma[slab * W + c], a.beta[slab * W + c]);
+    }
+    const bool has_res = a.res != nullptr;
+    const DropArgs drop = {a.state, a.threshold, a.keep_scale};
+    uint4 key = {};
+    if constexpr (DROP) key = uint4{a.state[0], a.state[1], a.state[2], a.state[3]};
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+        const int p = row + n * R;
+        if (p >= a.P) continue;
+        float v[V], r[V];
+        bool keep[V];
+        typename IO::raw qs;
+        if (has_res) qs = IO::load(res + (size_t)p * a.C);
+        IO::unpack(q[n], v);
+        if constexpr (DROP) drop_keep<V>(drop, key, base + (size_t)p * a.C, keep);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            v[i] = act_c<ACT>(ch.t(i, v[i]));
+            if constexpr (DROP) v[i] = keep[i] ? v[i] * drop.keep_scale : 0.0f;
+        }
+        if (has_res) {
+            IO::unpack(qs, r);
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] += r[i];
+        }
+        IO::store(y + (size_t)p * a.C, v);
+    }
+}
+
+// Backward: x stays as it was read, dt as computed (fp32); the sums over a sample of each channel go to
+// part[b C + c] for the parameters' gradients.
+template <typename T, int V, int NV, int ACT, bool DROP>
+__global__ void __launch_bounds__(512) gn_slab_bwd_kernel(const GnArgs a, const GnSlab w, float2 *__restrict__ part) {
+    extern __shared__ float red[];                               // [8][sv V], then two of [sv V]
+    typedef vec_io<T, V> IO;
+    const int W = w.sv * V, cv = threadIdx.x % w.sv, row = threadIdx.x / w.sv, R = 512 / w.sv;
+    const int id = xcd_remap(blockIdx.x, gridDim.x), slab = id % w.nslab, b = id / w.nslab;
+    const size_t base = (size_t)b * a.P * a.C + slab * W + cv * V;
+    const T *__restrict__ x = (const T *)a.x + base, *__restrict__ dy = (const T *)a.dy + base;
+    T *__restrict__ dx = (T *)a.dx + base;
+    float *g1 = red + 8 * W, *g2 = g1 + W;
+    typename IO::raw q[NV], qd[NV];
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+        if (row + n * R < a.P) {
+            q[n] = IO::load(x + (size_t)(row + n * R) * a.C);
+            qd[n] = IO::load(dy + (size_t)(row + n * R) * a.C);
+        }
+    GnChannels<V> ch;
+    ch.load(a, b, slab * W + cv * V);
+    const DropArgs drop = {a.state, a.threshold, a.keep_scale};
+    uint4 key = {};
+    if constexpr (DROP) key = uint4{a.state[0], a.state[1], a.state[2], a.state[3]};
+    float dt[NV][V], s1[V], s2[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+        const int p = row + n * R;
+        if (p < a.P) {
+            float v[V], d[V];
+            IO::unpack(q[n], v);
+            IO::unpack(qd[n], d);
+            gn_dt<V, ACT, DROP>(ch, drop, key, base + (size_t)p * a.C, v, d, dt[n]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                s1[i] += dt[n][i];
+                s2[i] += dt[n][i] * (v[i] - ch.mean[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) s2[i] *= ch.r[i];
+    const float t1 = gn_slab_total<V>(s1, w.sv, red), t2 = gn_slab_total<V>(s2, w.sv, red);
+    const float inv_n = 1.0f / ((float)a.P * (float)a.D);
+    float ga = 0.0f;
+    if ((int)threadIdx.x < W) {
+        part[(size_t)b * a.C + slab * W + threadIdx.x] = float2{t1, t2};
+        ga = a.gamma[slab * W + threadIdx.x] * inv_n;
+    }
+    const float u1 = gn_group_sum(ga * t1, a.D), u2 = gn_group_sum(ga * t2, a.D);
+    if ((int)threadIdx.x < W) {
+        g1[threadIdx.x] = u1;
+        g2[threadIdx.x] = u2;
+    }
+    __syncthreads();
+    GnGradient<V> gr;
+#pragma unroll
+    for (int i = 0; i < V; ++i) gr.set(ch, i, g1[cv * V + i], g2[cv * V + i]);
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+        const int p = row + n * R;
+        if (p >= a.P) continue;
+        float v[V];
+        IO::unpack(q[n], v);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = gr.dx(ch, i, v[i], dt[n][i]);
+        IO::store(dx + (size_t)p * a.C, v);
+    }
 }
 
 // ---- host side -----------------------------------------------------------------------------------
@@ -365,6 +586,23 @@ static int gn_join_threads(const GnArgs &a, const GnWork &w) {
     return items <= 256 ? 64 : items <= 4096 ? 256 : 1024;
 }
 
+// The one-pass form's slabs, or sv = 0 where the chunked form runs: groups of a power of two of at most 64
+// channels in whole vectors, and the slab's pixels in at most `most` vectors a thread.  The widest slab up to 128
+// bytes of a pixel (what neighbouring lanes read together) that leaves a workgroup for every CU, else the
+// narrowest.
+template <int V> static GnSlab gn_slab(const GnArgs &a, int most) {
+    const int cv = a.C / V;
+    GnSlab best = {0, 0};
+    if (a.D > 64 || (a.D & (a.D - 1))) return best;
+    for (int sv = 1; sv <= 8 && cv % sv == 0; sv *= 2) {
+        if (sv * V % a.D || (long long)a.P * sv > 512ll * most) continue;
+        if (best.sv && (long long)a.B * (cv / sv) < 256) break;
+        best.sv = sv;
+        best.nslab = cv / sv;
+    }
+    return best;
+}
+
 // Calls f(vector width, activation, dropout) as types.
 template <int V, typename F> static void gn_pick_act(const GnArgs &a, F f) {
     auto drop = [&](auto act) {
@@ -386,24 +624,55 @@ template <typename T, typename F> static void gn_pick(const GnArgs &a, F f) {
 template <typename T> static int gn_forward(const GnArgs &a, void *ws, hipStream_t s) {
     float2 *part = (float2 *)ws;
     gn_pick<T>(a, [&](auto v, auto act, auto drop) {
-        constexpr int V = decltype(v)::value;
+        constexpr int V = decltype(v)::value, ACT = decltype(act)::value;
+        constexpr bool DROP = decltype(drop)::value;
+        if constexpr (V > 1) {
+            const GnSlab sl = gn_slab<V>(a, 16);
+            if (sl.sv) {
+                const int nv = (a.P * sl.sv + 511) / 512, lds = 9 * sl.sv * V * 4;
+                const dim3 grid((unsigned)(a.B * sl.nslab));
+                if (nv <= 2) hipLaunchKernelGGL((gn_slab_kernel<T, V, 2, ACT, DROP>), grid, dim3(512), lds, s, a, sl);
+                else if (nv <= 4) hipLaunchKernelGGL((gn_slab_kernel<T, V, 4, ACT, DROP>), grid, dim3(512), lds, s, a, sl);
+                else if (nv <= 8) hipLaunchKernelGGL((gn_slab_kernel<T, V, 8, ACT, DROP>), grid, dim3(512), lds, s, a, sl);
+                else if (nv <= 12) hipLaunchKernelGGL((gn_slab_kernel<T, V, 12, ACT, DROP>), grid, dim3(512), lds, s, a, sl);
+                else hipLaunchKernelGGL((gn_slab_kernel<T, V, 16, ACT, DROP>), grid, dim3(512), lds, s, a, sl);
+                return;
+            }
+        }
         const GnWork w = gn_work<V>(a);
         const dim3 grid((unsigned)(a.B * w.nchunk * w.nzb));
         hipLaunchKernelGGL((gn_stats_kernel<T, V>), grid, dim3(256), 0, s, a, w, part);
         hipLaunchKernelGGL(gn_stats_join_kernel, dim3((unsigned)(a.B * a.G)), dim3(gn_join_threads(a, w)), 0, s, a, w, part);
-        hipLaunchKernelGGL((gn_apply_kernel<T, V, decltype(act)::value, decltype(drop)::value>), grid, dim3(256), 0, s, a, w);
+        hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, DROP>), grid, dim3(256), 0, s, a, w);
     });
     return check_launch("group_norm_forward");
 }
 template <typename T> static int gn_backward(const GnArgs &a, void *ws, hipStream_t s) {
     gn_pick<T>(a, [&](auto v, auto act, auto drop) {
-        constexpr int V = decltype(v)::value;
+        constexpr int V = decltype(v)::value, ACT = decltype(act)::value;
+        constexpr bool DROP = decltype(drop)::value;
+        if constexpr (V > 1) {
+            const GnSlab sl = gn_slab<V>(a, 12);
+            if (sl.sv) {
+                const int nv = (a.P * sl.sv + 511) / 512, lds = 10 * sl.sv * V * 4;
+                const dim3 grid((unsigned)(a.B * sl.nslab));
+                float2 *part = (float2 *)ws;
+                if (nv <= 2) hipLaunchKernelGGL((gn_slab_bwd_kernel<T, V, 2, ACT, DROP>), grid, dim3(512), lds, s, a, sl, part);
+                else if (nv <= 4) hipLaunchKernelGGL((gn_slab_bwd_kernel<T, V, 4, ACT, DROP>), grid, dim3(512), lds, s, a, sl, part);
+                else if (nv <= 6) hipLaunchKernelGGL((gn_slab_bwd_kernel<T, V, 6, ACT, DROP>), grid, dim3(512), lds, s, a, sl, part);
+                else hipLaunchKernelGGL((gn_slab_bwd_kernel<T, V, 12, ACT, DROP>), grid, dim3(512), lds, s, a, sl, part);
+                GnWork w = {};
+                w.nchunk = 1;
+                hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)((a.C + 15) / 16)), dim3(1024), 0, s, a, w, part, (float2 *)nullptr, 0);
+                return;
+            }
+        }
         const GnWork w = gn_work<V>(a);
         const dim3 grid((unsigned)(a.B * w.nchunk * w.nzb));
         float2 *gsum = (float2 *)ws, *part = gsum + (size_t)a.B * a.G;
-        hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, decltype(act)::value, decltype(drop)::value>), grid, dim3(256), 0, s, a, w, part);
-        hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)(a.B * a.G + (a.C + 31) / 32)), dim3(256), 0, s, a, w, part, gsum);
-        hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, decltype(act)::value, decltype(drop)::value>), grid, dim3(256), 0, s, a, w, gsum);
+        hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT, DROP>), grid, dim3(256), 0, s, a, w, part);
+        hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)(a.B * a.G + (a.C + 15) / 16)), dim3(1024), 0, s, a, w, part, gsum, a.B * a.G);
+        hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, DROP>), grid, dim3(256), 0, s, a, w, gsum);
     });
     return check_launch("group_norm_backward");
 }

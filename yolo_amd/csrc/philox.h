@@ -65,15 +65,20 @@ template <> struct vec_io<bf16_t, 8> {
             v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
         }
     }
+    __device__ static __forceinline__ uint32_t pack(float lo, float hi) {          // one v_cvt_pk_bf16_f32
+        typedef __bf16 pair_t __attribute__((ext_vector_type(2)));
+        const f32x2_t v = {lo, hi};
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, pair_t));
+    }
     __device__ static __forceinline__ void store(bf16_t *p, const float (&v)[8]) {
-        store_stream16(p, pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]), pack2_bf16(v[4], v[5]), pack2_bf16(v[6], v[7]));
+        *(uint4 *)p = uint4{pack(v[0], v[1]), pack(v[2], v[3]), pack(v[4], v[5]), pack(v[6], v[7])};
     }
 };
 template <> struct vec_io<float, 4> {
     typedef float4 raw;
     __device__ static __forceinline__ raw load(const float *p) { return *(const float4 *)p; }
     __device__ static __forceinline__ void unpack(const raw &r, float (&v)[4]) { v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w; }
-    __device__ static __forceinline__ void store(float *p, const float (&v)[4]) { store_stream16(p, v[0], v[1], v[2], v[3]); }
+    __device__ static __forceinline__ void store(float *p, const float (&v)[4]) { *(float4 *)p = float4{v[0], v[1], v[2], v[3]}; }
 };
 template <typename T> struct vec_io<T, 1> {
     typedef T raw;
