@@ -430,3 +430,32 @@ def test_training_step_in_a_graph():
         for a, b in zip(out, eager[i]):
             assert torch.equal(a, b), i
         torch.ones(1000, device=DEV).sum().item()                    # eager work between the replays
+
+
+def test_second_derivatives_are_refused():
+    from yolo_amd import training as T
+    x = torch.randn(2, 4, 4, 32, device=DEV, requires_grad=True)
+    ga, be = torch.ones(32, device=DEV, requires_grad=True), torch.zeros(32, device=DEV, requires_grad=True)
+    for y in (T.group_norm_act(x, ga, be, 4, "mish"), T.dropout(x, 0.5, torch.tensor([1, 2], device=DEV))):
+        g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward()
+
+
+def test_partial_gradients_and_empty_batches():
+    from yolo_amd import training as T
+    x = torch.randn(2, 6, 6, 32, device=DEV)
+    ga, be = torch.randn(32, device=DEV, requires_grad=True), torch.randn(32, device=DEV, requires_grad=True)
+    y = T.group_norm_act(x, ga, be.detach(), 4, "mish", shortcut=x)
+    (only,) = torch.autograd.grad(y.sum(), ga)
+    full = torch.autograd.grad(T.group_norm_act(x, ga, be, 4, "mish").sum(), (ga, be))
+    assert torch.equal(only, full[0])
+    s = x.clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(T.group_norm_act(x, ga.detach(), be.detach(), 4, shortcut=s).sum(), s)[0], torch.ones_like(x))
+    e = torch.empty(0, 6, 6, 32, device=DEV, requires_grad=True)
+    y = T.group_norm_act(e, ga, be, 4, "mish")
+    got = torch.autograd.grad(y.sum(), (e, ga, be))
+    assert y.shape == e.shape and got[0].shape == e.shape and not got[1].any() and not got[2].any()
+    half = T.group_norm_act(x, ga.to(torch.bfloat16), be, 4)                        # parameters of another type: gradients of theirs
+    p = ga.detach().to(torch.bfloat16).requires_grad_(True)
+    assert torch.autograd.grad(T.group_norm_act(x, p, be, 4).sum(), p)[0].dtype == torch.bfloat16 and half.dtype == torch.float32

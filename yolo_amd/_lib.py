@@ -151,7 +151,8 @@ def require_gpu(*tensors):
 
 
 def ptr(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    """The address of a tensor as the entry points take it (None: a null pointer)."""
+    return None if t is None else t.data_ptr()
 
 
 def stream(ref=None):
@@ -160,14 +161,23 @@ def stream(ref=None):
     return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
 
 
+_entry = {}
+
+
 def launch(name, ref, *args):
     """Call the launching entry point ``name`` with ``args`` plus, as its last argument, the
     current stream of the device that tensor ``ref`` lives on, with that device current
-    (kernel attributes and launches are per device), and raise on a negative return code."""
-    fn = getattr(lib(), name)
-    dev = ref.device
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        check(fn(*args, stream(ref)))
+    (kernel attributes and launches are per device), and raise on a negative return code.
+    (torch.cuda.current_stream builds a Stream object for the same number: 2 us of the 8 a small
+    launch costs the host, more on the thread that runs backward().)"""
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(lib(), name)
+    index = ref.device.index
+    if index is None or index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
     else:
-        with torch.cuda.device(dev):
-            check(fn(*args, stream(ref)))
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc)

@@ -520,56 +520,76 @@ def _records(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _dense(t, dtype):
+    """t as a contiguous tensor of dtype (itself where it is one)."""
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+# The backward steps below are Python run by autograd's own thread, where every call costs about twice
+# what it does on the caller's: what can be decided in the forward pass is decided there.
 def _group_norm_forward(x, gamma, beta, shortcut, groups, act, epsilon, rate, state):
-    """(y, contiguous x, gamma and beta as the kernels take them, statistics)"""
-    x = x.contiguous()
+    """(y, contiguous x, gamma and beta as the kernels take them, statistics, the geometry of the launches)"""
+    x = x if x.is_contiguous() else x.contiguous()
     b, c = x.shape[0], x.shape[-1]
-    gamma, beta = gamma.float().contiguous(), beta.float().contiguous()
-    sc = None if shortcut is None else shortcut.to(x.dtype).contiguous()
+    gamma, beta = _dense(gamma, torch.float32), _dense(beta, torch.float32)
+    sc = None if shortcut is None else _dense(shortcut, x.dtype)
     y = torch.empty_like(x)
     stats = torch.empty((b, groups, 2), device=x.device, dtype=torch.float32)
-    if x.numel():
-        pix = x.numel() // (b * c)
+    geo = None
+    n = x.numel()
+    if n:
+        pix = n // (b * c)
         nb = _lib.lib().ymx_group_norm_workspace_bytes(b, pix, c, groups)
+        geo = (b, pix, c, groups, act, _lib.dtype_code(x.dtype), rate, nb)
         ws = torch.empty((nb,), device=x.device, dtype=torch.uint8)
-        _lib.launch("ymx_group_norm_forward", x, _lib.ptr(x), _lib.ptr(gamma), _lib.ptr(beta), _lib.ptr(sc), _lib.ptr(y), _lib.ptr(stats),
-                    b, pix, c, groups, act, epsilon, _lib.dtype_code(x.dtype), rate, _lib.ptr(state), _lib.ptr(ws), nb)
-    return y, x, gamma, beta, stats
+        _lib.launch("ymx_group_norm_forward", x, x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), _lib.ptr(sc), y.data_ptr(), stats.data_ptr(),
+                    b, pix, c, groups, act, epsilon, geo[5], rate, _lib.ptr(state), ws.data_ptr(), nb)
+    return y, x, gamma, beta, stats, geo
+
+
+def _group_norm_backward(ctx, dy):
+    x, gamma, beta, stats, state = ctx.saved_tensors
+    need_x, need_g, need_b, need_s = ctx.needs_input_grad[:4]
+    dy = _dense(dy, x.dtype)
+    dx = dgamma = dbeta = None
+    if need_x or need_g or need_b:
+        dx = torch.empty_like(x)
+        dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(beta)
+        if ctx.geo is not None:
+            b, pix, c, groups, act, code, rate, nb = ctx.geo
+            ws = torch.empty((nb,), device=x.device, dtype=torch.uint8)
+            _lib.launch("ymx_group_norm_backward", x, x.data_ptr(), dy.data_ptr(), gamma.data_ptr(), beta.data_ptr(), stats.data_ptr(), dx.data_ptr(),
+                        dgamma.data_ptr(), dbeta.data_ptr(), b, pix, c, groups, act, code, rate, _lib.ptr(state), ws.data_ptr(), nb)
+        else:
+            dgamma.zero_()
+            dbeta.zero_()
+        if dgamma.dtype != ctx.dtypes[0]:
+            dgamma = dgamma.to(ctx.dtypes[0])
+        if dbeta.dtype != ctx.dtypes[1]:
+            dbeta = dbeta.to(ctx.dtypes[1])
+    dsc = None
+    if need_s:
+        dsc = dy if dy.dtype == ctx.dtypes[2] else dy.to(ctx.dtypes[2])
+    return dx if need_x else None, dgamma if need_g else None, dbeta if need_b else None, dsc, None, None, None, None, None
+
+
+_group_norm_backward_once = torch.autograd.function.once_differentiable(_group_norm_backward)
 
 
 class _GroupNormAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gamma, beta, shortcut, groups, act, epsilon, rate, state):
-        y, xc, ga, be, stats = _group_norm_forward(x, gamma, beta, shortcut, groups, act, epsilon, rate, state)
+        y, xc, ga, be, stats, ctx.geo = _group_norm_forward(x, gamma, beta, shortcut, groups, act, epsilon, rate, state)
         ctx.save_for_backward(xc, ga, be, stats, state)
-        ctx.args = (groups, act, rate)
         ctx.dtypes = (gamma.dtype, beta.dtype, None if shortcut is None else shortcut.dtype)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, gamma, beta, stats, state = ctx.saved_tensors
-        groups, act, rate = ctx.args
-        b, c = x.shape[0], x.shape[-1]
-        dy = dy.to(x.dtype).contiguous()
-        dx = dgamma = dbeta = None
-        if any(ctx.needs_input_grad[:3]):
-            dx = torch.empty_like(x)
-            if x.numel():
-                dgamma, dbeta = (torch.empty((c,), device=x.device, dtype=torch.float32) for _ in range(2))
-                pix = x.numel() // (b * c)
-                nb = _lib.lib().ymx_group_norm_workspace_bytes(b, pix, c, groups)
-                ws = torch.empty((nb,), device=x.device, dtype=torch.uint8)
-                _lib.launch("ymx_group_norm_backward", x, _lib.ptr(x), _lib.ptr(dy), _lib.ptr(gamma), _lib.ptr(beta), _lib.ptr(stats), _lib.ptr(dx),
-                            _lib.ptr(dgamma), _lib.ptr(dbeta), b, pix, c, groups, act, _lib.dtype_code(x.dtype), rate,
-                            _lib.ptr(state), _lib.ptr(ws), nb)
-            else:
-                dgamma, dbeta = (torch.zeros((c,), device=x.device, dtype=torch.float32) for _ in range(2))
-            dgamma = dgamma.to(ctx.dtypes[0]) if ctx.needs_input_grad[1] else None
-            dbeta = dbeta.to(ctx.dtypes[1]) if ctx.needs_input_grad[2] else None
-        dsc = dy.to(ctx.dtypes[2]) if ctx.needs_input_grad[3] else None
-        return (dx if ctx.needs_input_grad[0] else None), dgamma, dbeta, dsc, None, None, None, None, None
+        # with create_graph=True the results carry an error for whoever differentiates them
+        return _group_norm_backward_once(ctx, dy) if torch.is_grad_enabled() else _group_norm_backward(ctx, dy)
 
 
 def group_norm_act(x, gamma, beta, groups, activation=None, shortcut=None, epsilon=1e-3, rate=0.0, state=None):
@@ -602,30 +622,36 @@ def group_norm_act(x, gamma, beta, groups, activation=None, shortcut=None, epsil
 
 
 def _dropout_launch(x, shortcut, rate, state):
-    x = x.contiguous()
+    x = x if x.is_contiguous() else x.contiguous()
     y = torch.empty_like(x)
-    sc = None if shortcut is None else shortcut.to(x.dtype).contiguous()
-    _lib.launch("ymx_dropout", x, _lib.ptr(x), _lib.ptr(sc), _lib.ptr(y), x.numel(), _lib.dtype_code(x.dtype), rate, _lib.ptr(state))
+    sc = None if shortcut is None else _dense(shortcut, x.dtype)
+    _lib.launch("ymx_dropout", x, x.data_ptr(), _lib.ptr(sc), y.data_ptr(), x.numel(), _lib.dtype_code(x.dtype), rate, state.data_ptr())
     return y
+
+
+def _dropout_backward(ctx, dy):
+    (state,) = ctx.saved_tensors
+    need_x, need_s = ctx.needs_input_grad[:2]
+    rate, x_dtype, shortcut_dtype = ctx.args
+    if dy.dtype != x_dtype:
+        dy = dy.to(x_dtype)
+    dx = _dropout_launch(dy, None, rate, state) if need_x else None
+    return dx, (dy if dy.dtype == shortcut_dtype else dy.to(shortcut_dtype)) if need_s else None, None, None
+
+
+_dropout_backward_once = torch.autograd.function.once_differentiable(_dropout_backward)
 
 
 class _DropoutFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, shortcut, rate, state):
         ctx.save_for_backward(state)
-        ctx.rate = rate
-        ctx.x_dtype = x.dtype
-        ctx.shortcut_dtype = None if shortcut is None else shortcut.dtype
+        ctx.args = (rate, x.dtype, None if shortcut is None else shortcut.dtype)
         return _dropout_launch(x, shortcut, rate, state)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        (state,) = ctx.saved_tensors
-        dy = dy.to(ctx.x_dtype)
-        dx = _dropout_launch(dy, None, ctx.rate, state) if (ctx.needs_input_grad[0] and dy.numel()) else \
-            (torch.empty_like(dy) if ctx.needs_input_grad[0] else None)
-        return dx, (dy.to(ctx.shortcut_dtype) if ctx.needs_input_grad[1] else None), None, None
+        return _dropout_backward_once(ctx, dy) if torch.is_grad_enabled() else _dropout_backward(ctx, dy)
 
 
 def dropout(x, rate, state, shortcut=None):
