@@ -412,7 +412,7 @@ int ymx_bn_backward_apply(const void *dz, const void *u, const float *a, const f
                           long long n_pix, int C, int dtype, void *stream);
 
 /* ---- group normalisation with activation, dropout and shortcut (no counterpart in the reference) ----
- * x [B][n_pix][C] dense, G groups of C / G neighbouring channels, statistics of every (sample,
+ * x [B][n_pix][C] dense, G <= 4096 groups of C / G neighbouring channels, statistics of every (sample,
  * group) over its pixels and channels (biased variance):
  *   h = (x - mean) / sqrt(var + eps),  t = gamma h + beta
  *   y = keep * act(t) / (1 - rate) + residual            (residual may be NULL)

@@ -62,6 +62,12 @@ CASES = [   # shape, groups, activation, shortcut, rate, type
     ((2, 4, 5, 6, 16), 2, "mish", True, 0.1, "bf16"),           # more than two pixel axes
     ((300, 4, 4, 32), 8, "mish", True, 0.1, "bf16"),            # many samples
     ((1, 208, 208, 32), 8, "mish", True, 0.1, "bf16"),
+    ((2, 6, 7, 1023), 1, "mish", True, 0.1, "f32"),             # a group in four parts
+    ((2, 40, 41, 771), 3, "leaky", False, 0.0, "bf16"),         # groups of 257: two parts each
+    ((1, 9, 9, 4112), 1, "mish", False, 0.0, "bf16"),           # ... of vectors
+    ((1, 4, 4, 6168), 8, "leaky", True, 0.0, "bf16"),           # 771 channels a group: no whole vectors
+    ((1, 5, 5, 2400), 300, "mish", False, 0.1, "bf16"),         # more than 256 groups
+    ((1, 77, 77, 1024), 1, "mish", True, 0.0, "bf16"),          # one wide group over many chunks
 ]
 
 

@@ -36,6 +36,7 @@ def test_group_norm_entry_points_validate_without_gpu():
                              (lambda: fwd(dtype=2), -1, b"dtype"), (lambda: fwd(rate=1.0, state=one), -1, b"rate"), (lambda: fwd(rate=float("nan"), state=one), -1, b"rate"),
                              (lambda: fwd(rate=0.5), -1, b"state"), (lambda: fwd(rate=0.5, state=odd), -1, b"state"), (lambda: fwd(ws=odd), -1, b"aligned"),
                              (lambda: fwd(nb=need - 1), -3, b"workspace"), (lambda: fwd(P=1 << 31), -2, b"pixels"), (lambda: fwd(B=1 << 21), -2, b"samples"),
+                             (lambda: fwd(C=8192, G=8192), -2, b"groups"),
                              (lambda: bwd(dx=None), -1, b"null"), (lambda: bwd(G=0), -1, b"size"), (lambda: bwd(rate=-0.1), -1, b"rate"),
                              (lambda: bwd(nb=8), -3, b"workspace"),
                              (lambda: L.ymx_dropout(one, None, one, 8, _lib.BF16, 0.5, None, None), -1, b"null"),

@@ -911,6 +911,7 @@ static int gn_args(const char *what, GnArgs &a, long long B, long long n_pix, in
     if (!(rate >= 0.0 && rate < 1.0)) return fail(YMX_EARG, "%s: dropout rate %g (0 <= rate < 1)", what, rate);
     if (rate > 0.0 && (!state || ((uintptr_t)state & 7))) return fail(YMX_EARG, "%s: dropout needs a state of two 64-bit words", what);
     // pixel indexes are 32-bit in the kernels, and so are workgroup numbers; offsets are 64-bit
+    if (G > 4096) return fail(YMX_EUNSUPPORTED, "%s: %d groups (at most 4096)", what, G);      // a pair of each in LDS
     if (n_pix > (1ll << 30) || B > (1ll << 20) || B * G > (1ll << 30) || (long long)C * B > (1ll << 33))
         return fail(YMX_EUNSUPPORTED, "%s: %lld samples of %lld pixels and %d channels", what, B, n_pix, C);
     const size_t need = group_norm_workspace_bytes((int)B, (int)n_pix, C, G);
@@ -925,7 +926,7 @@ static int gn_args(const char *what, GnArgs &a, long long B, long long n_pix, in
 }
 
 size_t ymx_group_norm_workspace_bytes(long long B, long long n_pix, int C, int G) {
-    if (B <= 0 || n_pix <= 0 || C <= 0 || G <= 0 || B > (1ll << 20) || n_pix > (1ll << 30)) return 0;
+    if (B <= 0 || n_pix <= 0 || C <= 0 || G <= 0 || C % G || B > (1ll << 20) || n_pix > (1ll << 30)) return 0;
     return group_norm_workspace_bytes((int)B, (int)n_pix, C, G);
 }
 

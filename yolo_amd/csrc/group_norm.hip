@@ -12,10 +12,11 @@
 // against 4 and 6 bytes in bf16.  t, dt and the dropout mask are computed again where they are
 // needed instead of being stored.
 //
-// Form: the pixels of a sample are cut into chunks, a workgroup per chunk.  Pass 1 leaves one pair
-// of numbers per (chunk, channel) -- mean and centred sum of squares, or sum dt and sum dt h --
-// a small launch adds them per group (and per channel) in a fixed order, pass 2 reads the map
-// again and writes.  All sums are fp32 and no result depends on the order workgroups run in.
+// Chunked form: the pixels of a sample are cut into chunks, a workgroup per chunk.  Pass 1 leaves one
+// pair of numbers per (chunk, group) -- mean and centred sum of squares, or S1 and S2 -- and, backward,
+// one per (chunk, channel); every workgroup of pass 2 first joins the pairs of its sample (a few
+// hundred, from L2), then reads the map again and writes.  Slab form: see gn_slab_kernel.  All sums
+// are fp32, added in a fixed order: no result depends on the order workgroups run in.
 #include <algorithm>
 #include <type_traits>
 
@@ -23,26 +24,45 @@
 
 namespace ymx {
 
-// Where a thread of the chunked kernels works: V channels from c0 of the pixels p, p + R, ... < p1 of sample b.
+// Where a thread of the chunked kernels works: V channels from c0 of the pixels p, p + R, ... < p1 of sample b.  A
+// workgroup covers wc channels from cb: whole groups, or (nsub > 1) one of the nsub parts of a group that
+// is wider than 256 vectors.
 struct GnWork {
     int cvb, R, nzb;             // channel vectors per workgroup, pixels side by side, channel blocks
+    int nsub;                    // blocks per group where a group needs several, else 1
     int nchunk, per;             // chunks per sample, pixels per chunk
 };
 template <int V> struct GnPos {
-    int b, chunk, zb, cv, r, c0, p, p1;
+    int b, chunk, cb, wc, cv, r, c0, p, p1;
+    int g0, sub, D;              // first group, part of it, channels per group of this block
     bool on;
-    __device__ __forceinline__ GnPos(const GnArgs &a, const GnWork &w) {
-        int id = blockIdx.x;
-        zb = id % w.nzb;
+    __device__ __forceinline__ GnPos(const GnArgs &a, const GnWork &w, int first = 0) {
+        int id = blockIdx.x - first;
+        const int zb = id % w.nzb, W = w.cvb * V;
         id /= w.nzb;
         chunk = id % w.nchunk;
         b = id / w.nchunk;
+        if (w.nsub > 1) {
+            g0 = zb / w.nsub;
+            sub = zb - g0 * w.nsub;
+            cb = g0 * a.D + sub * W;
+            D = wc = min(W, a.D - sub * W);
+        } else {
+            cb = zb * W;
+            wc = min(W, a.C - cb);
+            g0 = cb / a.D;
+            sub = 0;
+            D = a.D;
+        }
         cv = threadIdx.x % w.cvb;
         r = threadIdx.x / w.cvb;
-        c0 = (zb * w.cvb + cv) * V;
-        on = r < w.R && c0 < a.C;
+        c0 = cb + cv * V;
+        on = r < w.R && cv * V < wc;
         p = chunk * w.per + r;
         p1 = min(a.P, (chunk + 1) * w.per);
+    }
+    __device__ __forceinline__ size_t pair(const GnArgs &a, const GnWork &w) const {      // of group g0 in the table of pairs
+        return (((size_t)b * w.nchunk + chunk) * w.nsub + sub) * a.G + g0;
     }
 };
 
@@ -58,13 +78,45 @@ template <int U, typename L, typename F> __device__ __forceinline__ void gn_rows
     for (; p < p1; p += R) use(p, load(p));
 }
 
-__device__ __forceinline__ int gn_chunk_pixels(int P, int per, int k) { return min(P - k * per, per); }
+// Sum over the D channels of a group of f(channel), every group of the workgroup's W channels handed to done(group,
+// sum): a thread per group for narrow groups, a wave per group for wide ones.  `sum` returns a float2.
+template <typename F, typename D2> __device__ __forceinline__ void gn_over_groups(int W, int D, F f, D2 done) {
+    const int ng = W / D;
+    if (D <= 16) {
+        for (int g = threadIdx.x; g < ng; g += 256) {
+            float2 s = {0.0f, 0.0f};
+            for (int c = 0; c < D; ++c) {
+                const float2 v = f(g * D + c);
+                s.x += v.x;
+                s.y += v.y;
+            }
+            done(g, s);
+        }
+    } else {
+        const int lane = threadIdx.x & 63;
+        for (int g = threadIdx.x >> 6; g < ng; g += 4) {
+            float2 s = {0.0f, 0.0f};
+            for (int c = lane; c < D; c += 64) {
+                const float2 v = f(g * D + c);
+                s.x += v.x;
+                s.y += v.y;
+            }
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) {
+                s.x += __shfl_xor(s.x, o);
+                s.y += __shfl_xor(s.y, o);
+            }
+            if (lane == 0) done(g, s);
+        }
+    }
+}
 
-// Pass 1, forward: part[(b nchunk + chunk) C + c] = (mean, sum of squares about it) of the chunk's pixels.
+// Pass 1, forward: part[((b nchunk + chunk) nsub + sub) G + g] = (mean, sum of squares about it) of the block's values.
 // A thread sums about its own first value, so what cancels in s2 - s1^2 / n is at most n eps of the result.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) gn_stats_kernel(const GnArgs a, const GnWork w, float2 *__restrict__ part) {
-    __shared__ float2 red[256 * V];
+    __shared__ float2 red[256 * V];                              // [R][W]; row 0 then holds the channels' pairs
+    __shared__ float gmean[256 * V];
     const GnPos<V> g(a, w);
     typedef vec_io<T, V> IO;
     const T *__restrict__ x = (const T *)a.x + (size_t)g.b * a.P * a.C + g.c0;
@@ -94,7 +146,7 @@ __global__ void __launch_bounds__(256) gn_stats_kernel(const GnArgs a, const GnW
     __syncthreads();
     const int np = g.p1 - g.chunk * w.per;                       // pixels of the chunk
     const int rows = min(w.R, np);
-    for (int c = threadIdx.x; c < W && g.zb * W + c < a.C; c += 256) {
+    for (int c = threadIdx.x; c < g.wc; c += 256) {
         float mean = 0.0f, m2 = 0.0f;
         for (int r = 0; r < rows; ++r) mean += (float)((np - r + w.R - 1) / w.R) * red[r * W + c].x;
         mean /= (float)np;
@@ -103,46 +155,80 @@ __global__ void __launch_bounds__(256) gn_stats_kernel(const GnArgs a, const GnW
             const float d = q.x - mean;
             m2 += q.y + (float)((np - r + w.R - 1) / w.R) * d * d;
         }
-        part[((size_t)g.b * w.nchunk + g.chunk) * a.C + g.zb * W + c] = float2{mean, m2};
+        red[c] = float2{mean, m2};
     }
+    __syncthreads();
+    const float inv_d = 1.0f / (float)g.D;
+    gn_over_groups(g.wc, g.D, [&](int c) { return float2{red[c].x, 0.0f}; }, [&](int gr, float2 t) { gmean[gr] = t.x * inv_d; });
+    __syncthreads();
+    float2 *dst = part + g.pair(a, w);
+    gn_over_groups(g.wc, g.D, [&](int c) {
+                       const float d = red[c].x - gmean[c / g.D];
+                       return float2{red[c].y + (float)np * d * d, 0.0f};
+                   },
+                   [&](int gr, float2 t) { dst[gr] = float2{gmean[gr], t.x}; });
 }
 
-// Sum of v over the workgroup, the same value on every thread; scratch holds one float per wave.
-__device__ __forceinline__ float gn_block_sum(float v, float *scratch) {
+// Pass 2 begins: the pairs of the sample's blocks joined for every group, all threads of the workgroup taking
+// part (256: group lanes x block lanes).  out[g] in LDS; scratch holds 256 pairs.
+//   forward   (mean, 1 / sqrt(var + eps)); one workgroup of the sample keeps it in stats
+//   backward  (S1, S2) / N
+template <bool BWD, int V>
+__device__ __forceinline__ void gn_join(const GnArgs &a, const GnWork &w, int b, bool keep, const float2 *__restrict__ part,
+                                        float2 *__restrict__ out, float2 *__restrict__ scratch) {
+    const int gl = min(a.G, 256), cl = 256 / gl, lane = threadIdx.x % gl, row = threadIdx.x / gl, blocks = w.nchunk * w.nsub;
+    const float2 *__restrict__ src = part + (size_t)b * blocks * a.G;
+    const float inv_n = 1.0f / ((float)a.P * (float)a.D);
+    auto values = [&](int k) {                                   // how many block k holds of a group
+        const int chunk = w.nsub == 1 ? k : k / w.nsub, sub = k - chunk * w.nsub;
+        const int pix = min(w.per, a.P - chunk * w.per), wid = w.nsub == 1 ? a.D : min(w.cvb * V, a.D - sub * w.cvb * V);
+        return (float)pix * (float)wid;
+    };
+    for (int g0 = 0; g0 < a.G; g0 += gl) {
+        const int g = g0 + lane;
+        const bool on = row < cl && g < a.G;
+        float2 s = {0.0f, 0.0f};
+        float piv = 0.0f;                                        // forward: sums about the first block's mean
+        if (on) {
+            if (!BWD) piv = src[g].x;
+            auto add = [&](int k, float2 v) {
+                if (BWD) {
+                    s.x += v.x;
+                    s.y += v.y;
+                } else {
+                    const float n = values(k), d = v.x - piv;
+                    s.x += n * d;
+                    s.y += v.y + n * d * d;
+                }
+            };
+            int k = row;
+            for (; k + 7 * cl < blocks; k += 8 * cl) {
+                float2 v[8];
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    const int nw = blockDim.x >> 6;
-    if (nw == 1) return v;
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float s = 0.0f;
-    for (int i = 0; i < nw; ++i) s += scratch[i];
-    return s;
-}
-
-// One workgroup per (sample, group): the chunks' pairs -> (mean, 1 / sqrt(var + eps)).
-__global__ void __launch_bounds__(1024) gn_stats_join_kernel(const GnArgs a, const GnWork w, const float2 *__restrict__ part) {
-    __shared__ float scratch[16];
-    const int b = blockIdx.x / a.G, g = blockIdx.x % a.G;
-    const float2 *__restrict__ q = part + (size_t)b * w.nchunk * a.C + g * a.D;
-    const int items = w.nchunk * a.D;
-    const float N = (float)a.P * (float)a.D;
-    float s = 0.0f;
-    for (int i = threadIdx.x; i < items; i += blockDim.x) {
-        const int k = i / a.D, c = i - k * a.D;
-        s += (float)gn_chunk_pixels(a.P, w.per, k) * q[(size_t)k * a.C + c].x;
+                for (int u = 0; u < 8; ++u) v[u] = src[(size_t)(k + u * cl) * a.G + g];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) add(k + u * cl, v[u]);
+            }
+            for (; k < blocks; k += cl) add(k, src[(size_t)k * a.G + g]);
+        }
+        __syncthreads();
+        if (on) scratch[row * gl + lane] = s;
+        __syncthreads();
+        if (on && row == 0) {
+            for (int r = 1; r < cl; ++r) {
+                s.x += scratch[r * gl + lane].x;
+                s.y += scratch[r * gl + lane].y;
+            }
+            if (BWD) {
+                out[g] = float2{s.x * inv_n, s.y * inv_n};
+            } else {
+                const float shift = s.x * inv_n;
+                out[g] = float2{piv + shift, 1.0f / sqrtf(fmaxf(s.y * inv_n - shift * shift, 0.0f) + a.eps)};
+                if (keep) ((float2 *)a.stats)[(size_t)b * a.G + g] = out[g];
+            }
+        }
     }
-    const float mean = gn_block_sum(s, scratch) / N;
-    s = 0.0f;
-    for (int i = threadIdx.x; i < items; i += blockDim.x) {
-        const int k = i / a.D, c = i - k * a.D;
-        const float2 v = q[(size_t)k * a.C + c];
-        const float d = v.x - mean;
-        s += v.y + (float)gn_chunk_pixels(a.P, w.per, k) * d * d;
-    }
-    const float var = gn_block_sum(s, scratch) / N;
-    if (threadIdx.x == 0) ((float2 *)a.stats)[blockIdx.x] = float2{mean, 1.0f / sqrtf(var + a.eps)};
+    __syncthreads();
 }
 
 // The numbers of a thread's V channels: d = x - mean first (exact next to the mean, so that a map without
@@ -155,8 +241,7 @@ template <int V> struct GnChannels {
         ta[i] = gamma * rstd;
         be[i] = beta;
     }
-    __device__ __forceinline__ void load(const GnArgs &a, int b, int c0) {
-        const float2 *__restrict__ st = (const float2 *)a.stats + (size_t)b * a.G;
+    __device__ __forceinline__ void load(const GnArgs &a, const float2 *st, int c0) {      // st: of the sample's groups
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const float2 m = st[(c0 + i) / a.D];
@@ -168,12 +253,14 @@ template <int V> struct GnChannels {
 
 // Pass 2, forward.
 template <typename T, int V, int ACT, bool DROP>
-__global__ void __launch_bounds__(256) gn_apply_kernel(const GnArgs a, const GnWork w) {
+__global__ void __launch_bounds__(256) gn_apply_kernel(const GnArgs a, const GnWork w, const float2 *__restrict__ part) {
+    extern __shared__ float2 joined[];                           // [G], then 256 of scratch
     const GnPos<V> g(a, w);
+    gn_join<false, V>(a, w, g.b, g.chunk == 0 && g.cb == 0, part, joined, joined + a.G);
     if (!g.on) return;
     typedef vec_io<T, V> IO;
     GnChannels<V> ch;
-    ch.load(a, g.b, g.c0);
+    ch.load(a, joined, g.c0);
     const size_t base = (size_t)g.b * a.P * a.C + g.c0;
     const T *__restrict__ x = (const T *)a.x + base, *__restrict__ res = (const T *)a.res + base;
     T *__restrict__ y = (T *)a.y + base;
@@ -233,16 +320,18 @@ template <int V> struct GnGradient {
     }
 };
 
-// Pass 1, backward: part[(b nchunk + chunk) C + c] = (sum dt, sum dt h) of the chunk's pixels.
+// Pass 1, backward: part[(b nchunk + chunk) C + c] = (sum dt, sum dt h) of the chunk's pixels, and
+// gpart[((b nchunk + chunk) nsub + sub) G + g] = (S1, S2) of the block's values.
 template <typename T, int V, int ACT, bool DROP>
-__global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const GnArgs a, const GnWork w, float2 *__restrict__ part) {
-    __shared__ float2 red[256 * V];
+__global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const GnArgs a, const GnWork w, float2 *__restrict__ part,
+                                                          float2 *__restrict__ gpart) {
+    __shared__ float2 red[256 * V];                              // [R][W]; row 0 then holds gamma times the channels' pairs
     const GnPos<V> g(a, w);
     typedef vec_io<T, V> IO;
     const int W = w.cvb * V;
     if (g.on) {
         GnChannels<V> ch;
-        ch.load(a, g.b, g.c0);
+        ch.load(a, (const float2 *)a.stats + (size_t)g.b * a.G, g.c0);
         const size_t base = (size_t)g.b * a.P * a.C + g.c0;
         const T *__restrict__ x = (const T *)a.x + base, *__restrict__ dy = (const T *)a.dy + base;
         const DropArgs drop = {a.state, a.threshold, a.keep_scale};
@@ -268,87 +357,82 @@ __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const GnArgs a, const 
         for (int i = 0; i < V; ++i) red[g.r * W + g.cv * V + i] = float2{s1[i], s2[i] * ch.r[i]};
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < W && g.zb * W + c < a.C; c += 256) {
+    for (int c = threadIdx.x; c < g.wc; c += 256) {
         float2 s = {0.0f, 0.0f};
         for (int r = 0; r < w.R; ++r) {
             const float2 q = red[r * W + c];
             s.x += q.x;
             s.y += q.y;
         }
-        part[((size_t)g.b * w.nchunk + g.chunk) * a.C + g.zb * W + c] = s;
+        part[((size_t)g.b * w.nchunk + g.chunk) * a.C + g.cb + c] = s;
+        const float ga = a.gamma[g.cb + c];
+        red[c] = float2{ga * s.x, ga * s.y};
     }
+    __syncthreads();
+    float2 *dst = gpart + g.pair(a, w);
+    gn_over_groups(g.wc, g.D, [&](int c) { return red[c]; }, [&](int gr, float2 t) { dst[gr] = t; });
 }
 
-// Workgroups 0 .. nsum - 1 (one per sample and group, or none): gsum[b][g] = (S1, S2) / N.  The others, 16
-// channels each: dbeta and dgamma, a channel's B nchunk pairs added by 64 row lanes (four chains each) and
-// those by a tree.
-__global__ void __launch_bounds__(1024) gn_bwd_join_kernel(const GnArgs a, const GnWork w, const float2 *__restrict__ part,
-                                                           float2 *__restrict__ gsum, int nsum) {
-    __shared__ float2 red[16 * 65];
-    if ((int)blockIdx.x < nsum) {
-        const int b = blockIdx.x / a.G, g = blockIdx.x % a.G;
-        const float2 *__restrict__ q = part + (size_t)b * w.nchunk * a.C + g * a.D;
-        const int items = w.nchunk * a.D;
-        float s1 = 0.0f, s2 = 0.0f;
-        for (int i = threadIdx.x; i < items; i += 1024) {
-            const int k = i / a.D, c = i - k * a.D;
-            const float2 v = q[(size_t)k * a.C + c];
-            const float ga = a.gamma[g * a.D + c];
-            s1 += ga * v.x;
-            s2 += ga * v.y;
-        }
-        s1 = gn_block_sum(s1, (float *)red);
-        s2 = gn_block_sum(s2, (float *)red + 16);
-        const float inv = 1.0f / ((float)a.P * (float)a.D);
-        if (threadIdx.x == 0) gsum[blockIdx.x] = float2{s1 * inv, s2 * inv};
-    } else {
-        const int cl = threadIdx.x & 15, row = threadIdx.x >> 4, c = ((int)blockIdx.x - nsum) * 16 + cl;
-        float2 s[4] = {};
-        if (c < a.C) {
-            const int rows = a.B * w.nchunk;
-            int i = row;
-            for (; i + 192 < rows; i += 256) {
-                float2 v[4];
+// dbeta and dgamma of 16 channels from `rows` pairs each, by a workgroup of 16 * RL threads: RL row lanes (four chains
+// each) and those by a tree.  red: 16 * (RL + 1) pairs.
+template <int RL>
+__device__ __forceinline__ void gn_param_grads(const GnArgs &a, int block, int rows, const float2 *__restrict__ part, float2 *__restrict__ red) {
+    const int cl = threadIdx.x & 15, row = threadIdx.x >> 4, c = block * 16 + cl;
+    float2 s[4] = {};
+    if (c < a.C) {
+        int i = row;
+        for (; i + 3 * RL < rows; i += 4 * RL) {
+            float2 v[4];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) v[u] = part[(size_t)(i + 64 * u) * a.C + c];
+            for (int u = 0; u < 4; ++u) v[u] = part[(size_t)(i + RL * u) * a.C + c];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) { s[u].x += v[u].x; s[u].y += v[u].y; }
-            }
-            for (; i < rows; i += 64) {
-                const float2 v = part[(size_t)i * a.C + c];
-                s[0].x += v.x;
-                s[0].y += v.y;
-            }
+            for (int u = 0; u < 4; ++u) { s[u].x += v[u].x; s[u].y += v[u].y; }
         }
-        red[cl * 65 + row] = float2{(s[0].x + s[1].x) + (s[2].x + s[3].x), (s[0].y + s[1].y) + (s[2].y + s[3].y)};
-        __syncthreads();
-        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;          // wave k adds channel k's 64 lanes
-        float2 t = red[wave * 65 + lane];
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            t.x += __shfl_xor(t.x, o);
-            t.y += __shfl_xor(t.y, o);
-        }
-        const int cw = ((int)blockIdx.x - nsum) * 16 + wave;
-        if (lane == 0 && cw < a.C) {
-            a.dbeta[cw] = t.x;
-            a.dgamma[cw] = t.y;
+        for (; i < rows; i += RL) {
+            const float2 v = part[(size_t)i * a.C + c];
+            s[0].x += v.x;
+            s[0].y += v.y;
         }
     }
+    red[cl * (RL + 1) + row] = float2{(s[0].x + s[1].x) + (s[2].x + s[3].x), (s[0].y + s[1].y) + (s[2].y + s[3].y)};
+    __syncthreads();
+    // RL lanes per channel, channels dealt to the groups of RL threads
+    const int lane = threadIdx.x % RL, cw = threadIdx.x / RL;
+    float2 t = red[cw * (RL + 1) + lane];
+#pragma unroll
+    for (int o = RL / 2; o > 0; o >>= 1) {
+        t.x += __shfl_xor(t.x, o);
+        t.y += __shfl_xor(t.y, o);
+    }
+    if (lane == 0 && block * 16 + cw < a.C) {
+        a.dbeta[block * 16 + cw] = t.x;
+        a.dgamma[block * 16 + cw] = t.y;
+    }
+}
+__global__ void __launch_bounds__(1024) gn_param_grads_kernel(const GnArgs a, int rows, const float2 *__restrict__ part) {
+    __shared__ float2 red[16 * 65];
+    gn_param_grads<64>(a, blockIdx.x, rows, part, red);
 }
 
 // Pass 2, backward.
 template <typename T, int V, int ACT, bool DROP>
-__global__ void __launch_bounds__(256) gn_bwd_apply_kernel(const GnArgs a, const GnWork w, const float2 *__restrict__ gsum) {
-    const GnPos<V> g(a, w);
+__global__ void __launch_bounds__(256) gn_bwd_apply_kernel(const GnArgs a, const GnWork w, const float2 *__restrict__ part,
+                                                           const float2 *__restrict__ gpart, int nparam) {
+    extern __shared__ float2 joined[];                           // [G], then 16 * 17 of scratch
+    if ((int)blockIdx.x < nparam) {                              // the first workgroups: parameter gradients, 16 channels each
+        gn_param_grads<16>(a, blockIdx.x, a.B * w.nchunk, part, joined + a.G);
+        return;
+    }
+    const GnPos<V> g(a, w, nparam);
+    gn_join<true, V>(a, w, g.b, false, gpart, joined, joined + a.G);
     if (!g.on) return;
     typedef vec_io<T, V> IO;
     GnChannels<V> ch;
     GnGradient<V> gr;
-    ch.load(a, g.b, g.c0);
+    ch.load(a, (const float2 *)a.stats + (size_t)g.b * a.G, g.c0);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const float2 m = gsum[(size_t)g.b * a.G + (g.c0 + i) / a.D];
+        const float2 m = joined[(g.c0 + i) / a.D];
         gr.set(ch, i, m.x, m.y);
     }
     const size_t base = (size_t)g.b * a.P * a.C + g.c0;
@@ -509,7 +593,7 @@ __global__ void __launch_bounds__(512) gn_slab_bwd_kernel(const GnArgs a, const 
             qd[n] = IO::load(dy + (size_t)(row + n * R) * a.C);
         }
     GnChannels<V> ch;
-    ch.load(a, b, slab * W + cv * V);
+    ch.load(a, (const float2 *)a.stats + (size_t)b * a.G, slab * W + cv * V);
     const DropArgs drop = {a.state, a.threshold, a.keep_scale};
     uint4 key = {};
     if constexpr (DROP) key = uint4{a.state[0], a.state[1], a.state[2], a.state[3]};
@@ -562,41 +646,57 @@ __global__ void __launch_bounds__(512) gn_slab_bwd_kernel(const GnArgs a, const 
 }
 
 // ---- host side -----------------------------------------------------------------------------------
-// About 2048 workgroups (eight of 256 threads on each of 256 CUs), none with less than 16 K elements to read.
+// Chunks of a sample: about 2048 workgroups (eight of 256 threads on each of 256 CUs), none with less than 16 K
+// elements to read while that leaves 512 of them, else 4 K (16 x 52^2 x 256 forward 27.4 us at 16 K, 36.9 at 4 K;
+// 52^2 x 256 alone 13.6 and 11.6, backward 17.3 and 11.2); at most 256, whose pairs every workgroup of pass 2 joins.
 static int gn_chunks(int B, int P, int C) {
-    const long long most = std::max<long long>(1, (long long)P * C / 16384);
+    const long long n = (long long)P * C;
+    const long long most = std::max<long long>(n / 16384, std::min<long long>(n / 4096, 512 / B));
     const long long want = std::max(1, 2048 / B);
-    return (int)std::min<long long>(std::min(most, want), P);
+    return (int)std::min<long long>(std::max<long long>(1, std::min<long long>(256, std::min(most, want))), P);
 }
+// Channels are cut into blocks of whole groups of at most 256 vectors; a wider group into equal parts.
 template <int V> static GnWork gn_work(const GnArgs &a) {
     GnWork w;
-    const int cv = (a.C + V - 1) / V;
-    w.nzb = (cv + 255) / 256;
-    w.cvb = (cv + w.nzb - 1) / w.nzb;
+    const int cv = a.C / V;
+    int unit = 1;                                                // vectors in the least run of whole groups
+    while ((long long)unit * V % a.D) ++unit;
+    w.nsub = 1;
+    if (cv <= 256) {
+        w.cvb = cv;
+        w.nzb = 1;
+    } else if (unit <= 256) {
+        w.cvb = 256 / unit * unit;
+        w.nzb = (cv + w.cvb - 1) / w.cvb;
+    } else {                                                     // D > 256 V, a multiple of V (gn_pick)
+        w.nsub = (a.D / V + 255) / 256;
+        w.cvb = (a.D / V + w.nsub - 1) / w.nsub;
+        w.nzb = a.G * w.nsub;
+    }
     w.R = 256 / w.cvb;
     w.per = (a.P + gn_chunks(a.B, a.P, a.C) - 1) / gn_chunks(a.B, a.P, a.C);
     w.nchunk = (a.P + w.per - 1) / w.per;
     return w;
 }
+// Pairs: one per (chunk, channel) and one per (chunk, group or part of one).
+static size_t gn_pairs(int G, int C) { return (size_t)G * ((C / G + 255) / 256); }
 size_t group_norm_workspace_bytes(int B, int P, int C, int G) {
-    return ((size_t)B * gn_chunks(B, P, C) * C + (size_t)B * G) * sizeof(float2);
-}
-static int gn_join_threads(const GnArgs &a, const GnWork &w) {
-    const long long items = (long long)w.nchunk * a.D;
-    return items <= 256 ? 64 : items <= 4096 ? 256 : 1024;
+    return (size_t)B * gn_chunks(B, P, C) * (C + gn_pairs(G, C)) * sizeof(float2);
 }
 
 // The one-pass form's slabs, or sv = 0 where the chunked form runs: groups of a power of two of at most 64
-// channels in whole vectors, and the slab's pixels in at most `most` vectors a thread.  The widest slab up to 128
-// bytes of a pixel (what neighbouring lanes read together) that leaves a workgroup for every CU, else the
+// channels in whole vectors, 64 bytes or more of a pixel (narrower slabs fetch every line several times: 16 x 52^2 x
+// 256 forward 32 us in slabs of 32 bytes, 27 in chunks), the slab's pixels in at most `most` vectors a
+// thread.  The widest of 64, 128 and 256 bytes that gives a thread at most six vectors and every CU a workgroup
+// (64 x 13^2 x 1024 forward: 25.5, 22.0, 19.2 us; 64 x 26^2 x 512: 40.2 us at six vectors, 41.8 at eleven), else the
 // narrowest.
 template <int V> static GnSlab gn_slab(const GnArgs &a, int most) {
     const int cv = a.C / V;
     GnSlab best = {0, 0};
     if (a.D > 64 || (a.D & (a.D - 1))) return best;
-    for (int sv = 1; sv <= 8 && cv % sv == 0; sv *= 2) {
+    for (int sv = 4; sv <= 16 && cv % sv == 0; sv *= 2) {
         if (sv * V % a.D || (long long)a.P * sv > 512ll * most) continue;
-        if (best.sv && (long long)a.B * (cv / sv) < 256) break;
+        if (best.sv && ((long long)a.B * (cv / sv) < 256 || (long long)a.P * sv > 512 * 6)) break;
         best.sv = sv;
         best.nslab = cv / sv;
     }
@@ -613,11 +713,15 @@ template <int V, typename F> static void gn_pick_act(const GnArgs &a, F f) {
     else if (a.act == YMX_ACT_LEAKY) drop(std::integral_constant<int, YMX_ACT_LEAKY>{});
     else drop(std::integral_constant<int, YMX_ACT_NONE>{});
 }
-// 16-byte vectors where the channel count and every map's address allow them, else one element at a time.
+// 16-byte vectors where the channel count and every map's address allow them and blocks of whole groups, or parts of
+// a group, are whole vectors; else one element at a time.
 template <typename T, typename F> static void gn_pick(const GnArgs &a, F f) {
     constexpr int V = 16 / sizeof(T);
     auto ok = [](const void *p) { return p == nullptr || aligned16(p); };
-    if (a.C % V == 0 && ok(a.x) && ok(a.res) && ok(a.dy) && ok(a.y) && ok(a.dx)) gn_pick_act<V>(a, f);
+    int unit = a.D;
+    for (int v = V; v > 1 && unit % 2 == 0; v /= 2) unit /= 2;   // vectors in the least run of whole groups
+    const bool blocks = a.C <= 256 * V || unit <= 256 || a.D % V == 0;
+    if (a.C % V == 0 && blocks && ok(a.x) && ok(a.res) && ok(a.dy) && ok(a.y) && ok(a.dx)) gn_pick_act<V>(a, f);
     else gn_pick_act<1>(a, f);
 }
 
@@ -642,8 +746,7 @@ template <typename T> static int gn_forward(const GnArgs &a, void *ws, hipStream
         const GnWork w = gn_work<V>(a);
         const dim3 grid((unsigned)(a.B * w.nchunk * w.nzb));
         hipLaunchKernelGGL((gn_stats_kernel<T, V>), grid, dim3(256), 0, s, a, w, part);
-        hipLaunchKernelGGL(gn_stats_join_kernel, dim3((unsigned)(a.B * a.G)), dim3(gn_join_threads(a, w)), 0, s, a, w, part);
-        hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, DROP>), grid, dim3(256), 0, s, a, w);
+        hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, DROP>), grid, dim3(256), (a.G + 256) * sizeof(float2), s, a, w, part);
     });
     return check_launch("group_norm_forward");
 }
@@ -661,18 +764,17 @@ template <typename T> static int gn_backward(const GnArgs &a, void *ws, hipStrea
                 else if (nv <= 4) hipLaunchKernelGGL((gn_slab_bwd_kernel<T, V, 4, ACT, DROP>), grid, dim3(512), lds, s, a, sl, part);
                 else if (nv <= 6) hipLaunchKernelGGL((gn_slab_bwd_kernel<T, V, 6, ACT, DROP>), grid, dim3(512), lds, s, a, sl, part);
                 else hipLaunchKernelGGL((gn_slab_bwd_kernel<T, V, 12, ACT, DROP>), grid, dim3(512), lds, s, a, sl, part);
-                GnWork w = {};
-                w.nchunk = 1;
-                hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)((a.C + 15) / 16)), dim3(1024), 0, s, a, w, part, (float2 *)nullptr, 0);
+                hipLaunchKernelGGL(gn_param_grads_kernel, dim3((unsigned)((a.C + 15) / 16)), dim3(1024), 0, s, a, a.B, part);
                 return;
             }
         }
         const GnWork w = gn_work<V>(a);
         const dim3 grid((unsigned)(a.B * w.nchunk * w.nzb));
-        float2 *gsum = (float2 *)ws, *part = gsum + (size_t)a.B * a.G;
-        hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT, DROP>), grid, dim3(256), 0, s, a, w, part);
-        hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)(a.B * a.G + (a.C + 15) / 16)), dim3(1024), 0, s, a, w, part, gsum, a.B * a.G);
-        hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, DROP>), grid, dim3(256), 0, s, a, w, gsum);
+        float2 *gpart = (float2 *)ws, *part = gpart + (size_t)a.B * w.nchunk * w.nsub * a.G;
+        const int nparam = (a.C + 127) / 128 * 8;                // whole eights: a chunk stays on the XCD that pass 1 read it on
+        hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT, DROP>), grid, dim3(256), 0, s, a, w, part, gpart);
+        hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, DROP>), dim3(grid.x + nparam), dim3(256), (a.G + 272) * sizeof(float2), s, a, w,
+                           part, gpart, nparam);
     });
     return check_launch("group_norm_backward");
 }
