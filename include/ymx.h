@@ -129,8 +129,8 @@ int ymx_conv2d_fused_ex(const void *x, const void *w, const void *scale, const v
  * are rounded to nearest even; NaN and infinities become NaN.
  *
  * A quantised map of n_pix pixels is one buffer of ymx_quantized_bytes(n_pix, C) bytes: the e4m3
- * bytes [n_pix][C], padding to a multiple of 256 bytes, then [n_pix][S] exponent bytes k + 127, of
- * which the first ceil(C / 128) are set, S = that number rounded up to 4.  x of
+ * bytes [n_pix][C], padding to a multiple of 256 bytes, then a plane of exponent bytes k + 127 for
+ * each block of channels, [ceil(C / 128)][n_pix rounded up to 4], the padding zero.  x of
  * ymx_quantize_blocks is fp32 or bf16 with pixel stride x_ld (elements, a multiple of 8; 0 = dense). */
 size_t ymx_quantized_bytes(long long n_pix, int C);
 int ymx_quantize_blocks(const void *x, void *q, long long n_pix, int C, int dtype, int x_ld, void *stream);

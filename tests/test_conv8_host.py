@@ -11,11 +11,11 @@ def test_entry_points_validate_without_gpu():
     from yolo_amd import _lib
     L = _lib.lib()
     one, odd = ctypes.c_void_p(256), ctypes.c_void_p(260)
-    assert L.ymx_packed_weight_bytes(3, 512, 1024, _lib.F8E4M3) == 1024 * 36 * (128 + 4)
-    assert L.ymx_packed_weight_bytes(1, 1024, 255, _lib.F8E4M3) == 256 * 8 * (128 + 4)
-    assert L.ymx_packed_weight_bytes(3, 144, 16, _lib.F8E4M3) == 256 * 18 * (128 + 4)
+    assert L.ymx_packed_weight_bytes(3, 512, 1024, _lib.F8E4M3) == 1024 * 36 * (128 + 1)
+    assert L.ymx_packed_weight_bytes(1, 1024, 255, _lib.F8E4M3) == 256 * 8 * (128 + 1)
+    assert L.ymx_packed_weight_bytes(3, 144, 16, _lib.F8E4M3) == 256 * 18 * (128 + 1)
     assert L.ymx_packed_weight_bytes(3, 24, 16, _lib.F8E4M3) == 0 and L.ymx_packed_weight_bytes(5, 32, 16, _lib.F8E4M3) == 0
-    assert L.ymx_quantized_bytes(10, 48) == 512 + 10 * 4 and L.ymx_quantized_bytes(1, 640) == 768 + 8
+    assert L.ymx_quantized_bytes(10, 48) == 512 + 12 and L.ymx_quantized_bytes(1, 640) == 768 + 5 * 4
     assert L.ymx_quantized_bytes(0, 48) == 0
 
     def quant(x=one, q=one, n=4, c=32, dtype=_lib.BF16, ld=0):
@@ -55,7 +55,7 @@ def test_layers_check_before_the_device():
     assert c.is_8bit() and c.map_dtype(torch.zeros(1)) == torch.bfloat16
     assert not YOLOConv((3, 3, 32), dtype=F8, in_channels=3).is_8bit()
     assert not YOLOConv((3, 3, 32), dtype=torch.bfloat16, in_channels=32).is_8bit()
-    q = BlockQuantized(torch.zeros(2 * 256 + 16 * 4, dtype=torch.uint8), (1, 4, 4, 32))
+    q = BlockQuantized(torch.zeros(2 * 256 + 16, dtype=torch.uint8), (1, 4, 4, 32))
     assert tuple(q.values.shape) == (1, 4, 4, 32) and tuple(q.exponents.shape) == (1, 4, 4, 1)
     assert torch.equal(q.dequantize(), torch.zeros(1, 4, 4, 32))
     with pytest.raises(ValueError, match="quantised map"):

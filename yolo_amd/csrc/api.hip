@@ -145,8 +145,7 @@ static int conv_impl(const void *x, const void *w, const void *scale, const void
         if (Cin % 16 || (k != 1 && k != 3)) return fail(YMX_EUNSUPPORTED, "conv2d: 8-bit kernels take input channels in multiples of 16 and 1x1 or 3x3 windows (%d, %d)", Cin, k);
         if (a.x_ld != Cin) return fail(YMX_EARG, "conv2d: a quantised map is dense");
         if (!aligned16(x) || !aligned16(w)) return fail(YMX_EARG, "conv2d: x and w must be 16-byte aligned");
-        const uintptr_t mis = out_dtype == YMX_BF16 ? 1 : 3;
-        if (((uintptr_t)y & mis) || ((uintptr_t)residual & mis)) return fail(YMX_EARG, "conv2d: y/residual not aligned to their elements");
+        if (!aligned16(y) || (residual && !aligned16(residual))) return fail(YMX_EARG, "conv2d: y/residual must be 16-byte aligned");
         if (label) { *label = "f8"; return YMX_OK; }
         return launch_conv_f8(a, (long long)B * H * W, s);
     }

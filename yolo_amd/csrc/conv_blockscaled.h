@@ -1,0 +1,163 @@
+// Shared by the 8-bit block-scaled convolution kernels: argument block, exponent DMA, fragments, epilogue.
+#pragma once
+#include <type_traits>
+
+#include "conv_epilogue.h"
+
+namespace ymx {
+
+typedef __attribute__((ext_vector_type(8))) int i32x8_t;
+
+struct F8Args {
+    ConvArgs a;                  // x_ld = 1: pixel_geometry then counts pixels
+    const void *xs, *ws;         // exponents of the map [block][plane] and of the kernel [K tile][rows], bytes
+    unsigned xs_bytes, ws_bytes;
+    unsigned plane;              // pixels of the map, rounded up to 4
+    int rows, nkt, taps;         // padded output channels, K tiles, filter taps
+    unsigned taps_m, taps_s;     // fastdiv of the taps
+};
+
+template <int N> __device__ __forceinline__ void f8_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+// LDS-DMA of exponents, as lds_dma16: one byte per lane, zero-extended to the dword at lds_addr + 4 lane ...
+__device__ __forceinline__ void lds_dma_u8(const i32x4_t rsrc, unsigned lds_addr, unsigned voff) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\t"
+                 "s_mov_b32 m0, %2\n\t"
+                 "s_nop 4\n\t"
+                 "buffer_load_ubyte %1, %3, 0 offen lds\n\t"
+                 "s_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(voff), "s"(lds_addr), "s"(rsrc)
+                 : "memory");
+}
+// ... or four neighbouring bytes per lane.
+__device__ __forceinline__ void lds_dma4(const i32x4_t rsrc, unsigned lds_addr, unsigned voff) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\t"
+                 "s_mov_b32 m0, %2\n\t"
+                 "s_nop 4\n\t"
+                 "buffer_load_dword %1, %3, 0 offen lds\n\t"
+                 "s_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(voff), "s"(lds_addr), "s"(rsrc)
+                 : "memory");
+}
+
+__device__ __forceinline__ i32x8_t f8_frag(const int4 &lo, const int4 &hi) {
+    return i32x8_t{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+}
+// 16 x 16 results += 128 products each, scaled by the row's and the column's power of two.
+__device__ __forceinline__ f32x4_t f8_mfma(const i32x8_t &w, const i32x8_t &x, const f32x4_t &c, int ws, int xs) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 0, 0, 0, ws, 0, xs);
+}
+
+// A fragment's 32 values as bf16, which holds every e4m3 number: eight at a time, in the order they lie in.
+__device__ __forceinline__ void f8_to_bf16(const i32x8_t &v, bf16x8_t (&o)[4]) {
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            w[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)v[2 * h + i], 1.0f, false));
+            w[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)v[2 * h + i], 1.0f, true));
+        }
+        o[h] = __builtin_bit_cast(bf16x8_t, uint4{w[0], w[1], w[2], w[3]});
+    }
+}
+
+// Rows of the fp32 accumulator image in LDS (see conv_epilogue.h for the layout) with 32-bit outputs, whose residual is
+// 32-bit too, and of any output whose channel count or pixel stride is no multiple of 8 (the 255 channels
+// of the logits): there a lane takes one channel and the wave 64 neighbouring ones of a pixel at a time.
+template <typename OT, int NI, int NJ>
+__device__ __forceinline__ void f8_epilogue_rows(const ConvArgs &a, f32x4_t (&acc)[NI][NJ], char *tbase, int cbase, int pbase, int lane) {
+    constexpr int HQ = NI * 16 < 64 ? NI * 16 : 64, NH = NI * 16 / HQ, SLOTS = HQ / 4, LPP = SLOTS / 2, PPI = 64 / LPP, NPASS = 16 * NJ / PPI;
+    OT *__restrict__ y = (OT *)a.y;
+    const OT *__restrict__ res = (const OT *)a.res;
+    const bool vec = sizeof(OT) == 4 && epi_vec_ok(a);
+    auto rows = [&](auto act_tag) {
+        constexpr int ACT = decltype(act_tag)::value;
+#pragma unroll
+        for (int half = 0; half < NH; ++half) {
+#pragma unroll
+            for (int il = 0; il < HQ / 16; ++il) {
+                const int slot = il * 4 + (lane >> 4);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    const int px = j * 16 + (lane & 15);
+                    *(f32x4_t *)(tbase + px * (HQ * 4) + ((slot ^ (px & (SLOTS - 1))) << 4)) = acc[half * (HQ / 16) + il][j];
+                }
+            }
+            const int c0 = cbase + half * HQ;
+            if (sizeof(OT) == 4 && vec) {
+                const int sl = lane % LPP, co = c0 + sl * 8;
+                float sc[8], sh[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    const bool in = co + r < a.Cout;
+                    sc[r] = in ? (a.scale ? a.scale[co + r] : 1.0f) : 0.0f;
+                    sh[r] = (in && a.shift) ? a.shift[co + r] : 0.0f;
+                }
+#pragma unroll 2
+                for (int n = 0; n < NPASS; ++n) {
+                    const int px = n * PPI + lane / LPP, p = pbase + px, sw = px & (SLOTS - 1);
+                    const char *row = tbase + px * (HQ * 4);
+                    const float4 v0 = *(const float4 *)(row + (((2 * sl) ^ sw) << 4));
+                    const float4 v1 = *(const float4 *)(row + (((2 * sl + 1) ^ sw) << 4));
+                    float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+                    if (p >= a.P || co >= a.Cout) continue;
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) v[r] = act_c<ACT>(affine_f(v[r], sc[r], sh[r]));
+                    if (res) {
+                        const float4 q0 = *(const float4 *)(res + (size_t)p * a.res_ld + co), q1 = *(const float4 *)(res + (size_t)p * a.res_ld + co + 4);
+                        v[0] = __fadd_rn(v[0], q0.x); v[1] = __fadd_rn(v[1], q0.y); v[2] = __fadd_rn(v[2], q0.z); v[3] = __fadd_rn(v[3], q0.w);
+                        v[4] = __fadd_rn(v[4], q1.x); v[5] = __fadd_rn(v[5], q1.y); v[6] = __fadd_rn(v[6], q1.z); v[7] = __fadd_rn(v[7], q1.w);
+                    }
+                    float *yp = (float *)y + (size_t)p * a.y_ld + co;
+                    store_stream16(yp, v[0], v[1], v[2], v[3]);
+                    store_stream16(yp + 4, v[4], v[5], v[6], v[7]);
+                }
+            } else {
+                const int cl = lane % HQ, co = c0 + cl;              // HQ lanes per pixel, 64 / HQ pixels at a time
+                const bool in = co < a.Cout;
+                const float sc = in && a.scale ? a.scale[co] : 1.0f, sh = in && a.shift ? a.shift[co] : 0.0f;
+#pragma unroll 4
+                for (int n = 0; n < 16 * NJ / (64 / HQ); ++n) {
+                    const int px = n * (64 / HQ) + lane / HQ, p = pbase + px;
+                    float v = *(const float *)(tbase + px * (HQ * 4) + (((cl >> 2) ^ (px & (SLOTS - 1))) << 4) + (cl & 3) * 4);
+                    if (p >= a.P || !in) continue;
+                    v = act_c<ACT>(affine_f(v, sc, sh));
+                    if (res) v = __fadd_rn(v, elem<OT>::load(res + (size_t)p * a.res_ld + co));
+                    elem<OT>::store(y + (size_t)p * a.y_ld + co, v);
+                }
+            }
+        }
+    };
+    if (a.act == YMX_ACT_MISH) rows(std::integral_constant<int, YMX_ACT_MISH>{});
+    else if (a.act == YMX_ACT_LEAKY) rows(std::integral_constant<int, YMX_ACT_LEAKY>{});
+    else rows(std::integral_constant<int, YMX_ACT_NONE>{});
+}
+
+// The end of a tile, after every wave's last LDS read: acc -> finished rows, by way of the wave's own part of LDS.
+template <typename OT, int NI, int NJ>
+__device__ __forceinline__ void f8_epilogue(const ConvArgs &a, f32x4_t (&acc)[NI][NJ], char *smem, int wave, int cbase, int pbase, int lane) {
+    typedef EpiGeom<NI, 64, 16 * NJ> Epi;
+    char *tbase = smem + wave * Epi::LDS_BYTES;
+    if (sizeof(OT) == 2 && epi_vec_ok(a) && (a.res == nullptr || a.res_bytes != 0)) {
+        epi_u32x4_t rpre[Epi::NH][Epi::NPASS];
+        if (epi_res_pre(a)) {
+            epi_load_res<NI, 64, 16 * NJ>(a, 0, cbase, pbase, lane, rpre[0]);
+        } else {
+#pragma unroll
+            for (int n = 0; n < Epi::NPASS; ++n) rpre[0][n] = epi_u32x4_t{0u, 0u, 0u, 0u};
+        }
+        epi_run<bf16_t, NI, NJ>(a, acc, tbase, cbase, pbase, lane, rpre);
+    } else {
+        f8_epilogue_rows<OT, NI, NJ>(a, acc, tbase, cbase, pbase, lane);
+    }
+}
+
+bool conv_f8_wide(const F8Args &g);
+int launch_conv_f8_wide(const F8Args &g, hipStream_t s);
+
+}  // namespace ymx

@@ -18,20 +18,17 @@
 // bf16 instructions, whose products and sums are exact to fp32 (e4m3 numbers are bf16 numbers), at half
 // the rate, the block's sum being scaled by v_ldexp on its way into the accumulator.
 //
-// Quantised map (ymx_quantize_blocks):  [pixel][C] e4m3 bytes (padded to 256), then
-// [pixel][4 ceil(nb / 4)] exponent bytes (k + 127; nb = ceil(C / 128)).
+// Quantised map (ymx_quantize_blocks):  [pixel][C] e4m3 bytes (padded to 256), then one plane of
+// exponent bytes (k + 127) per block of channels, [block][pixels rounded up to 4], the padding zero.
 // Packed kernel (ymx_pack_weights):  [channel, padded to 256][K tile][128] bytes, then
-// [K tile][channel] exponents as dwords.  K tile = (block of 128 input channels) * taps + tap, so
-// that the taps of a block, which read the same pixels, follow one another; channels past the
-// input's last are zeros.
+// [K tile][channel] exponent bytes.  K tile = (block of 128 input channels) * taps + tap, so that
+// the taps of a block, which read the same pixels, follow one another; channels past the input's
+// last are zeros.
 #include <algorithm>
-#include <type_traits>
 
-#include "conv_epilogue.h"
+#include "conv_blockscaled.h"
 
 namespace ymx {
-
-typedef __attribute__((ext_vector_type(8))) int i32x8_t;
 
 // ---- quantisation ---------------------------------------------------------------------------------
 // The block's exponent from the bits of its largest finite magnitude: 1.75 * 2^8 = 448.
@@ -55,22 +52,25 @@ __device__ __forceinline__ uint32_t f8_pack4(float a, float b, float c, float d)
 }
 
 static size_t f8_map_bytes(long long n_pix, int C) { return ((size_t)n_pix * C + 255) / 256 * 256; }
-static int f8_scale_ld(int C) { return ((C + 127) / 128 + 3) / 4 * 4; }
-size_t quant_bytes(long long n_pix, int C) { return f8_map_bytes(n_pix, C) + (size_t)n_pix * f8_scale_ld(C); }
+static long long f8_plane(long long n_pix) { return (n_pix + 3) / 4 * 4; }
+size_t quant_bytes(long long n_pix, int C) { return f8_map_bytes(n_pix, C) + (size_t)f8_plane(n_pix) * ((C + 127) / 128); }
 
 // GL lanes of 8 channels share a block of one pixel (16 lanes = 128 channels; 8 or 4 where the map has no more
-// than 64 or 32).  Reads 2 or 4 bytes a value, writes one: bound by memory.
+// than 64 or 32); a wave takes 64 / GL neighbouring pixels of one block, so that four exponents leave as a dword.
+// Reads 2 or 4 bytes a value, writes one: bound by memory (5.4 TB/s on a 177 MB map).
 template <typename T, int GL>
 __global__ void __launch_bounds__(256)
 quantize_kernel(const T *__restrict__ x, int x_ld, unsigned char *__restrict__ q, unsigned char *__restrict__ scales, long long n_pix,
-                int C, int nb, int s_ld) {
-    const long long groups = n_pix * nb;
-    const int gl = threadIdx.x % GL;
-    for (long long g = ((long long)blockIdx.x * 256 + threadIdx.x) / GL; g < groups; g += (long long)gridDim.x * (256 / GL)) {
-        const long long p = nb == 1 ? g : g / nb;
-        const int blk = nb == 1 ? 0 : (int)(g - p * nb);
+                int C, int nb, long long plane) {
+    constexpr int NPX = 64 / GL;
+    const long long units = (n_pix + NPX - 1) / NPX * nb;
+    const int lane = threadIdx.x & 63, gl = lane % GL;
+    for (long long u = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); u < units; u += (long long)gridDim.x * 4) {
+        const long long run = nb == 1 ? u : u / nb;
+        const int blk = nb == 1 ? 0 : (int)(u - run * nb);
+        const long long p = run * NPX + lane / GL;
         const int c = blk * 128 + gl * 8;
-        const bool on = c < C;
+        const bool on = c < C && p < n_pix;
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = 0.0f;
@@ -100,7 +100,11 @@ quantize_kernel(const T *__restrict__ x, int x_ld, unsigned char *__restrict__ q
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = f8_scaled(v[i], f);
         if (on) *(uint2 *)(q + (size_t)p * C + c) = uint2{f8_pack4(v[0], v[1], v[2], v[3]), f8_pack4(v[4], v[5], v[6], v[7])};
-        if (gl == 0) scales[(size_t)p * s_ld + blk] = (unsigned char)(k + 127);
+        // exponents of four neighbouring pixels -> the first one's leading lane (0 behind the last pixel)
+        uint32_t e = p < n_pix ? (uint32_t)(k + 127) : 0u;
+        e |= (uint32_t)__shfl_down((int)e, GL) << 8;
+        e |= (uint32_t)__shfl_down((int)e, 2 * GL) << 16;
+        if (lane % (4 * GL) == 0 && p < n_pix) *(uint32_t *)(scales + (size_t)blk * plane + p) = e;
     }
 }
 
@@ -110,9 +114,9 @@ int launch_quantize(const void *x, int x_ld, void *q, long long n_pix, int C, in
     auto go = [&](auto ttag, auto gtag) {
         typedef decltype(ttag) T;
         constexpr int GL = decltype(gtag)::value;
-        const long long wgs = (n_pix * nb * GL + 255) / 256;
-        hipLaunchKernelGGL((quantize_kernel<T, GL>), dim3((unsigned)std::min<long long>(wgs, 16384)), dim3(256), 0, s, (const T *)x, x_ld,
-                           (unsigned char *)q, sc, n_pix, C, nb, f8_scale_ld(C));
+        const long long units = (n_pix + 64 / GL - 1) / (64 / GL) * nb;
+        hipLaunchKernelGGL((quantize_kernel<T, GL>), dim3((unsigned)std::min<long long>((units + 3) / 4, 16384)), dim3(256), 0, s, (const T *)x, x_ld,
+                           (unsigned char *)q, sc, n_pix, C, nb, f8_plane(n_pix));
     };
     auto lanes = [&](auto ttag) {
         if (C > 64) go(ttag, std::integral_constant<int, 16>{});
@@ -127,11 +131,11 @@ int launch_quantize(const void *x, int x_ld, void *q, long long n_pix, int C, in
 // ---- packed kernels -------------------------------------------------------------------------------
 static int f8_rows(int Cout) { return (Cout + 255) / 256 * 256; }
 static int f8_tiles(int k, int Cin) { return (Cin + 127) / 128 * k * k; }
-size_t packed_f8_bytes(int k, int Cin, int Cout) { return (size_t)f8_rows(Cout) * f8_tiles(k, Cin) * (128 + 4); }
+size_t packed_f8_bytes(int k, int Cin, int Cout) { return (size_t)f8_rows(Cout) * f8_tiles(k, Cin) * (128 + 1); }
 
 // One thread per (output channel, K tile); neighbouring threads read neighbouring channels.
 __global__ void __launch_bounds__(256)
-pack_f8_kernel(const float *__restrict__ w, unsigned char *__restrict__ out, uint32_t *__restrict__ scales, int taps, int Cin, int Cout, int rows, int nkt) {
+pack_f8_kernel(const float *__restrict__ w, unsigned char *__restrict__ out, unsigned char *__restrict__ scales, int taps, int Cin, int Cout, int rows, int nkt) {
     const int co = blockIdx.x * 256 + threadIdx.x, kt = blockIdx.y;
     const int blk = kt / taps, tap = kt - blk * taps;
     const int c0 = blk * 128, nc = min(128, Cin - c0);
@@ -148,137 +152,18 @@ pack_f8_kernel(const float *__restrict__ w, unsigned char *__restrict__ out, uin
         for (int i = 0; i < 4; ++i) v[i] = (co < Cout && c + i < nc) ? f8_scaled(src[(size_t)(c + i) * Cout], f) : 0.0f;
         dst[c >> 2] = f8_pack4(v[0], v[1], v[2], v[3]);
     }
-    scales[(size_t)kt * rows + co] = (uint32_t)(k + 127);
+    scales[(size_t)kt * rows + co] = (unsigned char)(k + 127);
 }
 
 int launch_pack_f8(const float *w_hwio, void *packed, int k, int Cin, int Cout, hipStream_t s) {
     const int rows = f8_rows(Cout), nkt = f8_tiles(k, Cin);
     unsigned char *out = (unsigned char *)packed;
-    hipLaunchKernelGGL(pack_f8_kernel, dim3(rows / 256, nkt), dim3(256), 0, s, w_hwio, out, (uint32_t *)(out + (size_t)rows * nkt * 128), k * k, Cin, Cout,
-                       rows, nkt);
+    hipLaunchKernelGGL(pack_f8_kernel, dim3(rows / 256, nkt), dim3(256), 0, s, w_hwio, out, out + (size_t)rows * nkt * 128, k * k, Cin, Cout, rows,
+                       nkt);
     return check_launch("pack_weights");
 }
 
 // ---- the product ----------------------------------------------------------------------------------
-// One LDS-DMA wave-instruction of dwords: lane l's 4 bytes land at lds_addr + 4 l (see lds_dma16).
-__device__ __forceinline__ void lds_dma4(const i32x4_t rsrc, unsigned lds_addr, unsigned voff) {
-    unsigned keep;
-    asm volatile("s_mov_b32 %0, m0\n\t"
-                 "s_mov_b32 m0, %2\n\t"
-                 "s_nop 4\n\t"
-                 "buffer_load_dword %1, %3, 0 offen lds\n\t"
-                 "s_mov_b32 m0, %0"
-                 : "=&s"(keep)
-                 : "v"(voff), "s"(lds_addr), "s"(rsrc)
-                 : "memory");
-}
-template <int N> __device__ __forceinline__ void f8_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
-
-struct F8Args {
-    ConvArgs a;                  // x_ld = 1: pixel_geometry then counts pixels; k_m, k_s as in ConvArgs
-    const void *xs, *ws;         // exponents of the map and of the kernel
-    unsigned xs_bytes, ws_bytes;
-    int s_ld, rows, nkt, taps;   // exponent bytes per pixel, padded output channels, K tiles
-    unsigned taps_m, taps_s;     // fastdiv of the taps
-};
-
-// A fragment's 32 values as bf16, which holds every e4m3 number: eight at a time, in the order they lie in.
-__device__ __forceinline__ void f8_to_bf16(const i32x8_t &v, bf16x8_t (&o)[4]) {
-#pragma unroll
-    for (int h = 0; h < 4; ++h) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            w[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)v[2 * h + i], 1.0f, false));
-            w[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)v[2 * h + i], 1.0f, true));
-        }
-        o[h] = __builtin_bit_cast(bf16x8_t, uint4{w[0], w[1], w[2], w[3]});
-    }
-}
-
-// Finished rows from a wave's accumulators (16 NI channels x 64 pixels, a lane holding 4 channels of one
-// pixel per block), by way of a private LDS image as in conv_epilogue.h.  The residual has the output's type.
-template <typename OT, int NI>
-__device__ __forceinline__ void f8_epilogue(const ConvArgs &a, f32x4_t (&acc)[NI][4], char *tbase, int cbase, int pbase, int lane) {
-    constexpr int HQ = NI * 16 < 64 ? NI * 16 : 64, NH = NI * 16 / HQ, SLOTS = HQ / 4, LPP = SLOTS / 2, PPI = 64 / LPP, NPASS = 64 / PPI;
-    OT *__restrict__ y = (OT *)a.y;
-    const OT *__restrict__ res = (const OT *)a.res;
-    const int sl = lane % LPP;
-    const bool vec = (a.Cout & 7) == 0 && (a.y_ld & 7) == 0 && ((uintptr_t)y & 15) == 0 &&
-                     (res == nullptr || ((a.res_ld & 7) == 0 && ((uintptr_t)res & 15) == 0));
-    auto rows = [&](auto act_tag, auto vec_tag) {
-        constexpr int ACT = decltype(act_tag)::value;
-        constexpr bool VEC = decltype(vec_tag)::value;
-#pragma unroll
-        for (int half = 0; half < NH; ++half) {
-#pragma unroll
-            for (int il = 0; il < HQ / 16; ++il) {
-                const int slot = il * 4 + (lane >> 4);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int px = j * 16 + (lane & 15);
-                    *(f32x4_t *)(tbase + px * (HQ * 4) + ((slot ^ (px & (SLOTS - 1))) << 4)) = acc[half * (HQ / 16) + il][j];
-                }
-            }
-            const int co = cbase + half * HQ + sl * 8;
-            float sc[8], sh[8];
-#pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                const bool in = co + r < a.Cout;
-                sc[r] = in ? (a.scale ? a.scale[co + r] : 1.0f) : 0.0f;
-                sh[r] = (in && a.shift) ? a.shift[co + r] : 0.0f;
-            }
-#pragma unroll 2
-            for (int n = 0; n < NPASS; ++n) {
-                const int px = n * PPI + lane / LPP, p = pbase + px;
-                const char *row = tbase + px * (HQ * 4);
-                const int sw = px & (SLOTS - 1);
-                const float4 v0 = *(const float4 *)(row + (((2 * sl) ^ sw) << 4));
-                const float4 v1 = *(const float4 *)(row + (((2 * sl + 1) ^ sw) << 4));
-                float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-                if (p >= a.P || co >= a.Cout) continue;
-#pragma unroll
-                for (int r = 0; r < 8; ++r) v[r] = act_c<ACT>(affine_f(v[r], sc[r], sh[r]));
-                OT *yp = y + (size_t)p * a.y_ld + co;
-                const OT *rp = res + (size_t)p * a.res_ld + co;
-                if constexpr (VEC) {
-                    if constexpr (sizeof(OT) == 2) {
-                        if (res) {
-                            const uint4 q = *(const uint4 *)rp;
-                            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                v[2 * r] += __uint_as_float(w[r] << 16);
-                                v[2 * r + 1] += __uint_as_float(w[r] & 0xffff0000u);
-                            }
-                        }
-                        store_stream16(yp, pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]), pack2_bf16(v[4], v[5]), pack2_bf16(v[6], v[7]));
-                    } else {
-                        if (res) {
-                            const float4 q0 = *(const float4 *)rp, q1 = *(const float4 *)(rp + 4);
-                            v[0] += q0.x; v[1] += q0.y; v[2] += q0.z; v[3] += q0.w;
-                            v[4] += q1.x; v[5] += q1.y; v[6] += q1.z; v[7] += q1.w;
-                        }
-                        store_stream16(yp, v[0], v[1], v[2], v[3]);
-                        store_stream16(yp + 4, v[4], v[5], v[6], v[7]);
-                    }
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 8; ++r)
-                        if (co + r < a.Cout) elem<OT>::store(yp + r, res ? v[r] + elem<OT>::load(rp + r) : v[r]);
-                }
-            }
-        }
-    };
-    auto pick = [&](auto act_tag) {
-        if (vec) rows(act_tag, std::true_type{});
-        else rows(act_tag, std::false_type{});
-    };
-    if (a.act == YMX_ACT_MISH) pick(std::integral_constant<int, YMX_ACT_MISH>{});
-    else if (a.act == YMX_ACT_LEAKY) pick(std::integral_constant<int, YMX_ACT_LEAKY>{});
-    else pick(std::integral_constant<int, YMX_ACT_NONE>{});
-}
-
 // NWQ x NWP waves, each 16 NI channels x 64 pixels; K tiles of 128 channels of one tap through NSTAGE stages
 // of LDS, filled by LDS-DMA NSTAGE - 1 tiles ahead, one barrier per tile.  Rows are 128 bytes (one pixel's or one
 // channel's 128 values), the 16-byte chunk c of row r in slot c ^ (r & 7): the lanes that read one fragment then
@@ -311,8 +196,8 @@ conv_f8_kernel(const F8Args g, const int ntile_q) {
     for (int i = 0; i < NXI; ++i) pixel_geometry(a, p0 + (wave * NXI + i) * 8 + srow, xpix[i], xmask[i]);
     const unsigned woff = (unsigned)(q0 + wave * NWI * 8 + srow) * (unsigned)(g.nkt * 128) + (unsigned)chunk * 16u;
     const unsigned wstep = 8u * (unsigned)(g.nkt * 128);
-    // exponents: instructions 0 .. TP/64 - 1 fetch a dword (four blocks) per pixel, the others a dword per channel;
-    // waves past the last one repeat it
+    // exponents: instructions 0 .. TP/64 - 1 fetch those of 64 pixels, the others those of 64 channels; waves past
+    // the last instruction repeat it
     const int si = min(wave, NS - 1);
     int spix = 0;
     unsigned smask = 0;
@@ -336,13 +221,13 @@ conv_f8_kernel(const F8Args g, const int ntile_q) {
         unsigned so;
         i32x4_t sr;
         if (si < TP / 64) {
-            so = (smask & bit) ? (unsigned)(spix + tpix) * (unsigned)g.s_ld + (unsigned)(blk & ~3) : OOB;
+            so = (smask & bit) ? (unsigned)blk * g.plane + (unsigned)(spix + tpix) : OOB;
             sr = xsr;
         } else {
-            so = on ? ((unsigned)kt * (unsigned)g.rows + (unsigned)(q0 + (si - TP / 64) * 64 + lane)) * 4u : OOB;
+            so = on ? (unsigned)kt * (unsigned)g.rows + (unsigned)(q0 + (si - TP / 64) * 64 + lane) : OOB;
             sr = wsr;
         }
-        lds_dma4(sr, sb + (unsigned)(XB + WB + si * 256), so);
+        lds_dma_u8(sr, sb + (unsigned)(XB + WB + si * 256), so);
     };
 
     f32x4_t acc[NI][NJ];
@@ -356,20 +241,16 @@ conv_f8_kernel(const F8Args g, const int ntile_q) {
     const int a_off = XB + (wq * NI * 16 + frow) * 128, b_off = (wp * 64 + frow) * 128;
     const int as_off = XB + WB + (TP + wq * NI * 16 + frow) * 4, bs_off = XB + WB + (wp * 64 + frow) * 4;
 
-    auto frag = [&](const char *p) {
-        const int4 lo = *(const int4 *)(p + s0), hi = *(const int4 *)(p + s1);
-        return i32x8_t{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-    };
+    auto frag = [&](const char *p) { return f8_frag(*(const int4 *)(p + s0), *(const int4 *)(p + s1)); };
     // 32-bit outputs: the same fragments as bf16 (exact), the block's sum scaled and added by the vector unit
-    auto compute_exact = [&](int kt, int stage) {
+    auto compute_exact = [&](int stage) {
         const char *base = smem + stage * STAGE;
-        const int sh = (fastdiv(kt, g.taps_m, g.taps_s) & 3) * 8;
         bf16x8_t b[NJ][4];
         int bs[NJ];
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             f8_to_bf16(frag(base + b_off + j * 2048), b[j]);
-            bs[j] = (int)((*(const uint32_t *)(base + bs_off + j * 64) >> sh) & 255u) - 254;
+            bs[j] = *(const int *)(base + bs_off + j * 64) - 254;
         }
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
@@ -388,16 +269,15 @@ conv_f8_kernel(const F8Args g, const int ntile_q) {
             }
         }
     };
-    auto compute = [&](int kt, int stage) {
-        if constexpr (sizeof(OT) == 4) return compute_exact(kt, stage);
+    auto compute = [&](int stage) {
+        if constexpr (sizeof(OT) == 4) return compute_exact(stage);
         const char *base = smem + stage * STAGE;
-        const int sh = (fastdiv(kt, g.taps_m, g.taps_s) & 3) * 8;
         i32x8_t b[NJ];
         int bs[NJ];
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             b[j] = frag(base + b_off + j * 2048);
-            bs[j] = (int)(*(const uint32_t *)(base + bs_off + j * 64) >> sh);
+            bs[j] = *(const int *)(base + bs_off + j * 64);
         }
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
@@ -405,7 +285,7 @@ conv_f8_kernel(const F8Args g, const int ntile_q) {
             const int ws = *(const int *)(base + as_off + i * 64);
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, b[j], acc[i][j], 0, 0, 0, ws, 0, bs[j]);
+                acc[i][j] = f8_mfma(w, b[j], acc[i][j], ws, bs[j]);
         }
     };
 
@@ -416,20 +296,19 @@ conv_f8_kernel(const F8Args g, const int ntile_q) {
     int st = 0;
     for (int kt = 0; kt < g.nkt; ++kt) {
         dma(kt + NSTAGE - 1, st == 0 ? NSTAGE - 1 : st - 1);
-        compute(kt, st);
+        compute(st);
         f8_vmcnt<PIECES * (NSTAGE - 2)>();
         __syncthreads();
         st = st + 1 == NSTAGE ? 0 : st + 1;
     }
     f8_vmcnt<0>();
     __syncthreads();
-    constexpr int EPI = 64 * (NI * 16 < 64 ? NI * 16 : 64) * 4;
-    f8_epilogue<OT, NI>(a, acc, smem + wave * EPI, q0 + wq * NI * 16, p0 + wp * 64, lane);
+    f8_epilogue<OT, NI, NJ>(a, acc, smem, wave, q0 + wq * NI * 16, p0 + wp * 64, lane);
 }
 
 template <typename OT, int NWQ, int NWP, int NI, int NSTAGE> static int launch_f8_cfg(const F8Args &g, hipStream_t s) {
     constexpr int TQ = NWQ * NI * 16, TP = NWP * 64, NW = NWQ * NWP;
-    constexpr int PIPE = NSTAGE * ((TP + TQ) * 128 + (TP + TQ) / 64 * 256), EPI = NW * 64 * (NI * 16 < 64 ? NI * 16 : 64) * 4;
+    constexpr int PIPE = NSTAGE * ((TP + TQ) * 128 + (TP + TQ) / 64 * 256), EPI = NW * EpiGeom<NI, 64, 64>::LDS_BYTES;
     constexpr int LDS = PIPE > EPI ? PIPE : EPI;
     auto kern = conv_f8_kernel<OT, NWQ, NWP, NI, NSTAGE>;
     static LdsReserve reserved;
@@ -458,17 +337,21 @@ int launch_conv_f8(const ConvArgs &args, long long in_pix, hipStream_t s) {
     g.taps = args.k * args.k;
     g.nkt = f8_tiles(args.k, args.Cin);
     g.rows = f8_rows(args.Cout);
-    g.s_ld = f8_scale_ld(args.Cin);
+    g.plane = (unsigned)f8_plane(in_pix);
     set_fastdiv((unsigned)g.taps, g.taps_m, g.taps_s);
     const unsigned long long xb = (unsigned long long)in_pix * args.Cin, wb = (unsigned long long)g.rows * g.nkt * 128;
-    if (xb >= (1ull << 31) || wb >= (1ull << 31) || (unsigned long long)in_pix * g.s_ld >= (1ull << 31))
+    if (xb >= (1ull << 31) || wb >= (1ull << 31) || (unsigned long long)g.plane * ((args.Cin + 127) / 128) >= (1ull << 31))
         return fail(YMX_EUNSUPPORTED, "conv2d: more than 2 GiB of 8-bit input or kernel");
     g.a.x_bytes = (unsigned)xb;
     g.a.w_bytes = (unsigned)wb;
     g.xs = (const char *)args.x + f8_map_bytes(in_pix, args.Cin);
-    g.xs_bytes = (unsigned)(in_pix * g.s_ld);
+    g.xs_bytes = g.plane * (unsigned)((args.Cin + 127) / 128);
     g.ws = (const char *)args.w + wb;
-    g.ws_bytes = (unsigned)((size_t)g.nkt * g.rows * 4);
+    g.ws_bytes = (unsigned)(g.nkt * g.rows);
+    if (args.res && args.out_dtype == YMX_BF16) {
+        const long long rb = ((long long)(args.P - 1) * args.res_ld + args.Cout) * 2;
+        g.a.res_bytes = rb < 0x80000000LL ? (unsigned)rb : 0u;
+    }
     return args.out_dtype == YMX_BF16 ? launch_f8_shape<bf16_t>(g, s) : launch_f8_shape<float>(g, s);
 }
 

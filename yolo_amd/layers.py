@@ -59,10 +59,10 @@ class BlockQuantized(object):
 
     @property
     def exponents(self):
-        n = self.shape.numel()
-        nb = -(-self.shape[-1] // 128)
-        tail = self.buffer[-(-n // 256) * 256:]
-        return tail.view(self.shape[:-1] + (-(-nb // 4) * 4,))[..., :nb]
+        n, nb = self.shape.numel(), -(-self.shape[-1] // 128)
+        pix = n // self.shape[-1]
+        planes = self.buffer[-(-n // 256) * 256:].view(nb, -(-pix // 4) * 4)
+        return planes[:, :pix].unflatten(1, self.shape[:-1]).movedim(0, -1)
 
     def dequantize(self, dtype=torch.float32):
         """The values the bytes stand for."""
@@ -436,9 +436,10 @@ class YOLOConv(nn.Module):
         y_ld = 0
         if out is not None:
             y_ld = self._check_out(out, b, oh, ow, odt, q.device)
+        if out is not None and out.data_ptr() % 16 == 0:
             y = out
         else:
-            y = torch.empty((b, oh, ow, cout), device=q.device, dtype=odt)
+            y, y_ld = torch.empty((b, oh, ow, cout), device=q.device, dtype=odt), 0
         if residual is not None:
             residual = _as_nhwc(residual)
             if residual.shape != y.shape:
@@ -446,6 +447,8 @@ class YOLOConv(nn.Module):
         fused = residual if self.act_fn is None else None
         if fused is not None and fused.dtype != odt:
             fused = fused.to(odt)
+        if fused is not None and fused.data_ptr() % 16:
+            fused = fused.clone()
         _lib.launch("ymx_conv2d_fused_ex", q, _lib.ptr(q.buffer), _lib.ptr(wp), _lib.ptr(scale), _lib.ptr(shift), _lib.ptr(fused),
                     _lib.ptr(y), b, h, w, cin, cout, k, 2 if self.downsample else 1, act_code, _lib.F8E4M3, _lib.F8E4M3,
                     _lib.dtype_code(odt), 0, 0, y_ld)
@@ -453,6 +456,8 @@ class YOLOConv(nn.Module):
             y = self.act_fn(y)
             if residual is not None:
                 y = residual + y
+        if out is not None and y is not out:
+            return out.copy_(y)                 # a slice that is not 16-byte aligned
         return y
 
     def _check_out(self, out, b, oh, ow, odt, device):
