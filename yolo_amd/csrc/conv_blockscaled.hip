@@ -321,10 +321,8 @@ template <typename OT, int NWQ, int NWP, int NI, int NSTAGE> static int launch_f
 }
 
 template <typename OT> static int launch_f8_shape(const F8Args &g, hipStream_t s) {
-    const long long big = (long long)((g.a.P + 255) / 256) * ((g.a.Cout + 255) / 256);
+    if (conv_f8_wide(g)) return launch_conv_f8_wide(g, s);
     const long long mid = (long long)((g.a.P + 127) / 128) * ((g.a.Cout + 127) / 128);
-    if constexpr (sizeof(OT) == 2)
-        if (big >= 160) return launch_f8_cfg<OT, 2, 4, 8, 2>(g, s);
     if (mid >= 160) return launch_f8_cfg<OT, 2, 2, 4, 2>(g, s);
     return launch_f8_cfg<OT, 4, 1, 1, 4>(g, s);
 }
