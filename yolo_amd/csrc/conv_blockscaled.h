@@ -19,30 +19,21 @@ struct F8Args {
 
 template <int N> __device__ __forceinline__ void f8_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
-// LDS-DMA of exponents, as lds_dma16: one byte per lane, zero-extended to the dword at lds_addr + 4 lane ...
-__device__ __forceinline__ void lds_dma_u8(const i32x4_t rsrc, unsigned lds_addr, unsigned voff) {
-    unsigned keep;
-    asm volatile("s_mov_b32 %0, m0\n\t"
-                 "s_mov_b32 m0, %2\n\t"
-                 "s_nop 4\n\t"
-                 "buffer_load_ubyte %1, %3, 0 offen lds\n\t"
-                 "s_mov_b32 m0, %0"
-                 : "=&s"(keep)
-                 : "v"(voff), "s"(lds_addr), "s"(rsrc)
-                 : "memory");
-}
-// ... or four neighbouring bytes per lane.
-__device__ __forceinline__ void lds_dma4(const i32x4_t rsrc, unsigned lds_addr, unsigned voff) {
-    unsigned keep;
-    asm volatile("s_mov_b32 %0, m0\n\t"
-                 "s_mov_b32 m0, %2\n\t"
-                 "s_nop 4\n\t"
-                 "buffer_load_dword %1, %3, 0 offen lds\n\t"
-                 "s_mov_b32 m0, %0"
-                 : "=&s"(keep)
-                 : "v"(voff), "s"(lds_addr), "s"(rsrc)
-                 : "memory");
-}
+// One LDS-DMA wave-instruction: lane l's 16 bytes (4 bytes; one byte, zero-extended to 4) at buffer offset voff land at
+// lds_addr + 16 l (4 l), zeros where voff is out of range.  Inline asm on purpose, see lds_dma16; the caller counts them
+// (vmcnt) and waits before a barrier.  M0 is not restored: the compiler reserves it and sets it before each use of its own.
+// That, and one wait state instead of five, makes 30 cycles less of the issue of each; operands are scalars computed long
+// before (f8_dma_ready before the first).
+#define YMX_F8_DMA(NAME, OP)                                                                                     \
+    __device__ __forceinline__ void NAME(const i32x4_t rsrc, unsigned lds_addr, unsigned voff) {                 \
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\t" OP " %0, %2, 0 offen lds"                                \
+                     :: "v"(voff), "s"(lds_addr), "s"(rsrc) : "memory");                                         \
+    }
+YMX_F8_DMA(f8_dma16, "buffer_load_dwordx4")
+YMX_F8_DMA(f8_dma4, "buffer_load_dword")
+YMX_F8_DMA(f8_dma_u8, "buffer_load_ubyte")
+#undef YMX_F8_DMA
+__device__ __forceinline__ void f8_dma_ready() { asm volatile("s_nop 7" ::: "memory"); }
 
 __device__ __forceinline__ i32x8_t f8_frag(const int4 &lo, const int4 &hi) {
     return i32x8_t{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
@@ -52,15 +43,17 @@ __device__ __forceinline__ f32x4_t f8_mfma(const i32x8_t &w, const i32x8_t &x, c
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 0, 0, 0, ws, 0, xs);
 }
 
-// A fragment's 32 values as bf16, which holds every e4m3 number: eight at a time, in the order they lie in.
-__device__ __forceinline__ void f8_to_bf16(const i32x8_t &v, bf16x8_t (&o)[4]) {
+// A fragment's 32 values times 2^(exponent byte - 127) as bf16: eight at a time, in the order they lie in.  Exact down to
+// 2^-126, bf16 having e4m3's digits and fp32's exponents.
+__device__ __forceinline__ void f8_to_bf16(const i32x8_t &v, int exponent, bf16x8_t (&o)[4]) {
+    const float f = __uint_as_float((uint32_t)exponent << 23);
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            w[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)v[2 * h + i], 1.0f, false));
-            w[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)v[2 * h + i], 1.0f, true));
+            w[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)v[2 * h + i], f, false));
+            w[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)v[2 * h + i], f, true));
         }
         o[h] = __builtin_bit_cast(bf16x8_t, uint4{w[0], w[1], w[2], w[3]});
     }
@@ -143,7 +136,9 @@ template <typename OT, int NI, int NJ>
 __device__ __forceinline__ void f8_epilogue(const ConvArgs &a, f32x4_t (&acc)[NI][NJ], char *smem, int wave, int cbase, int pbase, int lane) {
     typedef EpiGeom<NI, 64, 16 * NJ> Epi;
     char *tbase = smem + wave * Epi::LDS_BYTES;
-    if (sizeof(OT) == 2 && epi_vec_ok(a) && (a.res == nullptr || a.res_bytes != 0)) {
+    constexpr bool WIDE = sizeof(OT) == 2 && NJ >= 3;
+    if (WIDE && epi_vec_ok(a) && (a.res == nullptr || a.res_bytes != 0)) {
+      if constexpr (WIDE) {
         epi_u32x4_t rpre[Epi::NH][Epi::NPASS];
         if (epi_res_pre(a)) {
             epi_load_res<NI, 64, 16 * NJ>(a, 0, cbase, pbase, lane, rpre[0]);
@@ -152,6 +147,7 @@ __device__ __forceinline__ void f8_epilogue(const ConvArgs &a, f32x4_t (&acc)[NI
             for (int n = 0; n < Epi::NPASS; ++n) rpre[0][n] = epi_u32x4_t{0u, 0u, 0u, 0u};
         }
         epi_run<bf16_t, NI, NJ>(a, acc, tbase, cbase, pbase, lane, rpre);
+      }
     } else {
         f8_epilogue_rows<OT, NI, NJ>(a, acc, tbase, cbase, pbase, lane);
     }

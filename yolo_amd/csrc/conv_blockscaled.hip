@@ -15,8 +15,8 @@
 // which 13 bits below its leading one survive, and the groups in fp32 (measured with single products;
 // 5e-5 of the result's magnitude on random operands).  That is a thirtieth of bf16's half step, so
 // bf16 outputs take it.  32-bit outputs (the logits) would show it: they run the same tiles through the
-// bf16 instructions, whose products and sums are exact to fp32 (e4m3 numbers are bf16 numbers), at half
-// the rate, the block's sum being scaled by v_ldexp on its way into the accumulator.
+// bf16 instructions at half the rate, whose products are exact and whose sums are fp32: a scaled e4m3
+// number is a bf16 number, one conversion instruction per pair.
 //
 // Quantised map (ymx_quantize_blocks):  [pixel][C] e4m3 bytes (padded to 256), then one plane of
 // exponent bytes (k + 127) per block of channels, [block][pixels rounded up to 4], the padding zero.
@@ -164,18 +164,25 @@ int launch_pack_f8(const float *w_hwio, void *packed, int k, int Cin, int Cout, 
 }
 
 // ---- the product ----------------------------------------------------------------------------------
-// NWQ x NWP waves, each 16 NI channels x 64 pixels; K tiles of 128 channels of one tap through NSTAGE stages
+// NWQ x NWP waves, each 16 NI channels x 16 NJ pixels; K tiles of 128 channels of one tap through NSTAGE stages
 // of LDS, filled by LDS-DMA NSTAGE - 1 tiles ahead, one barrier per tile.  Rows are 128 bytes (one pixel's or one
 // channel's 128 values), the 16-byte chunk c of row r in slot c ^ (r & 7): the lanes that read one fragment then
 // touch 16 different slots.  A lane's 32 values of a fragment are the chunks q and q + 4 of its row, q = lane / 16,
 // for pixels and channels alike (the order inside a block does not matter: one exponent covers it).
-template <typename OT, int NWQ, int NWP, int NI, int NSTAGE>
+template <typename OT, int NWQ, int NWP, int NI, int NJ, int NSTAGE> struct F8Tile {
+    static constexpr int NW = NWQ * NWP, TQ = NWQ * NI * 16, TP = NWP * NJ * 16;
+    static constexpr int NXI = TP / 8 / NW, NWI = TQ / 8 / NW;                       // DMA instructions per wave: rows ...
+    static constexpr int SX = (TP + 63) / 64, NS = SX + (TQ + 63) / 64;              // ... and, in all, exponents
+    static constexpr int XB = TP * 128, WB = TQ * 128, STAGE = XB + WB + NS * 256, PIECES = NXI + NWI + 1;
+    static constexpr int EPI = NW * EpiGeom<NI, 64, 16 * NJ>::LDS_BYTES, LDS = NSTAGE * STAGE > EPI ? NSTAGE * STAGE : EPI;
+    static_assert(TP % (8 * NW) == 0 && TQ % (8 * NW) == 0 && NS <= NW, "whole instructions per wave, one of exponents");
+};
+template <typename OT, int NWQ, int NWP, int NI, int NJ, int NSTAGE>
 __global__ void __launch_bounds__(64 * NWQ * NWP, 2)
 conv_f8_kernel(const F8Args g, const int ntile_q) {
-    constexpr int NW = NWQ * NWP, TQ = NWQ * NI * 16, TP = NWP * 64, NJ = 4;
-    constexpr int NXI = TP / 8 / NW, NWI = TQ / 8 / NW, NS = (TP + TQ) / 64;         // DMA instructions: rows per wave; exponents in all
-    static_assert(TP % (8 * NW) == 0 && TQ % (8 * NW) == 0 && NS <= NW, "whole instructions per wave, one of exponents");
-    constexpr int XB = TP * 128, WB = TQ * 128, STAGE = XB + WB + NS * 256, PIECES = NXI + NWI + 1;
+    typedef F8Tile<OT, NWQ, NWP, NI, NJ, NSTAGE> C;
+    constexpr int NXI = C::NXI, NWI = C::NWI, SX = C::SX, XB = C::XB, WB = C::WB, STAGE = C::STAGE;
+    constexpr bool EXACT = sizeof(OT) == 4;
     constexpr unsigned OOB = 0x80000000u;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const ConvArgs &a = g.a;
@@ -184,50 +191,58 @@ conv_f8_kernel(const F8Args g, const int ntile_q) {
     const int wq = wave % NWQ, wp = wave / NWQ;
     const int id = xcd_remap(blockIdx.x, gridDim.x);
     const int tq = id % ntile_q, tp = id / ntile_q;
-    const int p0 = tp * TP, q0 = tq * TQ;
+    const int p0 = tp * C::TP, q0 = tq * C::TQ;
     const i32x4_t xr = make_rsrc(a.x, a.x_bytes), wr = make_rsrc(a.w, a.w_bytes);
     const i32x4_t xsr = make_rsrc(g.xs, g.xs_bytes), wsr = make_rsrc(g.ws, g.ws_bytes);
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char *)smem;
 
     const int srow = lane >> 3, chunk = (lane & 7) ^ srow;
-    int xpix[NXI];
-    unsigned xmask[NXI];
+    unsigned xoff[NXI], xmask[NXI];
 #pragma unroll
-    for (int i = 0; i < NXI; ++i) pixel_geometry(a, p0 + (wave * NXI + i) * 8 + srow, xpix[i], xmask[i]);
-    const unsigned woff = (unsigned)(q0 + wave * NWI * 8 + srow) * (unsigned)(g.nkt * 128) + (unsigned)chunk * 16u;
-    const unsigned wstep = 8u * (unsigned)(g.nkt * 128);
-    // exponents: instructions 0 .. TP/64 - 1 fetch those of 64 pixels, the others those of 64 channels; waves past
-    // the last instruction repeat it
-    const int si = min(wave, NS - 1);
+    for (int i = 0; i < NXI; ++i) {
+        int pix;
+        pixel_geometry(a, p0 + (wave * NXI + i) * 8 + srow, pix, xmask[i]);
+        xoff[i] = (unsigned)pix * (unsigned)a.Cin + (unsigned)(chunk * 16);
+    }
+    const unsigned row_bytes = (unsigned)(g.nkt * 128);
+    const unsigned woff = (unsigned)(q0 + wave * NWI * 8 + srow) * row_bytes + (unsigned)chunk * 16u;
+    // exponents: instructions 0 .. SX - 1 fetch those of 64 pixels, the others those of 64 channels; waves past the last
+    // instruction repeat it
+    const int si = min(wave, C::NS - 1);
+    const bool s_x = si < SX;
     int spix = 0;
     unsigned smask = 0;
-    if (si < TP / 64) pixel_geometry(a, p0 + si * 64 + lane, spix, smask);
+    if (s_x) {
+        pixel_geometry(a, p0 + si * 64 + lane, spix, smask);
+        if (si * 64 + lane >= C::TP) smask = 0u;
+    }
+    i32x4_t er;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) er[i] = s_x ? xsr[i] : wsr[i];
+    const int ech = (si - SX) * 64 + lane;                      // channel of the tile
+    const unsigned ebase = s_x ? (unsigned)spix : ech < C::TQ ? (unsigned)(q0 + ech) : OOB;
 
-    auto dma = [&](int kt, int stage) {
+    // the K tile issued next: its block, its tap's row and column
+    int kn = 0, blk = 0, tr = 0, tc = 0;
+    auto dma = [&](int stage) {
         const unsigned sb = lds0 + (unsigned)(stage * STAGE);
-        const int blk = fastdiv(kt, g.taps_m, g.taps_s), tap = kt - blk * g.taps;
-        const int tr = fastdiv(tap, a.k_m, a.k_s), tc = tap - tr * a.k;
         const int tpix = tr * a.W + tc;
-        const bool on = kt < g.nkt;
-        const unsigned bit = on ? 1u << tap : 0u;
-        const int c = blk * 128 + chunk * 16;
-        const unsigned cbit = c < a.Cin ? bit : 0u;
+        const bool on = kn < g.nkt;
+        const unsigned bit = on ? 1u << (tr * a.k + tc) : 0u;
+        const unsigned step = (unsigned)tpix * (unsigned)a.Cin + (unsigned)(blk * 128);
+        const unsigned cbit = blk * 128 + chunk * 16 < a.Cin ? bit : 0u;
 #pragma unroll
-        for (int i = 0; i < NXI; ++i)
-            lds_dma16(xr, sb + (unsigned)((wave * NXI + i) * 1024), (xmask[i] & cbit) ? (unsigned)(xpix[i] + tpix) * (unsigned)a.Cin + (unsigned)c : OOB);
+        for (int i = 0; i < NXI; ++i) f8_dma16(xr, sb + (unsigned)((wave * NXI + i) * 1024), (xmask[i] & cbit) ? xoff[i] + step : OOB);
+        const unsigned wk = on ? woff + (unsigned)kn * 128u : OOB;
 #pragma unroll
-        for (int i = 0; i < NWI; ++i)
-            lds_dma16(wr, sb + (unsigned)(XB + (wave * NWI + i) * 1024), on ? woff + (unsigned)i * wstep + (unsigned)kt * 128u : OOB);
-        unsigned so;
-        i32x4_t sr;
-        if (si < TP / 64) {
-            so = (smask & bit) ? (unsigned)blk * g.plane + (unsigned)(spix + tpix) : OOB;
-            sr = xsr;
-        } else {
-            so = on ? (unsigned)kt * (unsigned)g.rows + (unsigned)(q0 + (si - TP / 64) * 64 + lane) : OOB;
-            sr = wsr;
-        }
-        lds_dma_u8(sr, sb + (unsigned)(XB + WB + si * 256), so);
+        for (int i = 0; i < NWI; ++i) f8_dma16(wr, sb + (unsigned)(XB + (wave * NWI + i) * 1024), wk + (unsigned)i * 8u * row_bytes);
+        const unsigned es = s_x ? (unsigned)blk * g.plane + (unsigned)tpix : (unsigned)(kn * g.rows);
+        const bool eon = s_x ? (smask & bit) != 0u : on && ebase != OOB;
+        f8_dma_u8(er, sb + (unsigned)(XB + WB + si * 256), eon ? ebase + es : OOB);
+        ++kn;
+        tc = tc + 1 == a.k ? 0 : tc + 1;
+        tr = tc != 0 ? tr : tr + 1 == a.k ? 0 : tr + 1;
+        blk += tc == 0 && tr == 0 ? 1 : 0;
     };
 
     f32x4_t acc[NI][NJ];
@@ -238,93 +253,94 @@ conv_f8_kernel(const F8Args g, const int ntile_q) {
 
     const int frow = lane & 15, q = lane >> 4;
     const int s0 = (q ^ (frow & 7)) << 4, s1 = ((q + 4) ^ (frow & 7)) << 4;
-    const int a_off = XB + (wq * NI * 16 + frow) * 128, b_off = (wp * 64 + frow) * 128;
-    const int as_off = XB + WB + (TP + wq * NI * 16 + frow) * 4, bs_off = XB + WB + (wp * 64 + frow) * 4;
+    const int a_off = XB + (wq * NI * 16 + frow) * 128, b_off = (wp * NJ * 16 + frow) * 128;
+    const int as_off = XB + WB + (SX * 64 + wq * NI * 16 + frow) * 4, bs_off = XB + WB + (wp * NJ * 16 + frow) * 4;
 
     auto frag = [&](const char *p) { return f8_frag(*(const int4 *)(p + s0), *(const int4 *)(p + s1)); };
-    // 32-bit outputs: the same fragments as bf16 (exact), the block's sum scaled and added by the vector unit
-    auto compute_exact = [&](int stage) {
-        const char *base = smem + stage * STAGE;
-        bf16x8_t b[NJ][4];
-        int bs[NJ];
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            f8_to_bf16(frag(base + b_off + j * 2048), b[j]);
-            bs[j] = *(const int *)(base + bs_off + j * 64) - 254;
-        }
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            bf16x8_t w[4];
-            f8_to_bf16(frag(base + a_off + i * 2048), w);
-            const int4 ws = *(const int4 *)(base + XB + WB + (TP + (wq * NI + i) * 16 + q * 4) * 4);     // of the lane's four results
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int h = 0; h < 4; ++h) sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[h], b[j][h], sum, 0, 0, 0);
-                acc[i][j][0] += __builtin_ldexpf(sum[0], ws.x + bs[j]);
-                acc[i][j][1] += __builtin_ldexpf(sum[1], ws.y + bs[j]);
-                acc[i][j][2] += __builtin_ldexpf(sum[2], ws.z + bs[j]);
-                acc[i][j][3] += __builtin_ldexpf(sum[3], ws.w + bs[j]);
-            }
-        }
+    // Fragments of a tile: all pixels', and the channels' where there are few of them (PRE), before the next DMA is issued,
+    // which then runs under the reads' latency.
+    constexpr int PRE = NI <= 2 ? NI : 1;
+    i32x8_t b[NJ], w[PRE];
+    int bs[NJ], ws[PRE];
+    auto load_w = [&](const char *base, int i, i32x8_t &f, int &e) {
+        f = frag(base + a_off + i * 2048);
+        e = *(const int *)(base + as_off + i * 64);
     };
-    auto compute = [&](int stage) {
-        if constexpr (sizeof(OT) == 4) return compute_exact(stage);
-        const char *base = smem + stage * STAGE;
-        i32x8_t b[NJ];
-        int bs[NJ];
+    auto load = [&](const char *base) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             b[j] = frag(base + b_off + j * 2048);
             bs[j] = *(const int *)(base + bs_off + j * 64);
         }
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            const i32x8_t w = frag(base + a_off + i * 2048);
-            const int ws = *(const int *)(base + as_off + i * 64);
+        for (int i = 0; i < PRE; ++i) load_w(base, i, w[i], ws[i]);
+    };
+    auto compute = [&](const char *base) {
+        bf16x8_t bb[EXACT ? NJ : 1][4];                          // 32-bit outputs: the same fragments, scaled, as bf16
+        if constexpr (EXACT)
 #pragma unroll
-            for (int j = 0; j < NJ; ++j)
-                acc[i][j] = f8_mfma(w, b[j], acc[i][j], ws, bs[j]);
+            for (int j = 0; j < NJ; ++j) f8_to_bf16(b[j], bs[j], bb[j]);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            i32x8_t wf;
+            int we;
+            if (i < PRE) {
+                wf = w[i < PRE ? i : 0];
+                we = ws[i < PRE ? i : 0];
+            } else {
+                load_w(base, i, wf, we);
+            }
+            if constexpr (EXACT) {
+                bf16x8_t wb[4];
+                f8_to_bf16(wf, we, wb);
+#pragma unroll
+                for (int h = 0; h < 4; ++h)
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[h], bb[j][h], acc[i][j], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) acc[i][j] = f8_mfma(wf, b[j], acc[i][j], we, bs[j]);
+            }
         }
     };
 
+    f8_dma_ready();
 #pragma unroll
-    for (int i = 0; i < NSTAGE - 1; ++i) dma(i, i);
-    f8_vmcnt<PIECES * (NSTAGE - 2)>();
+    for (int i = 0; i < NSTAGE - 1; ++i) dma(i);
+    f8_vmcnt<C::PIECES * (NSTAGE - 2)>();
     __syncthreads();
     int st = 0;
     for (int kt = 0; kt < g.nkt; ++kt) {
-        dma(kt + NSTAGE - 1, st == 0 ? NSTAGE - 1 : st - 1);
-        compute(st);
-        f8_vmcnt<PIECES * (NSTAGE - 2)>();
+        const char *base = smem + st * STAGE;
+        load(base);
+        dma(st == 0 ? NSTAGE - 1 : st - 1);
+        compute(base);
+        f8_vmcnt<C::PIECES * (NSTAGE - 2)>();
         __syncthreads();
         st = st + 1 == NSTAGE ? 0 : st + 1;
     }
     f8_vmcnt<0>();
     __syncthreads();
-    f8_epilogue<OT, NI, NJ>(a, acc, smem, wave, q0 + wq * NI * 16, p0 + wp * 64, lane);
+    f8_epilogue<OT, NI, NJ>(a, acc, smem, wave, q0 + wq * NI * 16, p0 + wp * NJ * 16, lane);
 }
 
-template <typename OT, int NWQ, int NWP, int NI, int NSTAGE> static int launch_f8_cfg(const F8Args &g, hipStream_t s) {
-    constexpr int TQ = NWQ * NI * 16, TP = NWP * 64, NW = NWQ * NWP;
-    constexpr int PIPE = NSTAGE * ((TP + TQ) * 128 + (TP + TQ) / 64 * 256), EPI = NW * EpiGeom<NI, 64, 64>::LDS_BYTES;
-    constexpr int LDS = PIPE > EPI ? PIPE : EPI;
-    auto kern = conv_f8_kernel<OT, NWQ, NWP, NI, NSTAGE>;
+template <typename OT, int NWQ, int NWP, int NI, int NJ, int NSTAGE> static int launch_f8_cfg(const F8Args &g, hipStream_t s) {
+    typedef F8Tile<OT, NWQ, NWP, NI, NJ, NSTAGE> C;
+    auto kern = conv_f8_kernel<OT, NWQ, NWP, NI, NJ, NSTAGE>;
     static LdsReserve reserved;
-    if (const int rc = reserve_lds(reserved, (const void *)kern, LDS, "conv_f8")) return rc;
-    const int ntq = (g.a.Cout + TQ - 1) / TQ;
-    const long long grid = (long long)((g.a.P + TP - 1) / TP) * ntq;
+    if (const int rc = reserve_lds(reserved, (const void *)kern, C::LDS, "conv_f8")) return rc;
+    const int ntq = (g.a.Cout + C::TQ - 1) / C::TQ;
+    const long long grid = (long long)((g.a.P + C::TP - 1) / C::TP) * ntq;
     if (grid > 0x7fffffffLL) return fail(YMX_EUNSUPPORTED, "conv_f8: grid too large");
-    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * NW), LDS, s, g, ntq);
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * C::NW), C::LDS, s, g, ntq);
     return check_launch("conv_f8");
 }
 
 template <typename OT> static int launch_f8_shape(const F8Args &g, hipStream_t s) {
     if (conv_f8_wide(g)) return launch_conv_f8_wide(g, s);
     const long long mid = (long long)((g.a.P + 127) / 128) * ((g.a.Cout + 127) / 128);
-    if (mid >= 160) return launch_f8_cfg<OT, 2, 2, 4, 2>(g, s);
-    return launch_f8_cfg<OT, 4, 1, 1, 4>(g, s);
+    if (mid >= 160) return launch_f8_cfg<OT, 2, 2, 4, 4, 2>(g, s);
+    return launch_f8_cfg<OT, 4, 1, 1, 4, 4>(g, s);
 }
 
 // a: geometry of the convolution with x_ld = Cin; x = quantised map, w = packed kernel.

@@ -109,7 +109,7 @@ __device__ __forceinline__ void f8_slab_tile(const F8Args &g, const int p0, cons
         const unsigned dst = ring0 + (unsigned)(((kt & 1) * 2 + half) * F8_PIECE + wave * 2048);
         const unsigned base = (unsigned)kt * 128u + (half ? whalf : 0u);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) lds_dma16(wr, dst + (unsigned)(i * 1024), kt < nk ? base + woff[i] : F8_OOB);
+        for (int i = 0; i < 2; ++i) f8_dma16(wr, dst + (unsigned)(i * 1024), kt < nk ? base + woff[i] : F8_OOB);
     };
     // loop form: offsets of W(m1) of tile kt + 1 and of W(m0) of tile kt + 2; tiles past the end fetch what lies
     // behind the row into slots that nothing reads any more
@@ -121,7 +121,7 @@ __device__ __forceinline__ void f8_slab_tile(const F8Args &g, const int p0, cons
         const bool real = idx < npieces && cb < ncb;
         const unsigned dst = real ? lds0 + (unsigned)((cb & 1) * slab_bytes + idx * 1024) : zero0;
         const unsigned src = slab_off0 + ((unsigned)idx * slab_step + (unsigned)cb * 128u);
-        lds_dma16(xr, dst, cb * 128 + chunk * 16 < (real ? a.Cin : 0) ? src : F8_OOB);
+        f8_dma16(xr, dst, cb * 128 + chunk * 16 < (real ? a.Cin : 0) ? src : F8_OOB);
     };
     // exponents: wave 0 those of the 256 channels of a K tile (esrc: of tile kt + 2), waves 1 and 2 those of a block's slab
     // pixels, from the first one's number rounded down to 4 (esrc: of block cb + 1), the others nothing
@@ -134,13 +134,14 @@ __device__ __forceinline__ void f8_slab_tile(const F8Args &g, const int p0, cons
     auto issue_exp = [&](int kt, int cb, bool pixels) {
         const bool take = e_x && pixels && cb < ncb;
         const unsigned xdst = xexp0 + (unsigned)((cb & 1) * 512 + (wave - 1) * 256), wdst = wexp0 + (unsigned)((kt & 3) * 256);
-        lds_dma4(er, e_w ? wdst : take ? xdst : zero0, e_w || take ? esrc : F8_OOB);
+        f8_dma4(er, e_w ? wdst : take ? xdst : zero0, e_w || take ? esrc : F8_OOB);
         esrc += e_w ? (unsigned)g.rows : take ? g.plane : 0u;
     };
 
+    f8_dma_ready();
 #pragma unroll
     for (int jj = 0; jj < 6; ++jj) issue_slab(0, jj * 8 + wave);
-    lds_dma16(xr, zero0, F8_OOB);                           // the zero KB starts out (and stays) zero
+    f8_dma16(xr, zero0, F8_OOB);                           // the zero KB starts out (and stays) zero
     issue_w(0, 0);
     issue_w(0, 1);
     issue_w(1, 0);
@@ -200,9 +201,9 @@ __device__ __forceinline__ void f8_slab_tile(const F8Args &g, const int p0, cons
             const unsigned d1 = ring0 + (unsigned)((((kt + 1) & 1) * 2 + 1) * F8_PIECE + wave * 2048);
             const unsigned d0 = ring0 + (unsigned)(((kt & 1) * 2) * F8_PIECE + wave * 2048);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) lds_dma16_steady(wr, d1 + (unsigned)(i * 1024), wcur[1][i]);
+            for (int i = 0; i < 2; ++i) f8_dma16(wr, d1 + (unsigned)(i * 1024), wcur[1][i]);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) lds_dma16_steady(wr, d0 + (unsigned)(i * 1024), wcur[0][i]);
+            for (int i = 0; i < 2; ++i) f8_dma16(wr, d0 + (unsigned)(i * 1024), wcur[0][i]);
             issue_slab(tap < 6 ? cb + 1 : ncb, tap * 8 + wave);
             issue_exp(kt + 2, cb + 1, tap == 0);
         }
@@ -279,22 +280,22 @@ __device__ __forceinline__ void f8_stag_tile(const F8Args &g, const int p0, cons
         const unsigned step = (unsigned)tpix * (unsigned)a.Cin + (unsigned)blk * 128u;
         const unsigned ok = blk * 128 + chunk * 16 < a.Cin ? bit : 0u;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) lds_dma16(xr, dst + (unsigned)(i * 1024), (xmask[half][i] & ok) ? xoff[half][i] + step : F8_OOB);
+        for (int i = 0; i < 2; ++i) f8_dma16(xr, dst + (unsigned)(i * 1024), (xmask[half][i] & ok) ? xoff[half][i] + step : F8_OOB);
     };
     auto issue_w = [&](int kt, int half) {
         const unsigned dst = lds0 + (unsigned)(((kt & 1) * 4 + (half ? 3 : 0)) * F8_PIECE + wave * 2048);
         const unsigned base = (unsigned)kt * 128u + (half ? whalf : 0u);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) lds_dma16(wr, dst + (unsigned)(i * 1024), kt < nk ? base + woff[i] : F8_OOB);
+        for (int i = 0; i < 2; ++i) f8_dma16(wr, dst + (unsigned)(i * 1024), kt < nk ? base + woff[i] : F8_OOB);
     };
     const bool e_w = wave == 4, e_x = wave < NJ;
     auto issue_exp = [&](int kt, int tpix, unsigned bit, int blk) {
         const unsigned slot = exp0 + (unsigned)((kt & 3) * F8_STAG_EXP);
         if (e_w) {
-            lds_dma4(wsr, slot, kt < nk ? (unsigned)(kt * g.rows + q0) + (unsigned)(lane * 4) : F8_OOB);
+            f8_dma4(wsr, slot, kt < nk ? (unsigned)(kt * g.rows + q0) + (unsigned)(lane * 4) : F8_OOB);
         } else {
             const unsigned src = (unsigned)spix + ((unsigned)blk * g.plane + (unsigned)tpix);
-            lds_dma_u8(xsr, e_x ? slot + 256u + (unsigned)(wave * 256) : dump, (smask & (e_x ? bit : 0u)) ? src : F8_OOB);
+            f8_dma_u8(xsr, e_x ? slot + 256u + (unsigned)(wave * 256) : dump, (smask & (e_x ? bit : 0u)) ? src : F8_OOB);
         }
     };
     auto first_half = [&](int kt) {                          // W(m0), X(n0), exponents
@@ -312,6 +313,7 @@ __device__ __forceinline__ void f8_stag_tile(const F8Args &g, const int p0, cons
         issue_x(kt, 1, tpix, bit, blk);
         issue_w(kt, 1);
     };
+    f8_dma_ready();
     first_half(0);
     second_half(0);
     first_half(1);
