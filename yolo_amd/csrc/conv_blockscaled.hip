@@ -173,15 +173,16 @@ template <typename OT, int NWQ, int NWP, int NI, int NJ, int NSTAGE> struct F8Ti
     static constexpr int NW = NWQ * NWP, TQ = NWQ * NI * 16, TP = NWP * NJ * 16;
     static constexpr int NXI = TP / 8 / NW, NWI = TQ / 8 / NW;                       // DMA instructions per wave: rows ...
     static constexpr int SX = (TP + 63) / 64, NS = SX + (TQ + 63) / 64;              // ... and, in all, exponents
-    static constexpr int XB = TP * 128, WB = TQ * 128, STAGE = XB + WB + NS * 256, PIECES = NXI + NWI + 1;
+    static constexpr int NSI = (NS + NW - 1) / NW;                                   // (per wave)
+    static constexpr int XB = TP * 128, WB = TQ * 128, STAGE = XB + WB + NS * 256, PIECES = NXI + NWI + NSI;
     static constexpr int EPI = NW * EpiGeom<NI, 64, 16 * NJ>::LDS_BYTES, LDS = NSTAGE * STAGE > EPI ? NSTAGE * STAGE : EPI;
-    static_assert(TP % (8 * NW) == 0 && TQ % (8 * NW) == 0 && NS <= NW, "whole instructions per wave, one of exponents");
+    static_assert(TP % (8 * NW) == 0 && TQ % (8 * NW) == 0, "whole instructions per wave");
 };
 template <typename OT, int NWQ, int NWP, int NI, int NJ, int NSTAGE>
 __global__ void __launch_bounds__(64 * NWQ * NWP, 2)
 conv_f8_kernel(const F8Args g, const int ntile_q) {
     typedef F8Tile<OT, NWQ, NWP, NI, NJ, NSTAGE> C;
-    constexpr int NXI = C::NXI, NWI = C::NWI, SX = C::SX, XB = C::XB, WB = C::WB, STAGE = C::STAGE;
+    constexpr int NXI = C::NXI, NWI = C::NWI, NSI = C::NSI, SX = C::SX, XB = C::XB, WB = C::WB, STAGE = C::STAGE;
     constexpr bool EXACT = sizeof(OT) == 4;
     constexpr unsigned OOB = 0x80000000u;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -206,21 +207,26 @@ conv_f8_kernel(const F8Args g, const int ntile_q) {
     }
     const unsigned row_bytes = (unsigned)(g.nkt * 128);
     const unsigned woff = (unsigned)(q0 + wave * NWI * 8 + srow) * row_bytes + (unsigned)chunk * 16u;
-    // exponents: instructions 0 .. SX - 1 fetch those of 64 pixels, the others those of 64 channels; waves past the last
-    // instruction repeat it
-    const int si = min(wave, C::NS - 1);
-    const bool s_x = si < SX;
-    int spix = 0;
-    unsigned smask = 0;
-    if (s_x) {
-        pixel_geometry(a, p0 + si * 64 + lane, spix, smask);
-        if (si * 64 + lane >= C::TP) smask = 0u;
-    }
-    i32x4_t er;
+    // exponents: instructions 0 .. SX - 1 fetch those of 64 pixels, the others those of 64 channels; instructions past the
+    // last repeat it
+    int si[NSI];
+    unsigned smask[NSI], ebase[NSI];
+    i32x4_t er[NSI];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) er[i] = s_x ? xsr[i] : wsr[i];
-    const int ech = (si - SX) * 64 + lane;                      // channel of the tile
-    const unsigned ebase = s_x ? (unsigned)spix : ech < C::TQ ? (unsigned)(q0 + ech) : OOB;
+    for (int e = 0; e < NSI; ++e) {
+        si[e] = min(wave + e * C::NW, C::NS - 1);
+        const bool s_x = si[e] < SX;
+        int pix = 0;
+        smask[e] = 0;
+        if (s_x) {
+            pixel_geometry(a, p0 + si[e] * 64 + lane, pix, smask[e]);
+            if (si[e] * 64 + lane >= C::TP) smask[e] = 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) er[e][i] = s_x ? xsr[i] : wsr[i];
+        const int ch = (si[e] - SX) * 64 + lane;                 // channel of the tile
+        ebase[e] = s_x ? (unsigned)pix : ch < C::TQ ? (unsigned)(q0 + ch) : OOB;
+    }
 
     // the K tile issued next: its block, its tap's row and column
     int kn = 0, blk = 0, tr = 0, tc = 0;
@@ -236,9 +242,13 @@ conv_f8_kernel(const F8Args g, const int ntile_q) {
         const unsigned wk = on ? woff + (unsigned)kn * 128u : OOB;
 #pragma unroll
         for (int i = 0; i < NWI; ++i) f8_dma16(wr, sb + (unsigned)(XB + (wave * NWI + i) * 1024), wk + (unsigned)i * 8u * row_bytes);
-        const unsigned es = s_x ? (unsigned)blk * g.plane + (unsigned)tpix : (unsigned)(kn * g.rows);
-        const bool eon = s_x ? (smask & bit) != 0u : on && ebase != OOB;
-        f8_dma_u8(er, sb + (unsigned)(XB + WB + si * 256), eon ? ebase + es : OOB);
+#pragma unroll
+        for (int e = 0; e < NSI; ++e) {
+            const bool s_x = si[e] < SX;
+            const unsigned es = s_x ? (unsigned)blk * g.plane + (unsigned)tpix : (unsigned)(kn * g.rows);
+            const bool eon = s_x ? (smask[e] & bit) != 0u : on && ebase[e] != OOB;
+            f8_dma_u8(er[e], sb + (unsigned)(XB + WB + si[e] * 256), eon ? ebase[e] + es : OOB);
+        }
         ++kn;
         tc = tc + 1 == a.k ? 0 : tc + 1;
         tr = tc != 0 ? tr : tr + 1 == a.k ? 0 : tr + 1;
@@ -336,10 +346,21 @@ template <typename OT, int NWQ, int NWP, int NI, int NJ, int NSTAGE> static int 
     return check_launch("conv_f8");
 }
 
+// The tile, by how many there are.  Measured (us, batch x map, in -> out channels, window):
+//   256 x 256, staggered (conv_blockscaled_wide.hip): 160 tiles and more (16 x 104^2 128 -> 256 3x3 stride 2: 25.2, 64 x 128 30.3)
+//   64 ch x 128 px, two stages, three workgroups a CU: from 512 tiles.  64 x 104^2 128 -> 64 1x1: 48, in tiles of
+//       128 x 128 75, of 64 x 64 82; up to 32 channels as 32 x 128 (64 x 208^2 64 -> 32 1x1: 142 against 170)
+//   64 x 64, two stages, four workgroups a CU: from 200 (52^2 512 -> 1024 3x3: 30.8, 64 x 128 34.5)
+//   64 x 64, four stages: fewer (26^2 512 -> 1024 3x3: 19.2, two stages 27.3)
+//   64 x 32, four stages: where even that leaves half the CUs idle (13^2 512 -> 1024 3x3: 15.1, 64 x 64 18.0), and for
+//       32-bit outputs, whose conversions weigh more, wherever there are few tiles (8 x 26^2 1024 -> 255 1x1: 12.3, 14.4)
 template <typename OT> static int launch_f8_shape(const F8Args &g, hipStream_t s) {
     if (conv_f8_wide(g)) return launch_conv_f8_wide(g, s);
-    const long long mid = (long long)((g.a.P + 127) / 128) * ((g.a.Cout + 127) / 128);
-    if (mid >= 160) return launch_f8_cfg<OT, 2, 2, 4, 4, 2>(g, s);
+    const long long np = g.a.P, nq = (g.a.Cout + 63) / 64;
+    const long long tiles = (np + 127) / 128 * nq;
+    if (tiles >= 512) return g.a.Cout <= 32 ? launch_f8_cfg<OT, 2, 2, 1, 4, 2>(g, s) : launch_f8_cfg<OT, 2, 2, 2, 4, 2>(g, s);
+    if (tiles >= 200 && sizeof(OT) == 2) return launch_f8_cfg<OT, 4, 1, 1, 4, 2>(g, s);
+    if (sizeof(OT) == 4 || (np + 63) / 64 * nq <= 128) return launch_f8_cfg<OT, 4, 1, 1, 2, 4>(g, s);
     return launch_f8_cfg<OT, 4, 1, 1, 4, 4>(g, s);
 }
 
