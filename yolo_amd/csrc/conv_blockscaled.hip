@@ -348,6 +348,8 @@ template <typename OT, int NWQ, int NWP, int NI, int NJ, int NSTAGE> static int 
 
 // The tile, by how many there are.  Measured (us, batch x map, in -> out channels, window):
 //   256 x 256, staggered (conv_blockscaled_wide.hip): 160 tiles and more (16 x 104^2 128 -> 256 3x3 stride 2: 25.2, 64 x 128 30.3)
+//   128 ch x 128 px, eight waves, two workgroups a CU: from 300 tiles that are no more than a quarter wider than needed, bf16
+//       outputs (64 x 26^2 144 -> 768 3x3 stride 2: 26.5, 64 x 128 38.4)
 //   64 ch x 128 px, two stages, three workgroups a CU: from 512 tiles.  64 x 104^2 128 -> 64 1x1: 48, in tiles of
 //       128 x 128 75, of 64 x 64 82; up to 32 channels as 32 x 128 (64 x 208^2 64 -> 32 1x1: 142 against 170)
 //   64 x 64, two stages, four workgroups a CU: from 200 (52^2 512 -> 1024 3x3: 30.8, 64 x 128 34.5)
@@ -356,8 +358,10 @@ template <typename OT, int NWQ, int NWP, int NI, int NJ, int NSTAGE> static int 
 //       32-bit outputs, whose conversions weigh more, wherever there are few tiles (8 x 26^2 1024 -> 255 1x1: 12.3, 14.4)
 template <typename OT> static int launch_f8_shape(const F8Args &g, hipStream_t s) {
     if (conv_f8_wide(g)) return launch_conv_f8_wide(g, s);
-    const long long np = g.a.P, nq = (g.a.Cout + 63) / 64;
+    const long long np = g.a.P, nq = (g.a.Cout + 63) / 64, n128 = (g.a.Cout + 127) / 128;
     const long long tiles = (np + 127) / 128 * nq;
+    if constexpr (sizeof(OT) == 2)
+        if (n128 * 8 <= nq * 5 && (np + 127) / 128 * n128 >= 300) return launch_f8_cfg<OT, 4, 2, 2, 4, 2>(g, s);
     if (tiles >= 512) return g.a.Cout <= 32 ? launch_f8_cfg<OT, 2, 2, 1, 4, 2>(g, s) : launch_f8_cfg<OT, 2, 2, 2, 4, 2>(g, s);
     if (tiles >= 200 && sizeof(OT) == 2) return launch_f8_cfg<OT, 4, 1, 1, 4, 2>(g, s);
     if (sizeof(OT) == 4 || (np + 63) / 64 * nq <= 128) return launch_f8_cfg<OT, 4, 1, 1, 2, 4>(g, s);

@@ -382,11 +382,14 @@ static int slab_lds(int pieces) { return 2 * pieces * 1024 + 4 * F8_PIECE + 1024
 // Slabs of 192-pixel tiles fit for rows up to 91 pixels, of 256-pixel tiles up to 59.
 static bool slab_fits(const F8Args &g) { return g.taps == 9 && g.a.stride == 1 && slab_lds(slab_pieces(g.a.W, 192)) <= 160 * 1024; }
 
-// Layers for these kernels: bf16 outputs, 160 tiles and more, and 256-channel tiles no more than a quarter wider than
-// 64-channel ones would be (64 x 26^2 512 -> 300 3x3: 124 us here, 107 in tiles of 64 channels; 768 channels: the same).
+// Layers for these kernels: bf16 outputs, 160 tiles and more, 256-channel tiles no more than a quarter wider than
+// 64-channel ones would be (64 x 26^2 512 -> 300 3x3: 124 us here, 90 in tiles of 128), more than two K tiles (16 x 52^2
+// 144 -> 200 1x1: 21.4, 18.8), and, where both operands are fetched per K tile, not between one round of the chip and two
+// (64 x 26^2 1024 -> 512 1x1, 338 tiles: 47.6, 44.1; 64 x 52^2, 1352 tiles: 156, 194).
 bool conv_f8_wide(const F8Args &g) {
     const long long nq = (g.a.Cout + 255) / 256, n64 = (g.a.Cout + 63) / 64;
-    return g.a.out_dtype == YMX_BF16 && nq * 16 <= n64 * 5 && (long long)((g.a.P + 255) / 256) * nq >= 160;
+    const long long tiles = (long long)((g.a.P + 255) / 256) * nq;
+    return g.a.out_dtype == YMX_BF16 && nq * 16 <= n64 * 5 && tiles >= 160 && g.nkt > 2 && (slab_fits(g) || tiles <= 256 || tiles >= 512);
 }
 
 template <bool SLAB> static int launch_wide(const F8Args &g, hipStream_t s) {
