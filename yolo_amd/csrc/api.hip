@@ -932,7 +932,7 @@ size_t ymx_group_norm_workspace_bytes(long long B, long long n_pix, int C, int G
 int ymx_group_norm_forward(const void *x, const float *gamma, const float *beta, const void *residual, void *y, float *stats,
                            long long B, long long n_pix, int C, int G, int act, float eps, int dtype, double rate,
                            const void *state, void *workspace, size_t ws_bytes, void *stream) {
-    if (!x || !gamma || !beta || !y || !stats || !workspace) return fail(YMX_EARG, "group_norm_forward: null pointer");
+    if (!x || !gamma || !beta || !y || !workspace) return fail(YMX_EARG, "group_norm_forward: null pointer");
     if (!(eps > 0.0f)) return fail(YMX_EARG, "group_norm_forward: epsilon %g", (double)eps);
     GnArgs a = {};
     if (const int rc = gn_args("group_norm_forward", a, B, n_pix, C, G, act, dtype, rate, state, workspace, ws_bytes)) return rc;

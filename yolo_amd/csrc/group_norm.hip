@@ -224,7 +224,7 @@ __device__ __forceinline__ void gn_join(const GnArgs &a, const GnWork &w, int b,
             } else {
                 const float shift = s.x * inv_n;
                 out[g] = float2{piv + shift, 1.0f / sqrtf(fmaxf(s.y * inv_n - shift * shift, 0.0f) + a.eps)};
-                if (keep) ((float2 *)a.stats)[(size_t)b * a.G + g] = out[g];
+                if (keep && a.stats) ((float2 *)a.stats)[(size_t)b * a.G + g] = out[g];
             }
         }
     }
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const GnArgs a, const 
 #pragma unroll
         for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.0f;
         struct Row { typename IO::raw x, d; };
-        gn_rows<2>(g.p, g.p1, w.R, [&](int p) { return Row{IO::load(x + (size_t)p * a.C), IO::load(dy + (size_t)p * a.C)}; },
+        gn_rows<4>(g.p, g.p1, w.R, [&](int p) { return Row{IO::load(x + (size_t)p * a.C), IO::load(dy + (size_t)p * a.C)}; },
                    [&](int p, const Row &q) {
                        float v[V], d[V], dt[V];
                        IO::unpack(q.x, v);
@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(256) gn_bwd_apply_kernel(const GnArgs a, const
     uint4 key = {};
     if constexpr (DROP) key = uint4{a.state[0], a.state[1], a.state[2], a.state[3]};
     struct Row { typename IO::raw x, d; };
-    gn_rows<2>(g.p, g.p1, w.R, [&](int p) { return Row{IO::load(x + (size_t)p * a.C), IO::load(dy + (size_t)p * a.C)}; },
+    gn_rows<4>(g.p, g.p1, w.R, [&](int p) { return Row{IO::load(x + (size_t)p * a.C), IO::load(dy + (size_t)p * a.C)}; },
                [&](int p, const Row &q) {
                    float v[V], d[V], dt[V];
                    IO::unpack(q.x, v);
@@ -536,7 +536,7 @@ __global__ void __launch_bounds__(512) gn_slab_kernel(const GnArgs a, const GnSl
     t = 1.0f / sqrtf(t + a.eps);
     if ((int)threadIdx.x < W) {
         grp[threadIdx.x] = t;
-        if (threadIdx.x % a.D == 0) ((float2 *)a.stats)[(size_t)b * a.G + (slab * W + threadIdx.x) / a.D] = float2{m_keep, t};
+        if (a.stats && threadIdx.x % a.D == 0) ((float2 *)a.stats)[(size_t)b * a.G + (slab * W + threadIdx.x) / a.D] = float2{m_keep, t};
     }
     __syncthreads();
     GnChannels<V> ch;

@@ -52,7 +52,8 @@ template <int V> __device__ __forceinline__ void drop_keep(const DropArgs &d, co
     }
 }
 
-// V consecutive elements of a map as floats: 16-byte accesses for whole vectors, scalar ones for V = 1.
+// V consecutive elements of a map as floats: 16-byte accesses for whole vectors (streaming stores: group norm over 16 x
+// 208^2 x 64 forward 79.5 -> 74.4 us, backward 105.8 -> 100.4), scalar ones for V = 1.
 template <typename T, int V> struct vec_io;
 template <> struct vec_io<bf16_t, 8> {
     typedef uint4 raw;
@@ -71,14 +72,14 @@ template <> struct vec_io<bf16_t, 8> {
         return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, pair_t));
     }
     __device__ static __forceinline__ void store(bf16_t *p, const float (&v)[8]) {
-        *(uint4 *)p = uint4{pack(v[0], v[1]), pack(v[2], v[3]), pack(v[4], v[5]), pack(v[6], v[7])};
+        store_stream16(p, pack(v[0], v[1]), pack(v[2], v[3]), pack(v[4], v[5]), pack(v[6], v[7]));
     }
 };
 template <> struct vec_io<float, 4> {
     typedef float4 raw;
     __device__ static __forceinline__ raw load(const float *p) { return *(const float4 *)p; }
     __device__ static __forceinline__ void unpack(const raw &r, float (&v)[4]) { v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w; }
-    __device__ static __forceinline__ void store(float *p, const float (&v)[4]) { *(float4 *)p = float4{v[0], v[1], v[2], v[3]}; }
+    __device__ static __forceinline__ void store(float *p, const float (&v)[4]) { store_stream16(p, v[0], v[1], v[2], v[3]); }
 };
 template <typename T> struct vec_io<T, 1> {
     typedef T raw;

@@ -529,14 +529,15 @@ def _dense(t, dtype):
 
 # The backward steps below are Python run by autograd's own thread, where every call costs about twice
 # what it does on the caller's: what can be decided in the forward pass is decided there.
-def _group_norm_forward(x, gamma, beta, shortcut, groups, act, epsilon, rate, state):
-    """(y, contiguous x, gamma and beta as the kernels take them, statistics, the geometry of the launches)"""
+def _group_norm_forward(x, gamma, beta, shortcut, state, cfg, keep):
+    """(y, contiguous x, gamma and beta as the kernels take them, statistics if `keep`, the geometry of the launches)"""
+    groups, act, epsilon, rate = cfg
     x = x if x.is_contiguous() else x.contiguous()
     b, c = x.shape[0], x.shape[-1]
     gamma, beta = _dense(gamma, torch.float32), _dense(beta, torch.float32)
     sc = None if shortcut is None else _dense(shortcut, x.dtype)
     y = torch.empty_like(x)
-    stats = torch.empty((b, groups, 2), device=x.device, dtype=torch.float32)
+    stats = torch.empty((b, groups, 2), device=x.device, dtype=torch.float32) if keep else None
     geo = None
     n = x.numel()
     if n:
@@ -544,7 +545,7 @@ def _group_norm_forward(x, gamma, beta, shortcut, groups, act, epsilon, rate, st
         nb = _lib.lib().ymx_group_norm_workspace_bytes(b, pix, c, groups)
         geo = (b, pix, c, groups, act, _lib.dtype_code(x.dtype), rate, nb)
         ws = torch.empty((nb,), device=x.device, dtype=torch.uint8)
-        _lib.launch("ymx_group_norm_forward", x, x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), _lib.ptr(sc), y.data_ptr(), stats.data_ptr(),
+        _lib.launch("ymx_group_norm_forward", x, x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), _lib.ptr(sc), y.data_ptr(), _lib.ptr(stats),
                     b, pix, c, groups, act, epsilon, geo[5], rate, _lib.ptr(state), ws.data_ptr(), nb)
     return y, x, gamma, beta, stats, geo
 
@@ -572,7 +573,7 @@ def _group_norm_backward(ctx, dy):
     dsc = None
     if need_s:
         dsc = dy if dy.dtype == ctx.dtypes[2] else dy.to(ctx.dtypes[2])
-    return dx if need_x else None, dgamma if need_g else None, dbeta if need_b else None, dsc, None, None, None, None, None
+    return dx if need_x else None, dgamma if need_g else None, dbeta if need_b else None, dsc, None, None
 
 
 _group_norm_backward_once = torch.autograd.function.once_differentiable(_group_norm_backward)
@@ -580,8 +581,8 @@ _group_norm_backward_once = torch.autograd.function.once_differentiable(_group_n
 
 class _GroupNormAct(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, gamma, beta, shortcut, groups, act, epsilon, rate, state):
-        y, xc, ga, be, stats, ctx.geo = _group_norm_forward(x, gamma, beta, shortcut, groups, act, epsilon, rate, state)
+    def forward(ctx, x, gamma, beta, shortcut, state, cfg):
+        y, xc, ga, be, stats, ctx.geo = _group_norm_forward(x, gamma, beta, shortcut, state, cfg, True)
         ctx.save_for_backward(xc, ga, be, stats, state)
         ctx.dtypes = (gamma.dtype, beta.dtype, None if shortcut is None else shortcut.dtype)
         return y
@@ -616,9 +617,9 @@ def group_norm_act(x, gamma, beta, groups, activation=None, shortcut=None, epsil
     rate = _check_dropout(x, rate, state, "group_norm_act")
     state = state if rate > 0.0 else None
     if _records(x, gamma, beta, shortcut):
-        return _GroupNormAct.apply(x, gamma, beta, shortcut, groups, code, float(epsilon), rate, state)
+        return _GroupNormAct.apply(x, gamma, beta, shortcut, state, (groups, code, float(epsilon), rate))
     with torch.no_grad():
-        return _group_norm_forward(x, gamma, beta, shortcut, groups, code, float(epsilon), rate, state)[0]
+        return _group_norm_forward(x, gamma, beta, shortcut, state, (groups, code, float(epsilon), rate), False)[0]
 
 
 def _dropout_launch(x, shortcut, rate, state):
