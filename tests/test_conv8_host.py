@@ -63,5 +63,7 @@ def test_layers_check_before_the_device():
     with T.backprop():
         with pytest.raises(ValueError, match="quantised map"):
             c(q)
+    with pytest.raises(ValueError, match="residual"):
+        c(q, residual=q)
     with pytest.raises(ValueError, match="input channels"):
         YOLOConv((3, 3, 32), dtype=F8, in_channels=64)(q)

@@ -220,6 +220,26 @@ def test_conv8_in_a_graph():
         torch.ones(1000, device=DEV).sum().item()
 
 
+def test_conv8_capture_needs_a_packed_kernel():
+    """The packed kernel is kept by the layer: it must not live in a graph's memory."""
+    from yolo_amd.layers import YOLOConv
+    layer = YOLOConv((1, 1, 64), dtype=F8, in_channels=64).to(DEV)
+    x = torch.randn(1, 8, 8, 64, device=DEV).bfloat16()
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="before capturing"):
+        with torch.cuda.graph(g):
+            layer(x)
+    torch.cuda.synchronize()
+    want = layer(x).clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = layer(x)
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+
+
 def test_networks_run_in_8_bits():
     """Darknet53, CSPDarknet53 and YoloV3 with dtype=torch.float8_e4m3fn (the first layers in bf16): every layer's
     result is the layer function's own on the same input, the maps stay close to the bf16 network's.  e4m3 operands

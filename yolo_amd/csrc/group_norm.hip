@@ -16,7 +16,7 @@
 // pair of numbers per (chunk, group) -- mean and centred sum of squares, or S1 and S2 -- and, backward,
 // one per (chunk, channel); every workgroup of pass 2 first joins the pairs of its sample (a few
 // hundred, from L2), then reads the map again and writes.  Slab form: see gn_slab_kernel.  All sums
-// are fp32, added in a fixed order: no result depends on the order workgroups run in.
+// are fp32 or wider, added in a fixed order: no result depends on the order workgroups run in.
 #include <algorithm>
 #include <type_traits>
 
@@ -254,7 +254,7 @@ template <int V> struct GnChannels {
 // Pass 2, forward.
 template <typename T, int V, int ACT, bool DROP>
 __global__ void __launch_bounds__(256) gn_apply_kernel(const GnArgs a, const GnWork w, const float2 *__restrict__ part) {
-    extern __shared__ float2 joined[];                           // [G], then 256 of scratch
+    extern __shared__ __attribute__((aligned(16))) float2 joined[];      // [G], then 256 of scratch
     const GnPos<V> g(a, w);
     gn_join<false, V>(a, w, g.b, g.chunk == 0 && g.cb == 0, part, joined, joined + a.G);
     if (!g.on) return;
@@ -358,12 +358,13 @@ __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const GnArgs a, const 
     }
     __syncthreads();
     for (int c = threadIdx.x; c < g.wc; c += 256) {
-        float2 s = {0.0f, 0.0f};
+        double d1 = 0.0, d2 = 0.0;
         for (int r = 0; r < w.R; ++r) {
             const float2 q = red[r * W + c];
-            s.x += q.x;
-            s.y += q.y;
+            d1 += q.x;
+            d2 += q.y;
         }
+        const float2 s = {(float)d1, (float)d2};
         part[((size_t)g.b * w.nchunk + g.chunk) * a.C + g.cb + c] = s;
         const float ga = a.gamma[g.cb + c];
         red[c] = float2{ga * s.x, ga * s.y};
@@ -374,11 +375,12 @@ __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const GnArgs a, const 
 }
 
 // dbeta and dgamma of 16 channels from `rows` pairs each, by a workgroup of 16 * RL threads: RL row lanes (four chains
-// each) and those by a tree.  red: 16 * (RL + 1) pairs.
+// each) and those by a tree, in 64 bits: the sums run over a whole batch of maps, and there are few of them.
+// red: 16 * (RL + 1) pairs of doubles.
 template <int RL>
-__device__ __forceinline__ void gn_param_grads(const GnArgs &a, int block, int rows, const float2 *__restrict__ part, float2 *__restrict__ red) {
+__device__ __forceinline__ void gn_param_grads(const GnArgs &a, int block, int rows, const float2 *__restrict__ part, double2 *__restrict__ red) {
     const int cl = threadIdx.x & 15, row = threadIdx.x >> 4, c = block * 16 + cl;
-    float2 s[4] = {};
+    double2 s[4] = {};
     if (c < a.C) {
         int i = row;
         for (; i + 3 * RL < rows; i += 4 * RL) {
@@ -394,23 +396,23 @@ __device__ __forceinline__ void gn_param_grads(const GnArgs &a, int block, int r
             s[0].y += v.y;
         }
     }
-    red[cl * (RL + 1) + row] = float2{(s[0].x + s[1].x) + (s[2].x + s[3].x), (s[0].y + s[1].y) + (s[2].y + s[3].y)};
+    red[cl * (RL + 1) + row] = double2{(s[0].x + s[1].x) + (s[2].x + s[3].x), (s[0].y + s[1].y) + (s[2].y + s[3].y)};
     __syncthreads();
     // RL lanes per channel, channels dealt to the groups of RL threads
     const int lane = threadIdx.x % RL, cw = threadIdx.x / RL;
-    float2 t = red[cw * (RL + 1) + lane];
+    double2 t = red[cw * (RL + 1) + lane];
 #pragma unroll
     for (int o = RL / 2; o > 0; o >>= 1) {
         t.x += __shfl_xor(t.x, o);
         t.y += __shfl_xor(t.y, o);
     }
     if (lane == 0 && block * 16 + cw < a.C) {
-        a.dbeta[block * 16 + cw] = t.x;
-        a.dgamma[block * 16 + cw] = t.y;
+        a.dbeta[block * 16 + cw] = (float)t.x;
+        a.dgamma[block * 16 + cw] = (float)t.y;
     }
 }
 __global__ void __launch_bounds__(1024) gn_param_grads_kernel(const GnArgs a, int rows, const float2 *__restrict__ part) {
-    __shared__ float2 red[16 * 65];
+    __shared__ double2 red[16 * 65];
     gn_param_grads<64>(a, blockIdx.x, rows, part, red);
 }
 
@@ -418,9 +420,9 @@ __global__ void __launch_bounds__(1024) gn_param_grads_kernel(const GnArgs a, in
 template <typename T, int V, int ACT, bool DROP>
 __global__ void __launch_bounds__(256) gn_bwd_apply_kernel(const GnArgs a, const GnWork w, const float2 *__restrict__ part,
                                                            const float2 *__restrict__ gpart, int nparam) {
-    extern __shared__ float2 joined[];                           // [G], then 16 * 17 of scratch
+    extern __shared__ __attribute__((aligned(16))) float2 joined[];      // [G], then 256 of scratch; or 16 * 17 pairs of doubles
     if ((int)blockIdx.x < nparam) {                              // the first workgroups: parameter gradients, 16 channels each
-        gn_param_grads<16>(a, blockIdx.x, a.B * w.nchunk, part, joined + a.G);
+        gn_param_grads<16>(a, blockIdx.x, a.B * w.nchunk, part, (double2 *)joined);
         return;
     }
     const GnPos<V> g(a, w, nparam);
@@ -773,7 +775,8 @@ template <typename T> static int gn_backward(const GnArgs &a, void *ws, hipStrea
         float2 *gpart = (float2 *)ws, *part = gpart + (size_t)a.B * w.nchunk * w.nsub * a.G;
         const int nparam = (a.C + 127) / 128 * 8;                // whole eights: a chunk stays on the XCD that pass 1 read it on
         hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT, DROP>), grid, dim3(256), 0, s, a, w, part, gpart);
-        hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, DROP>), dim3(grid.x + nparam), dim3(256), (a.G + 272) * sizeof(float2), s, a, w,
+        hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, DROP>), dim3(grid.x + nparam), dim3(256),
+                           std::max((a.G + 256) * sizeof(float2), 16 * 17 * sizeof(double2)), s, a, w,
                            part, gpart, nparam);
     });
     return check_launch("group_norm_backward");

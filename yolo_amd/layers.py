@@ -367,7 +367,10 @@ class YOLOConv(nn.Module):
         if hit is not None and hit[0] == key:
             return hit[1]
         _lib.require_gpu(self.kernel)
-        code = _lib.F8E4M3 if dtype == torch.float8_e4m3fn else _lib.dtype_code(dtype)
+        f8 = dtype == torch.float8_e4m3fn
+        if f8 and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("YOLOConv: call an 8-bit layer once before capturing it (its kernel is packed then)")
+        code = _lib.F8E4M3 if f8 else _lib.dtype_code(dtype)
         k, cin, cout = self.kernel_size, self.in_channels, self.filters
         nbytes = _lib.lib().ymx_packed_weight_bytes(k, cin, cout, code)
         wp = torch.empty(nbytes, dtype=torch.uint8, device=dev)
@@ -380,6 +383,8 @@ class YOLOConv(nn.Module):
         else:
             scale, shift = None, self.bias.detach().float().contiguous()
         entry = (wp, scale, shift, src)      # src kept alive until the pack kernel has run
+        if f8:                               # later calls may be on any stream
+            torch.cuda.current_stream(dev).synchronize()
         self._packed["entry"] = (key, entry)
         return entry
 
@@ -481,6 +486,8 @@ class YOLOConv(nn.Module):
         activation inside the kernel; out_dtype overrides the output element type; out, if
         given, receives the result: a [B,H',W',Cout] view whose pixels may be spaced wider than
         Cout (a channel slice of a larger NHWC buffer: how a concat is written in place)."""
+        if isinstance(residual, BlockQuantized):
+            raise ValueError("YOLOConv: the residual is a plain tensor, not a quantised map")
         if not isinstance(x, BlockQuantized):
             x = _as_nhwc(x)
         elif len(x.shape) != 4 or self.compute_dtype != torch.float8_e4m3fn or _training.enabled():
