@@ -240,6 +240,40 @@ def test_conv8_capture_needs_a_packed_kernel():
         assert torch.equal(y, want)
 
 
+@pytest.mark.parametrize("norm", [dict(), dict(batchNormalization=True)])
+def test_conv8_graph_follows_a_repacked_kernel(norm):
+    """A changed kernel is packed again where the old one was, so that a graph captured before reads no freed memory
+    and, from the next call of the layer on, the new values."""
+    from yolo_amd.layers import YOLOConv
+    torch.manual_seed(4)
+    layer = YOLOConv((3, 3, 64), dtype=F8, in_channels=64, **norm).to(DEV)
+    x = torch.randn(1, 8, 8, 64, device=DEV).bfloat16()
+    with torch.inference_mode():
+        layer(x)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = layer(x)
+    for step in range(3):
+        with torch.no_grad():
+            layer.kernel.mul_(1.5)
+            (layer.bn.beta if norm else layer.bias).add_(1.0)
+        want = layer(x).clone()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+
+
+def test_conv8_group_norm_output_view_is_checked():
+    from yolo_amd.layers import YOLOConv
+    layer = YOLOConv((1, 1, 64), dtype=F8, in_channels=64, groupNormalization=8).to(DEV)
+    x = torch.randn(2, 8, 8, 64, device=DEV).bfloat16()
+    buf = torch.zeros(2, 8, 8, 128, device=DEV, dtype=torch.bfloat16)
+    assert torch.equal(layer(x, out=buf[..., 64:]), layer(x)) and not buf[..., :64].any()
+    for bad in (buf, buf[:1, ..., :64], buf[..., :64].float()):
+        with pytest.raises(ValueError, match="out must be"):
+            layer(x, out=bad)
+
+
 def test_networks_run_in_8_bits():
     """Darknet53, CSPDarknet53 and YoloV3 with dtype=torch.float8_e4m3fn (the first layers in bf16): every layer's
     result is the layer function's own on the same input, the maps stay close to the bf16 network's.  e4m3 operands

@@ -130,6 +130,45 @@ def test_group_norm_constant_outlier_and_nan():
         assert torch.isnan(y[..., 4:8]).any() and torch.equal(y[..., :4], ok[..., :4]) and torch.equal(y[..., 8:], ok[..., 8:])
 
 
+@pytest.mark.parametrize("act", ["mish", None])
+@pytest.mark.parametrize("size", [13, 40, 96])            # slabs, chunks, several chunks
+def test_group_norm_non_finite_values_reach_their_group(size, act):
+    """A NaN or an infinity makes the statistics of its sample and group NaN, hence y, dx and the parameters' gradients
+    there (dbeta through the activation's derivative), and nothing else."""
+    from yolo_amd import training as T
+    g = torch.Generator().manual_seed(size)
+    x, dy = torch.randn(2, size, size, 48, generator=g), torch.randn(2, size, size, 48, generator=g)
+    ga, be = torch.ones(48), torch.zeros(48)
+
+    def run(z):
+        leaves = [t.to(DEV).requires_grad_() for t in (z, ga, be)]
+        y = T.group_norm_act(*leaves, 6, act)
+        return [t.detach().cpu() for t in (y, *torch.autograd.grad(y, leaves, dy.to(DEV)))]
+    ok = run(x)
+    for bad, pix in ((float("nan"), 0), (float("inf"), 1), (float("-inf"), size * size - 1), (float("inf"), size * size // 2)):
+        z = x.clone()
+        z.view(2, -1, 48)[1, pix, 19] = bad               # group 2 of sample 1: channels 16 ... 23
+        y, dx, dga, dbe = run(z)
+        for a, b in ((y, ok[0]), (dx, ok[1])):
+            assert torch.isnan(a[1, ..., 16:24]).all()
+            a[1, ..., 16:24] = b[1, ..., 16:24]
+            assert torch.equal(a, b)
+        assert torch.isnan(dga[16:24]).all() and torch.equal(dga[:16], ok[2][:16]) and torch.equal(dga[24:], ok[2][24:])
+        assert (torch.isnan(dbe[16:24]).all() if act else torch.equal(dbe, ok[3])) and torch.equal(dbe[24:], ok[3][24:])
+
+
+@pytest.mark.parametrize("samples,c,g", [(70000, 2048, 64), (1 << 20, 128, 4)])
+def test_group_norm_many_samples_of_one_pixel(samples, c, g):
+    """More channel slabs than a grid has room for: the chunked form takes them."""
+    from yolo_amd import training as T
+    x = torch.randn(samples, c, device=DEV).bfloat16()
+    ga, be = torch.linspace(0.5, 1.5, c, device=DEV), torch.linspace(-1, 1, c, device=DEV)
+    y = T.group_norm_act(x, ga, be, g)
+    for part in (slice(0, 3), slice(samples // 2, samples // 2 + 3), slice(samples - 3, samples)):
+        want = O.group_norm(x[part].float().cpu(), ga.cpu(), be.cpu(), g, None, 1e-3)
+        _within("y", y[part], want["y"], want["t_mag"], torch.bfloat16)
+
+
 @pytest.mark.parametrize("how", ["slice", "permuted", "offset", "expanded", "mixed"])
 def test_group_norm_strides_and_alignment(how):
     """Inputs that are not dense or not 16-byte aligned give the bits of the dense copy."""

@@ -48,6 +48,19 @@ def test_group_norm_entry_points_validate_without_gpu():
     assert L.ymx_dropout(one, None, one, 0, _lib.F32, 0.5, one, None) == 0
 
 
+def test_sizes_beyond_a_grid_are_refused():
+    """More workgroups than a launch has room for; the workspace may then be missing as well."""
+    from yolo_amd import _lib
+    L, one = _lib.lib(), ctypes.c_void_p(256)
+
+    def fwd(B, P, C, G, ws=one):
+        return L.ymx_group_norm_forward(one, one, one, None, one, one, B, P, C, G, 0, 1e-3, _lib.BF16, 0.0, None, ws, 1 << 50, None)
+    for B, P, C, G in ((1 << 20, 1, 2048, 1), (1, 1 << 20, 1 << 20, 4096), (4096, 8, 1 << 19, 8), ((1 << 20) + 1, 4, 64, 8)):
+        for ws in (one, None):
+            assert fwd(B, P, C, G, ws) == -2 and b"samples" in L.ymx_last_error()
+    assert fwd(2, 8, 64, 8, None) == -1 and b"null" in L.ymx_last_error()
+
+
 def test_functions_refuse_before_the_device():
     from yolo_amd import training as T
     x, v = torch.zeros(1, 2, 2, 8), torch.zeros(8)

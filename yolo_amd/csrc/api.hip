@@ -911,9 +911,10 @@ static int gn_args(const char *what, GnArgs &a, long long B, long long n_pix, in
     if (rate > 0.0 && (!state || ((uintptr_t)state & 7))) return fail(YMX_EARG, "%s: dropout needs a state of two 64-bit words", what);
     // pixel indexes are 32-bit in the kernels, and so are workgroup numbers; offsets are 64-bit
     if (G > 4096) return fail(YMX_EUNSUPPORTED, "%s: %d groups (at most 4096)", what, G);      // a pair of each in LDS
-    if (n_pix > (1ll << 30) || B > (1ll << 20) || B * G > (1ll << 30) || (long long)C * B > (1ll << 33))
+    if (n_pix > (1ll << 30) || B > (1ll << 20) || std::max(B, 2048ll) * C > (1ll << 30))
         return fail(YMX_EUNSUPPORTED, "%s: %lld samples of %lld pixels and %d channels", what, B, n_pix, C);
     const size_t need = group_norm_workspace_bytes((int)B, (int)n_pix, C, G);
+    if (!ws) return fail(YMX_EARG, "%s: null pointer", what);
     if (!aligned16(ws)) return fail(YMX_EARG, "%s: the workspace must be 16-byte aligned", what);
     if (ws_bytes < need) return fail(YMX_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, ws_bytes, need);
     a.B = (int)B; a.P = (int)n_pix; a.C = C; a.G = G; a.D = C / G;
@@ -932,7 +933,7 @@ size_t ymx_group_norm_workspace_bytes(long long B, long long n_pix, int C, int G
 int ymx_group_norm_forward(const void *x, const float *gamma, const float *beta, const void *residual, void *y, float *stats,
                            long long B, long long n_pix, int C, int G, int act, float eps, int dtype, double rate,
                            const void *state, void *workspace, size_t ws_bytes, void *stream) {
-    if (!x || !gamma || !beta || !y || !workspace) return fail(YMX_EARG, "group_norm_forward: null pointer");
+    if (!x || !gamma || !beta || !y) return fail(YMX_EARG, "group_norm_forward: null pointer");
     if (!(eps > 0.0f)) return fail(YMX_EARG, "group_norm_forward: epsilon %g", (double)eps);
     GnArgs a = {};
     if (const int rc = gn_args("group_norm_forward", a, B, n_pix, C, G, act, dtype, rate, state, workspace, ws_bytes)) return rc;
@@ -943,7 +944,7 @@ int ymx_group_norm_forward(const void *x, const float *gamma, const float *beta,
 int ymx_group_norm_backward(const void *x, const void *dy, const float *gamma, const float *beta, const float *stats, void *dx,
                             float *dgamma, float *dbeta, long long B, long long n_pix, int C, int G, int act, int dtype,
                             double rate, const void *state, void *workspace, size_t ws_bytes, void *stream) {
-    if (!x || !dy || !gamma || !beta || !stats || !dx || !dgamma || !dbeta || !workspace)
+    if (!x || !dy || !gamma || !beta || !stats || !dx || !dgamma || !dbeta)
         return fail(YMX_EARG, "group_norm_backward: null pointer");
     GnArgs a = {};
     if (const int rc = gn_args("group_norm_backward", a, B, n_pix, C, G, act, dtype, rate, state, workspace, ws_bytes)) return rc;

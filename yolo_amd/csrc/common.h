@@ -120,7 +120,7 @@ __device__ __forceinline__ float mish_grad_f(float z) {
     return z > 20.0f ? 1.0f : g;
 }
 template <int ACT> __device__ __forceinline__ float act_grad_c(float z) {
-    if constexpr (ACT == YMX_ACT_MISH) return mish_grad_f(z);
+    if constexpr (ACT == YMX_ACT_MISH) return z == z ? mish_grad_f(z) : z;       // (its minimum drops a NaN)
     if constexpr (ACT == YMX_ACT_LEAKY) return z > 0.0f ? 1.0f : 0.1f;
     return 1.0f;
 }

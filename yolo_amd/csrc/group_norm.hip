@@ -66,6 +66,9 @@ template <int V> struct GnPos {
     }
 };
 
+// A sum of squares that rounding may have taken below zero; NaN stays NaN (an infinity in the map makes the variance one).
+__device__ __forceinline__ float gn_squares(float v) { return v < 0.0f ? 0.0f : v; }
+
 // Calls use(p, load(p)) for p, p + R, ... < p1, U loads in flight at a time.
 template <int U, typename L, typename F> __device__ __forceinline__ void gn_rows(int p, int p1, int R, L load, F use) {
     for (; p + (U - 1) * R < p1; p += U * R) {
@@ -141,7 +144,7 @@ __global__ void __launch_bounds__(256) gn_stats_kernel(const GnArgs a, const GnW
         const float inv = n > 0 ? 1.0f / (float)n : 0.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            red[g.r * W + g.cv * V + i] = float2{piv[i] + s1[i] * inv, fmaxf(s2[i] - s1[i] * s1[i] * inv, 0.0f)};
+            red[g.r * W + g.cv * V + i] = float2{piv[i] + s1[i] * inv, gn_squares(s2[i] - s1[i] * s1[i] * inv)};
     }
     __syncthreads();
     const int np = g.p1 - g.chunk * w.per;                       // pixels of the chunk
@@ -223,7 +226,7 @@ __device__ __forceinline__ void gn_join(const GnArgs &a, const GnWork &w, int b,
                 out[g] = float2{s.x * inv_n, s.y * inv_n};
             } else {
                 const float shift = s.x * inv_n;
-                out[g] = float2{piv + shift, 1.0f / sqrtf(fmaxf(s.y * inv_n - shift * shift, 0.0f) + a.eps)};
+                out[g] = float2{piv + shift, 1.0f / sqrtf(gn_squares(s.y * inv_n - shift * shift) + a.eps)};
                 if (keep && a.stats) ((float2 *)a.stats)[(size_t)b * a.G + g] = out[g];
             }
         }
@@ -697,7 +700,7 @@ template <int V> static GnSlab gn_slab(const GnArgs &a, int most) {
     GnSlab best = {0, 0};
     if (a.D > 64 || (a.D & (a.D - 1))) return best;
     for (int sv = 4; sv <= 16 && cv % sv == 0; sv *= 2) {
-        if (sv * V % a.D || (long long)a.P * sv > 512ll * most) continue;
+        if (sv * V % a.D || (long long)a.P * sv > 512ll * most || (long long)a.B * (cv / sv) > (1 << 22)) continue;   // (a grid has 2^32 threads)
         if (best.sv && ((long long)a.B * (cv / sv) < 256 || (long long)a.P * sv > 512 * 6)) break;
         best.sv = sv;
         best.nslab = cv / sv;

@@ -32,8 +32,8 @@ struct DropArgs {
     float keep_scale;
 };
 
-// Multiplier (keep_scale or, for a dropped element, a zero the caller must select by: keep[i]) of
-// V consecutive elements from linear index i0 (a multiple of V where V > 1).
+// Which of V consecutive elements from linear index i0 (a multiple of V where V > 1) are kept.  The caller selects (a
+// dropped element is 0 whatever it held).
 template <int V> __device__ __forceinline__ void drop_keep(const DropArgs &d, const uint4 &sc, unsigned long long i0, bool (&keep)[V]) {
     if constexpr (V >= 4) {
 #pragma unroll
