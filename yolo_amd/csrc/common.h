@@ -119,8 +119,18 @@ __device__ __forceinline__ float mish_grad_f(float z) {
     const float g = e * w * __builtin_amdgcn_rcpf(d * d);
     return z > 20.0f ? 1.0f : g;
 }
+// The same derivative in fewer operations, for kernels that evaluate it twice per element: with n = e (e + 2), r = 1 / (n + 2),
+// tanh(softplus(z)) = n r and the other term is 4 z e (e + 1) r^2 = 4 z (n - e) r^2.  No difference of it cancels
+// but the one at the derivative's zero.  z > 40 gives 1 as it is; NaN stays NaN.
+__device__ __forceinline__ float mish_grad2_f(float z) {
+#pragma clang fp contract(fast)
+    const float zc = z > 40.0f ? 40.0f : z;
+    const float e = __builtin_amdgcn_exp2f(zc * 1.44269504088896f);
+    const float n = e * (e + 2.0f), r = __builtin_amdgcn_rcpf(n + 2.0f);
+    return (n + 4.0f * (zc * (n - e) * r)) * r;
+}
 template <int ACT> __device__ __forceinline__ float act_grad_c(float z) {
-    if constexpr (ACT == YMX_ACT_MISH) return z == z ? mish_grad_f(z) : z;       // (its minimum drops a NaN)
+    if constexpr (ACT == YMX_ACT_MISH) return mish_grad2_f(z);
     if constexpr (ACT == YMX_ACT_LEAKY) return z > 0.0f ? 1.0f : 0.1f;
     return 1.0f;
 }
