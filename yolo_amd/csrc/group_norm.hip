@@ -297,18 +297,24 @@ __global__ void __launch_bounds__(256) gn_apply_kernel(const GnArgs a, const GnW
                });
 }
 
-// dt of one vector of a map and its gradient.
+// dt of one vector of a map and its gradient; bit i of keep: element i is kept.
 template <int V, int ACT, bool DROP>
-__device__ __forceinline__ void gn_dt(const GnChannels<V> &ch, const DropArgs &drop, const uint4 &key, unsigned long long i0,
-                                      const float (&x)[V], const float (&dy)[V], float (&dt)[V]) {
-    bool keep[V];
-    if constexpr (DROP) drop_keep<V>(drop, key, i0, keep);
+__device__ __forceinline__ void gn_dt(const GnChannels<V> &ch, float keep_scale, unsigned keep, const float (&x)[V], const float (&dy)[V],
+                                      float (&dt)[V]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         float d = dy[i];
-        if constexpr (DROP) d = keep[i] ? d * drop.keep_scale : 0.0f;
+        if constexpr (DROP) d = (keep >> i & 1u) ? d * keep_scale : 0.0f;
         dt[i] = d * act_grad_c<ACT>(ch.t(i, x[i]));
     }
+}
+template <int V> __device__ __forceinline__ unsigned gn_keep_bits(const DropArgs &drop, const uint4 &key, unsigned long long i0) {
+    bool keep[V];
+    drop_keep<V>(drop, key, i0, keep);
+    unsigned m = 0u;
+#pragma unroll
+    for (int i = 0; i < V; ++i) m |= keep[i] ? 1u << i : 0u;
+    return m;
 }
 
 // dx of V values: r (gamma dt - (m1 + h m2)) = ta dt + d b + c with the group's m1 = S1 / N, m2 = S2 / N.
@@ -324,10 +330,12 @@ template <int V> struct GnGradient {
 };
 
 // Pass 1, backward: part[(b nchunk + chunk) C + c] = (sum dt, sum dt h) of the chunk's pixels, and
-// gpart[((b nchunk + chunk) nsub + sub) G + g] = (S1, S2) of the block's values.
+// gpart[((b nchunk + chunk) nsub + sub) G + g] = (S1, S2) of the block's values.  With dropout, mask (V > 1) receives a byte
+// of kept elements per vector for pass 2: the random words are a fifth of this pass (16 x 208^2 x 64, rate 0.1: backward
+// 126.8 us with the words in both passes, 117.0 with the bytes).
 template <typename T, int V, int ACT, bool DROP>
 __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const GnArgs a, const GnWork w, float2 *__restrict__ part,
-                                                          float2 *__restrict__ gpart) {
+                                                          float2 *__restrict__ gpart, unsigned char *__restrict__ mask) {
     __shared__ float2 red[256 * V];                              // [R][W]; row 0 then holds gamma times the channels' pairs
     const GnPos<V> g(a, w);
     typedef vec_io<T, V> IO;
@@ -349,7 +357,13 @@ __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const GnArgs a, const 
                        float v[V], d[V], dt[V];
                        IO::unpack(q.x, v);
                        IO::unpack(q.d, d);
-                       gn_dt<V, ACT, DROP>(ch, drop, key, base + (size_t)p * a.C, v, d, dt);
+                       unsigned keep = 0u;
+                       if constexpr (DROP) {
+                           const size_t at = base + (size_t)p * a.C;
+                           keep = gn_keep_bits<V>(drop, key, at);
+                           if constexpr (V > 1) mask[at / V] = (unsigned char)keep;
+                       }
+                       gn_dt<V, ACT, DROP>(ch, drop.keep_scale, keep, v, d, dt);
 #pragma unroll
                        for (int i = 0; i < V; ++i) {
                            s1[i] += dt[i];
@@ -422,7 +436,7 @@ __global__ void __launch_bounds__(1024) gn_param_grads_kernel(const GnArgs a, in
 // Pass 2, backward.
 template <typename T, int V, int ACT, bool DROP>
 __global__ void __launch_bounds__(256) gn_bwd_apply_kernel(const GnArgs a, const GnWork w, const float2 *__restrict__ part,
-                                                           const float2 *__restrict__ gpart, int nparam) {
+                                                           const float2 *__restrict__ gpart, const unsigned char *__restrict__ mask, int nparam) {
     extern __shared__ __attribute__((aligned(16))) float2 joined[];      // [G], then 256 of scratch; or 16 * 17 pairs of doubles
     if ((int)blockIdx.x < nparam) {                              // the first workgroups: parameter gradients, 16 channels each
         gn_param_grads<16>(a, blockIdx.x, a.B * w.nchunk, part, (double2 *)joined);
@@ -445,14 +459,20 @@ __global__ void __launch_bounds__(256) gn_bwd_apply_kernel(const GnArgs a, const
     T *__restrict__ dx = (T *)a.dx + base;
     const DropArgs drop = {a.state, a.threshold, a.keep_scale};
     uint4 key = {};
-    if constexpr (DROP) key = uint4{a.state[0], a.state[1], a.state[2], a.state[3]};
-    struct Row { typename IO::raw x, d; };
-    gn_rows<4>(g.p, g.p1, w.R, [&](int p) { return Row{IO::load(x + (size_t)p * a.C), IO::load(dy + (size_t)p * a.C)}; },
+    if constexpr (DROP && V == 1) key = uint4{a.state[0], a.state[1], a.state[2], a.state[3]};
+    struct Row { typename IO::raw x, d; unsigned keep; };
+    gn_rows<4>(g.p, g.p1, w.R, [&](int p) {
+                   Row q = {IO::load(x + (size_t)p * a.C), IO::load(dy + (size_t)p * a.C), 0u};
+                   if constexpr (DROP && V > 1) q.keep = mask[(base + (size_t)p * a.C) / V];
+                   return q;
+               },
                [&](int p, const Row &q) {
                    float v[V], d[V], dt[V];
                    IO::unpack(q.x, v);
                    IO::unpack(q.d, d);
-                   gn_dt<V, ACT, DROP>(ch, drop, key, base + (size_t)p * a.C, v, d, dt);
+                   unsigned keep = q.keep;
+                   if constexpr (DROP && V == 1) keep = gn_keep_bits<V>(drop, key, base + (size_t)p * a.C);
+                   gn_dt<V, ACT, DROP>(ch, drop.keep_scale, keep, v, d, dt);
 #pragma unroll
                    for (int i = 0; i < V; ++i) v[i] = gr.dx(ch, i, v[i], dt[i]);
                    IO::store(dx + (size_t)p * a.C, v);
@@ -612,7 +632,9 @@ __global__ void __launch_bounds__(512) gn_slab_bwd_kernel(const GnArgs a, const 
             float v[V], d[V];
             IO::unpack(q[n], v);
             IO::unpack(qd[n], d);
-            gn_dt<V, ACT, DROP>(ch, drop, key, base + (size_t)p * a.C, v, d, dt[n]);
+            unsigned keep = 0u;
+            if constexpr (DROP) keep = gn_keep_bits<V>(drop, key, base + (size_t)p * a.C);
+            gn_dt<V, ACT, DROP>(ch, drop.keep_scale, keep, v, d, dt[n]);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 s1[i] += dt[n][i];
@@ -683,10 +705,11 @@ template <int V> static GnWork gn_work(const GnArgs &a) {
     w.nchunk = (a.P + w.per - 1) / w.per;
     return w;
 }
-// Pairs: one per (chunk, channel) and one per (chunk, group or part of one).
+// Pairs: one per (chunk, channel) and one per (chunk, group or part of one).  Behind them the backward pass's bytes of kept
+// elements, one for four or eight.
 static size_t gn_pairs(int G, int C) { return (size_t)G * ((C / G + 255) / 256); }
 size_t group_norm_workspace_bytes(int B, int P, int C, int G) {
-    return (size_t)B * gn_chunks(B, P, C) * (C + gn_pairs(G, C)) * sizeof(float2);
+    return (size_t)B * gn_chunks(B, P, C) * (C + gn_pairs(G, C)) * sizeof(float2) + (size_t)B * P * C / 4;
 }
 
 // The one-pass form's slabs, or sv = 0 where the chunked form runs: groups of a power of two of at most 64
@@ -776,11 +799,12 @@ template <typename T> static int gn_backward(const GnArgs &a, void *ws, hipStrea
         const GnWork w = gn_work<V>(a);
         const dim3 grid((unsigned)(a.B * w.nchunk * w.nzb));
         float2 *gpart = (float2 *)ws, *part = gpart + (size_t)a.B * w.nchunk * w.nsub * a.G;
+        unsigned char *mask = (unsigned char *)(part + (size_t)a.B * w.nchunk * a.C);
         const int nparam = (a.C + 127) / 128 * 8;                // whole eights: a chunk stays on the XCD that pass 1 read it on
-        hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT, DROP>), grid, dim3(256), 0, s, a, w, part, gpart);
+        hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT, DROP>), grid, dim3(256), 0, s, a, w, part, gpart, mask);
         hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, DROP>), dim3(grid.x + nparam), dim3(256),
                            std::max((a.G + 256) * sizeof(float2), 16 * 17 * sizeof(double2)), s, a, w,
-                           part, gpart, nparam);
+                           part, gpart, mask, nparam);
     });
     return check_launch("group_norm_backward");
 }
