@@ -240,6 +240,36 @@ def test_conv8_capture_needs_a_packed_kernel():
         assert torch.equal(y, want)
 
 
+@pytest.mark.parametrize("b,size,cin,cout,stride,out", [(1, 13, 1024, 512, 1, torch.bfloat16), (1, 13, 16, 40, 1, torch.bfloat16),
+                                                        (3, 7, 144, 255, 1, torch.float32), (1, 1, 272, 64, 1, torch.bfloat16),
+                                                        (2, 23, 400, 72, 2, torch.bfloat16), (8, 13, 1024, 512, 1, torch.float32)])
+def test_conv8_quantises_small_maps_itself(b, size, cin, cout, stride, out):
+    """A 1x1 layer of few pixels takes the plain map in one launch: the bits of quantisation and product one after the other,
+    for blocks of any size, zeros, NaN and infinities, fp32 maps and maps that are not 16-byte aligned."""
+    from yolo_amd import _lib
+    from yolo_amd.layers import YOLOConv, quantize_blocks
+    oh = size if stride == 1 else (size + 1 - 1) // 2 + 1
+    assert _lib.lib().ymx_conv2d_quantizes(b * oh * oh, cout, 1) == 1 and _lib.lib().ymx_conv2d_quantizes(b * oh * oh, cout, 3) == 0
+    layer = YOLOConv((1, 1, cout), downsample=stride == 2, dtype=F8, in_channels=cin).to(DEV)
+    g = torch.Generator().manual_seed(cin)
+    x = torch.randn(b, size, size, cin, generator=g)
+    flat = x.view(-1, cin)
+    flat *= torch.exp2(torch.randint(-40, 40, (flat.shape[0], 1), generator=g).float())
+    flat[0] = 0.0
+    if flat.shape[0] > 8:
+        flat[1, :16] = 0.0
+        flat[2, cin // 2], flat[3, 0], flat[4, cin - 1] = float("nan"), float("inf"), float("-inf")
+        flat[5], flat[6], flat[7] = torch.finfo(torch.bfloat16).max, 1e-38, float("inf")
+    x = x.to(DEV).bfloat16()
+    oh, ow = layer.output_hw(size, size)
+    res = torch.randn(b, oh, ow, cout, device=DEV)
+    for r in (None, res):
+        want = layer(quantize_blocks(x), residual=r, out_dtype=out)
+        shifted = torch.empty(x.numel() + 1, device=DEV, dtype=x.dtype)[1:].view(x.shape).copy_(x)
+        for y in (layer(x, residual=r, out_dtype=out), layer(x.float(), residual=r, out_dtype=out), layer(shifted, residual=r, out_dtype=out)):
+            assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(torch.nan_to_num(y), torch.nan_to_num(want))
+
+
 @pytest.mark.parametrize("norm", [dict(), dict(batchNormalization=True)])
 def test_conv8_graph_follows_a_repacked_kernel(norm):
     """A changed kernel is packed again where the old one was, so that a graph captured before reads no freed memory

@@ -13,6 +13,7 @@ struct F8Args {
     const void *xs, *ws;         // exponents of the map [block][plane] and of the kernel [K tile][rows], bytes
     unsigned xs_bytes, ws_bytes;
     unsigned plane;              // pixels of the map, rounded up to 4
+    unsigned pitch;              // bytes from pixel to pixel of the map
     int rows, nkt, taps;         // padded output channels, K tiles, filter taps
     unsigned taps_m, taps_s;     // fastdiv of the taps
 };

@@ -163,25 +163,68 @@ int launch_pack_f8(const float *w_hwio, void *packed, int k, int Cin, int Cout, 
     return check_launch("pack_weights");
 }
 
+// ---- quantisation inside the product ------------------------------------------------------------------
+// 16 bf16 values -> e4m3 numbers and the exponent byte of their block, which eight neighbouring lanes share: the values
+// and bytes that quantize_kernel gives.
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u16x2_t f8_max2(u16x2_t a, uint32_t b) { return __builtin_elementwise_max(a, __builtin_bit_cast(u16x2_t, b)); }
+__device__ __forceinline__ uint4 f8_quantize16(uint32_t (&w)[8], int &e) {
+    u16x2_t m = {0, 0};
+#pragma unroll
+    for (int n = 0; n < 8; ++n) m = f8_max2(m, w[n] & 0x7fff7fffu);
+    if (__any(max((uint32_t)m.x, (uint32_t)m.y) >= 0x7f80u)) {   // NaN and infinities: NaN, and no part in the maximum
+        m = u16x2_t{0, 0};
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            const bool lo = (w[n] & 0x7fffu) >= 0x7f80u, hi = (w[n] & 0x7fff0000u) >= 0x7f800000u;
+            m = f8_max2(m, w[n] & ((lo ? 0u : 0x7fffu) | (hi ? 0u : 0x7fff0000u)));
+            w[n] |= (lo ? 0x7fffu : 0u) | (hi ? 0x7fff0000u : 0u);
+        }
+    }
+    uint32_t p = max((uint32_t)m.x, (uint32_t)m.y);
+    p = max(p, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)p, 0xb1, 0xf, 0xf, false));       // lane ^ 1
+    p = max(p, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)p, 0x4e, 0xf, 0xf, false));       // lane ^ 2
+    p = max(p, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)p, 0x141, 0xf, 0xf, false));      // 7 - lane of eight
+    e = f8_exponent(p << 16) + 127;
+    const float f = __uint_as_float((uint32_t)e << 23);
+    typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+    typedef short s2 __attribute__((ext_vector_type(2)));
+    uint32_t o[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        s2 v = {0, 0};
+        v = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(v, __builtin_bit_cast(bf2, w[2 * n]), f, false);
+        v = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(v, __builtin_bit_cast(bf2, w[2 * n + 1]), f, true);
+        o[n] = __builtin_bit_cast(uint32_t, v);
+    }
+    return uint4{o[0], o[1], o[2], o[3]};
+}
+
 // ---- the product ----------------------------------------------------------------------------------
 // NWQ x NWP waves, each 16 NI channels x 16 NJ pixels; K tiles of 128 channels of one tap through NSTAGE stages
 // of LDS, filled by LDS-DMA NSTAGE - 1 tiles ahead, one barrier per tile.  Rows are 128 bytes (one pixel's or one
 // channel's 128 values), the 16-byte chunk c of row r in slot c ^ (r & 7): the lanes that read one fragment then
 // touch 16 different slots.  A lane's 32 values of a fragment are the chunks q and q + 4 of its row, q = lane / 16,
 // for pixels and channels alike (the order inside a block does not matter: one exponent covers it).
-template <typename OT, int NWQ, int NWP, int NI, int NJ, int NSTAGE> struct F8Tile {
+//
+// RAW: x is a bf16 map, staged as such (256 bytes per pixel and K tile, chunk c of row r in slot c ^ (r & 15)).  While
+// tile kt is multiplied, the threads quantise tile kt + 1, 16 channels each, into one of two further row buffers.
+template <bool RAW, int NWQ, int NWP, int NI, int NJ, int NSTAGE> struct F8Tile {
     static constexpr int NW = NWQ * NWP, TQ = NWQ * NI * 16, TP = NWP * NJ * 16;
-    static constexpr int NXI = TP / 8 / NW, NWI = TQ / 8 / NW;                       // DMA instructions per wave: rows ...
-    static constexpr int SX = (TP + 63) / 64, NS = SX + (TQ + 63) / 64;              // ... and, in all, exponents
+    static constexpr int XROW = RAW ? 256 : 128, XPER = 1024 / XROW;                // bytes of a pixel, pixels per instruction
+    static constexpr int NXI = TP / XPER / NW, NWI = TQ / 8 / NW;                       // DMA instructions per wave: rows ...
+    static constexpr int SX = RAW ? 0 : (TP + 63) / 64, NS = SX + (TQ + 63) / 64;              // ... and, in all, exponents
     static constexpr int NSI = (NS + NW - 1) / NW;                                   // (per wave)
-    static constexpr int XB = TP * 128, WB = TQ * 128, STAGE = XB + WB + NS * 256, PIECES = NXI + NWI + NSI;
-    static constexpr int EPI = NW * EpiGeom<NI, 64, 16 * NJ>::LDS_BYTES, LDS = NSTAGE * STAGE > EPI ? NSTAGE * STAGE : EPI;
-    static_assert(TP % (8 * NW) == 0 && TQ % (8 * NW) == 0, "whole instructions per wave");
+    static constexpr int XB = TP * XROW, WB = TQ * 128, STAGE = XB + WB + NS * 256, PIECES = NXI + NWI + NSI;
+    static constexpr int EPI = NW * EpiGeom<NI, 64, 16 * NJ>::LDS_BYTES;
+    static constexpr int XQ = RAW ? TP * 132 : 0, USED = NSTAGE * STAGE + 2 * XQ, LDS = USED > EPI ? USED : EPI;     // (rows and exponents)
+    static constexpr int AHEAD = NSTAGE - (RAW ? 3 : 2);                             // K tiles in flight behind the one waited for
+    static_assert(TP % (XPER * NW) == 0 && TQ % (8 * NW) == 0, "whole instructions per wave");
 };
-template <typename OT, int NWQ, int NWP, int NI, int NJ, int NSTAGE>
+template <bool RAW, typename OT, int NWQ, int NWP, int NI, int NJ, int NSTAGE>
 __global__ void __launch_bounds__(64 * NWQ * NWP, 2)
 conv_f8_kernel(const F8Args g, const int ntile_q) {
-    typedef F8Tile<OT, NWQ, NWP, NI, NJ, NSTAGE> C;
+    typedef F8Tile<RAW, NWQ, NWP, NI, NJ, NSTAGE> C;
     constexpr int NXI = C::NXI, NWI = C::NWI, NSI = C::NSI, SX = C::SX, XB = C::XB, WB = C::WB, STAGE = C::STAGE;
     constexpr bool EXACT = sizeof(OT) == 4;
     constexpr unsigned OOB = 0x80000000u;
@@ -199,11 +242,14 @@ conv_f8_kernel(const F8Args g, const int ntile_q) {
 
     const int srow = lane >> 3, chunk = (lane & 7) ^ srow;
     unsigned xoff[NXI], xmask[NXI];
+    int xch[NXI];                                            // first channel, within the block, of the 16 bytes
 #pragma unroll
     for (int i = 0; i < NXI; ++i) {
         int pix;
-        pixel_geometry(a, p0 + (wave * NXI + i) * 8 + srow, pix, xmask[i]);
-        xoff[i] = (unsigned)pix * (unsigned)a.Cin + (unsigned)(chunk * 16);
+        const int row = (wave * NXI + i) * C::XPER + (RAW ? lane >> 4 : srow), ck = RAW ? (lane & 15) ^ (row & 15) : chunk;
+        pixel_geometry(a, p0 + row, pix, xmask[i]);
+        xoff[i] = (unsigned)pix * g.pitch + (unsigned)(ck * 16);
+        xch[i] = ck * (RAW ? 8 : 16);
     }
     const unsigned row_bytes = (unsigned)(g.nkt * 128);
     const unsigned woff = (unsigned)(q0 + wave * NWI * 8 + srow) * row_bytes + (unsigned)chunk * 16u;
@@ -235,10 +281,10 @@ conv_f8_kernel(const F8Args g, const int ntile_q) {
         const int tpix = tr * a.W + tc;
         const bool on = kn < g.nkt;
         const unsigned bit = on ? 1u << (tr * a.k + tc) : 0u;
-        const unsigned step = (unsigned)tpix * (unsigned)a.Cin + (unsigned)(blk * 128);
-        const unsigned cbit = blk * 128 + chunk * 16 < a.Cin ? bit : 0u;
+        const unsigned step = (unsigned)tpix * g.pitch + (unsigned)(blk * C::XROW);
 #pragma unroll
-        for (int i = 0; i < NXI; ++i) f8_dma16(xr, sb + (unsigned)((wave * NXI + i) * 1024), (xmask[i] & cbit) ? xoff[i] + step : OOB);
+        for (int i = 0; i < NXI; ++i)
+            f8_dma16(xr, sb + (unsigned)((wave * NXI + i) * 1024), (xmask[i] & (blk * 128 + xch[i] < a.Cin ? bit : 0u)) ? xoff[i] + step : OOB);
         const unsigned wk = on ? woff + (unsigned)kn * 128u : OOB;
 #pragma unroll
         for (int i = 0; i < NWI; ++i) f8_dma16(wr, sb + (unsigned)(XB + (wave * NWI + i) * 1024), wk + (unsigned)i * 8u * row_bytes);
@@ -264,7 +310,7 @@ conv_f8_kernel(const F8Args g, const int ntile_q) {
     const int frow = lane & 15, q = lane >> 4;
     const int s0 = (q ^ (frow & 7)) << 4, s1 = ((q + 4) ^ (frow & 7)) << 4;
     const int a_off = XB + (wq * NI * 16 + frow) * 128, b_off = (wp * NJ * 16 + frow) * 128;
-    const int as_off = XB + WB + (SX * 64 + wq * NI * 16 + frow) * 4, bs_off = XB + WB + (wp * NJ * 16 + frow) * 4;
+    const int as_off = XB + WB + (SX * 64 + wq * NI * 16 + frow) * 4, bs_off = (RAW ? C::TP * 128 : XB + WB) + (wp * NJ * 16 + frow) * 4;
 
     auto frag = [&](const char *p) { return f8_frag(*(const int4 *)(p + s0), *(const int4 *)(p + s1)); };
     // Fragments of a tile: all pixels', and the channels' where there are few of them (PRE), before the next DMA is issued,
@@ -276,14 +322,28 @@ conv_f8_kernel(const F8Args g, const int ntile_q) {
         f = frag(base + a_off + i * 2048);
         e = *(const int *)(base + as_off + i * 64);
     };
-    auto load = [&](const char *base) {
+    auto load = [&](const char *base, const char *xbase) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            b[j] = frag(base + b_off + j * 2048);
-            bs[j] = *(const int *)(base + bs_off + j * 64);
+            b[j] = frag(xbase + b_off + j * 2048);
+            bs[j] = *(const int *)(xbase + bs_off + j * 64);
         }
 #pragma unroll
         for (int i = 0; i < PRE; ++i) load_w(base, i, w[i], ws[i]);
+    };
+    // RAW: tile kt's pixels t / 8, t / 8 + 8 NW, ...: 16 channels a thread
+    char *xq = smem + NSTAGE * STAGE;
+    auto quantize = [&](const char *base, char *to) {
+#pragma unroll
+        for (int n = 0; n < C::TP / (8 * C::NW); ++n) {
+            const int row = n * 8 * C::NW + (t >> 3), part = t & 7;
+            const uint4 lo = *(const uint4 *)(base + row * 256 + (((2 * part) ^ (row & 15)) << 4));
+            const uint4 hi = *(const uint4 *)(base + row * 256 + (((2 * part + 1) ^ (row & 15)) << 4));
+            uint32_t v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+            int e;
+            *(uint4 *)(to + row * 128 + ((part ^ (row & 7)) << 4)) = f8_quantize16(v, e);
+            if (part == 0) *(int *)(to + C::TP * 128 + row * 4) = e;
+        }
     };
     auto compute = [&](const char *base) {
         bf16x8_t bb[EXACT ? NJ : 1][4];                          // 32-bit outputs: the same fragments, scaled, as bf16
@@ -317,26 +377,32 @@ conv_f8_kernel(const F8Args g, const int ntile_q) {
     f8_dma_ready();
 #pragma unroll
     for (int i = 0; i < NSTAGE - 1; ++i) dma(i);
-    f8_vmcnt<C::PIECES * (NSTAGE - 2)>();
+    f8_vmcnt<C::PIECES * C::AHEAD>();
     __syncthreads();
+    if constexpr (RAW) {
+        quantize(smem, xq);
+        __syncthreads();
+    }
     int st = 0;
     for (int kt = 0; kt < g.nkt; ++kt) {
         const char *base = smem + st * STAGE;
-        load(base);
+        const int next = st + 1 == NSTAGE ? 0 : st + 1;
+        load(base, RAW ? xq + (kt & 1) * C::XQ : base);
         dma(st == 0 ? NSTAGE - 1 : st - 1);
+        if constexpr (RAW) quantize(smem + next * STAGE, xq + (kt + 1 & 1) * C::XQ);
         compute(base);
-        f8_vmcnt<C::PIECES * (NSTAGE - 2)>();
+        f8_vmcnt<C::PIECES * C::AHEAD>();
         __syncthreads();
-        st = st + 1 == NSTAGE ? 0 : st + 1;
+        st = next;
     }
     f8_vmcnt<0>();
     __syncthreads();
     f8_epilogue<OT, NI, NJ>(a, acc, smem, wave, q0 + wq * NI * 16, p0 + wp * NJ * 16, lane);
 }
 
-template <typename OT, int NWQ, int NWP, int NI, int NJ, int NSTAGE> static int launch_f8_cfg(const F8Args &g, hipStream_t s) {
-    typedef F8Tile<OT, NWQ, NWP, NI, NJ, NSTAGE> C;
-    auto kern = conv_f8_kernel<OT, NWQ, NWP, NI, NJ, NSTAGE>;
+template <typename OT, int NWQ, int NWP, int NI, int NJ, int NSTAGE, bool RAW = false> static int launch_f8_cfg(const F8Args &g, hipStream_t s) {
+    typedef F8Tile<RAW, NWQ, NWP, NI, NJ, NSTAGE> C;
+    auto kern = conv_f8_kernel<RAW, OT, NWQ, NWP, NI, NJ, NSTAGE>;
     static LdsReserve reserved;
     if (const int rc = reserve_lds(reserved, (const void *)kern, C::LDS, "conv_f8")) return rc;
     const int ntq = (g.a.Cout + C::TQ - 1) / C::TQ;
@@ -368,7 +434,14 @@ template <typename OT> static int launch_f8_shape(const F8Args &g, hipStream_t s
     return launch_f8_cfg<OT, 4, 1, 1, 4, 4>(g, s);
 }
 
-// a: geometry of the convolution with x_ld = Cin; x = quantised map, w = packed kernel.
+// Whether a layer on a bf16 map quantises it in its own kernel, in tiles of 64 x 32.  Every tile of channels and every tap
+// quantises its pixels again, so where there are few of them: 1x1 windows, up to 176 tiles of 64 x 64.  Measured (us, one
+// launch against two): 13^2 1024 -> 512 11.3, 12.3; 26^2 256 -> 512 8.7, 10.7; 52^2 256 -> 255 to fp32 10.0, 11.9; 8 x 13^2 1024 ->
+// 512 (176 tiles) 13.9, 13.8; 8 x 13^2 1024 -> 1024 (352) 20.4, 15.2; 3x3: 13^2 512 -> 1024 25.8, 20.2.  And 6 us less on the host.
+bool conv_f8_raw(long long P, int Cout, int k) { return k == 1 && (P + 63) / 64 * ((Cout + 63) / 64) <= 176; }
+
+// a: geometry of the convolution with x_ld = Cin; x = quantised map, or a bf16 one
+// where conv_f8_raw says so; w = packed kernel.
 int launch_conv_f8(const ConvArgs &args, long long in_pix, hipStream_t s) {
     F8Args g;
     g.a = args;
@@ -378,19 +451,22 @@ int launch_conv_f8(const ConvArgs &args, long long in_pix, hipStream_t s) {
     g.rows = f8_rows(args.Cout);
     g.plane = (unsigned)f8_plane(in_pix);
     set_fastdiv((unsigned)g.taps, g.taps_m, g.taps_s);
-    const unsigned long long xb = (unsigned long long)in_pix * args.Cin, wb = (unsigned long long)g.rows * g.nkt * 128;
+    const bool raw = args.x_dtype == YMX_BF16;
+    g.pitch = raw ? (unsigned)args.x_ld * 2u : (unsigned)args.Cin;
+    const unsigned long long xb = raw ? ((unsigned long long)(in_pix - 1) * args.x_ld + args.Cin) * 2 : (unsigned long long)in_pix * args.Cin, wb = (unsigned long long)g.rows * g.nkt * 128;
     if (xb >= (1ull << 31) || wb >= (1ull << 31) || (unsigned long long)g.plane * ((args.Cin + 127) / 128) >= (1ull << 31))
         return fail(YMX_EUNSUPPORTED, "conv2d: more than 2 GiB of 8-bit input or kernel");
     g.a.x_bytes = (unsigned)xb;
     g.a.w_bytes = (unsigned)wb;
-    g.xs = (const char *)args.x + f8_map_bytes(in_pix, args.Cin);
-    g.xs_bytes = g.plane * (unsigned)((args.Cin + 127) / 128);
+    g.xs = raw ? nullptr : (const char *)args.x + f8_map_bytes(in_pix, args.Cin);
+    g.xs_bytes = raw ? 0u : g.plane * (unsigned)((args.Cin + 127) / 128);
     g.ws = (const char *)args.w + wb;
     g.ws_bytes = (unsigned)(g.nkt * g.rows);
     if (args.res && args.out_dtype == YMX_BF16) {
         const long long rb = ((long long)(args.P - 1) * args.res_ld + args.Cout) * 2;
         g.a.res_bytes = rb < 0x80000000LL ? (unsigned)rb : 0u;
     }
+    if (raw) return args.out_dtype == YMX_BF16 ? launch_f8_cfg<bf16_t, 4, 1, 1, 2, 4, true>(g, s) : launch_f8_cfg<float, 4, 1, 1, 2, 4, true>(g, s);
     return args.out_dtype == YMX_BF16 ? launch_f8_shape<bf16_t>(g, s) : launch_f8_shape<float>(g, s);
 }
 

@@ -441,11 +441,18 @@ class YOLOConv(nn.Module):
         return self.compute_dtype or x.dtype
 
     def _forward_8bit(self, x, residual, out_dtype, out, act_code):
-        q = x if isinstance(x, BlockQuantized) else quantize_blocks(x)
-        b, h, w, cin = q.shape
+        b, h, w, cin = x.shape
         k, cout = self.kernel_size, self.filters
         oh, ow = self.output_hw(h, w)
         odt = out_dtype or torch.bfloat16
+        if isinstance(x, BlockQuantized):
+            q, code, x_ptr = x, _lib.F8E4M3, x.buffer.data_ptr()
+        elif (k == 1 and x.dtype == torch.bfloat16 and x.data_ptr() % 16 == 0 and x.numel() and
+              _lib.lib().ymx_conv2d_quantizes(b * oh * ow, cout, 1)):
+            q, code, x_ptr = x, _lib.BF16, x.data_ptr()          # few pixels: quantised by the layer's own kernel
+        else:
+            q = quantize_blocks(x)
+            code, x_ptr = _lib.F8E4M3, q.buffer.data_ptr()
         if q.device != self.kernel.device:
             raise ValueError("YOLOConv: input on %s, kernel on %s" % (q.device, self.kernel.device))
         wp, scale, shift, _ = self.packed(torch.float8_e4m3fn)
@@ -465,8 +472,8 @@ class YOLOConv(nn.Module):
             fused = fused.to(odt)
         if fused is not None and fused.data_ptr() % 16:
             fused = fused.clone()
-        _lib.launch("ymx_conv2d_fused_ex", q, _lib.ptr(q.buffer), _lib.ptr(wp), _lib.ptr(scale), _lib.ptr(shift), _lib.ptr(fused),
-                    _lib.ptr(y), b, h, w, cin, cout, k, 2 if self.downsample else 1, act_code, _lib.F8E4M3, _lib.F8E4M3,
+        _lib.launch("ymx_conv2d_fused_ex", q, x_ptr, wp.data_ptr(), _lib.ptr(scale), _lib.ptr(shift), _lib.ptr(fused),
+                    y.data_ptr(), b, h, w, cin, cout, k, 2 if self.downsample else 1, act_code, _lib.F8E4M3, code,
                     _lib.dtype_code(odt), 0, 0, y_ld)
         if self.act_fn is not None:
             y = self.act_fn(y)
