@@ -182,3 +182,21 @@ def launch(name, ref, *args):
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         check(rc)
+
+
+_native = None
+
+
+def native():
+    """yolo_amd._native, the operators whose host side is C++, bound to the loaded library's entry
+    points."""
+    global _native
+    if _native is None:
+        try:
+            from . import _native as module
+        except ImportError as e:
+            raise RuntimeError("yolo_amd: %s is missing or does not load (%s); build it with: make -C %s" %
+                               (os.path.join(_HERE, "_native.so"), e, os.path.join(_HERE, "csrc")))
+        module.init({name: ctypes.cast(getattr(lib(), name), _vp).value for name in module.ENTRY_POINTS})
+        _native = module
+    return _native

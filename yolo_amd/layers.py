@@ -442,39 +442,27 @@ class YOLOConv(nn.Module):
 
     def _forward_8bit(self, x, residual, out_dtype, out, act_code):
         b, h, w, cin = x.shape
-        k, cout = self.kernel_size, self.filters
         oh, ow = self.output_hw(h, w)
-        odt = out_dtype or torch.bfloat16
-        if isinstance(x, BlockQuantized):
-            q, code, x_ptr = x, _lib.F8E4M3, x.buffer.data_ptr()
-        elif (k == 1 and x.dtype == torch.bfloat16 and x.data_ptr() % 16 == 0 and x.numel() and
-              _lib.lib().ymx_conv2d_quantizes(b * oh * ow, cout, 1)):
-            q, code, x_ptr = x, _lib.BF16, x.data_ptr()          # few pixels: quantised by the layer's own kernel
-        else:
-            q = quantize_blocks(x)
-            code, x_ptr = _lib.F8E4M3, q.buffer.data_ptr()
-        if q.device != self.kernel.device:
-            raise ValueError("YOLOConv: input on %s, kernel on %s" % (q.device, self.kernel.device))
+        quantised = isinstance(x, BlockQuantized)
+        f32 = out_dtype is not None and out_dtype != torch.bfloat16
+        if f32:
+            _lib.dtype_code(out_dtype)
+        if not quantised:
+            _lib.dtype_code(x.dtype)
+        if b * h * w == 0:
+            raise ValueError("YOLOConv: expected a non-empty map, got shape %s" % (tuple(x.shape),))
+        if x.device != self.kernel.device:
+            raise ValueError("YOLOConv: input on %s, kernel on %s" % (x.device, self.kernel.device))
         wp, scale, shift, _ = self.packed(torch.float8_e4m3fn)
-        y_ld = 0
-        if out is not None:
-            y_ld = self._check_out(out, b, oh, ow, odt, q.device)
-        if out is not None and out.data_ptr() % 16 == 0:
-            y = out
-        else:
-            y, y_ld = torch.empty((b, oh, ow, cout), device=q.device, dtype=odt), 0
+        y_ld = self._check_out(out, b, oh, ow, torch.float32 if f32 else torch.bfloat16, x.device) if out is not None else 0
+        in_place = out is not None and out.data_ptr() % 16 == 0
         if residual is not None:
             residual = _as_nhwc(residual)
-            if residual.shape != y.shape or residual.device != y.device:
-                raise ValueError("YOLOConv: residual %s on %s != output %s on %s" % (tuple(residual.shape), residual.device, tuple(y.shape), y.device))
-        fused = residual if self.act_fn is None else None
-        if fused is not None and fused.dtype != odt:
-            fused = fused.to(odt)
-        if fused is not None and fused.data_ptr() % 16:
-            fused = fused.clone()
-        _lib.launch("ymx_conv2d_fused_ex", q, x_ptr, wp.data_ptr(), _lib.ptr(scale), _lib.ptr(shift), _lib.ptr(fused),
-                    y.data_ptr(), b, h, w, cin, cout, k, 2 if self.downsample else 1, act_code, _lib.F8E4M3, code,
-                    _lib.dtype_code(odt), 0, 0, y_ld)
+            if residual.shape != (b, oh, ow, self.filters) or residual.device != x.device:
+                raise ValueError("YOLOConv: residual %s on %s != output %s on %s" % (tuple(residual.shape), residual.device, (b, oh, ow, self.filters), x.device))
+        y = _lib.native().conv8(x.buffer if quantised else x, quantised, b, h, w, cin, wp, scale, shift, residual if self.act_fn is None else None,
+                                out if in_place else None, y_ld if in_place else 0, self.kernel_size, 2 if self.downsample else 1, oh, ow,
+                                self.filters, act_code, f32)
         if self.act_fn is not None:
             y = self.act_fn(y)
             if residual is not None:

@@ -516,83 +516,6 @@ def _check_shortcut(x, shortcut, who):
                                                                               tuple(x.shape), x.device))
 
 
-def _records(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def _dense(t, dtype):
-    """t as a contiguous tensor of dtype (itself where it is one)."""
-    if t.dtype != dtype:
-        t = t.to(dtype)
-    return t if t.is_contiguous() else t.contiguous()
-
-
-# The backward steps below are Python run by autograd's own thread, where every call costs about twice
-# what it does on the caller's: what can be decided in the forward pass is decided there.
-def _group_norm_forward(x, gamma, beta, shortcut, state, cfg, keep):
-    """(y, contiguous x, gamma and beta as the kernels take them, statistics if `keep`, the geometry of the launches)"""
-    groups, act, epsilon, rate = cfg
-    x = x if x.is_contiguous() else x.contiguous()
-    b, c = x.shape[0], x.shape[-1]
-    gamma, beta = _dense(gamma, torch.float32), _dense(beta, torch.float32)
-    sc = None if shortcut is None else _dense(shortcut, x.dtype)
-    y = torch.empty_like(x)
-    stats = torch.empty((b, groups, 2), device=x.device, dtype=torch.float32) if keep else None
-    geo = None
-    n = x.numel()
-    if n:
-        pix = n // (b * c)
-        nb = _lib.lib().ymx_group_norm_workspace_bytes(b, pix, c, groups)
-        geo = (b, pix, c, groups, act, _lib.dtype_code(x.dtype), rate, nb)
-        ws = torch.empty((nb,), device=x.device, dtype=torch.uint8)
-        _lib.launch("ymx_group_norm_forward", x, x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), _lib.ptr(sc), y.data_ptr(), _lib.ptr(stats),
-                    b, pix, c, groups, act, epsilon, geo[5], rate, _lib.ptr(state), ws.data_ptr(), nb)
-    return y, x, gamma, beta, stats, geo
-
-
-def _group_norm_backward(ctx, dy):
-    x, gamma, beta, stats, state = ctx.saved_tensors
-    need_x, need_g, need_b, need_s = ctx.needs_input_grad[:4]
-    dy = _dense(dy, x.dtype)
-    dx = dgamma = dbeta = None
-    if need_x or need_g or need_b:
-        dx = torch.empty_like(x)
-        dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(beta)
-        if ctx.geo is not None:
-            b, pix, c, groups, act, code, rate, nb = ctx.geo
-            ws = torch.empty((nb,), device=x.device, dtype=torch.uint8)
-            _lib.launch("ymx_group_norm_backward", x, x.data_ptr(), dy.data_ptr(), gamma.data_ptr(), beta.data_ptr(), stats.data_ptr(), dx.data_ptr(),
-                        dgamma.data_ptr(), dbeta.data_ptr(), b, pix, c, groups, act, code, rate, _lib.ptr(state), ws.data_ptr(), nb)
-        else:
-            dgamma.zero_()
-            dbeta.zero_()
-        if dgamma.dtype != ctx.dtypes[0]:
-            dgamma = dgamma.to(ctx.dtypes[0])
-        if dbeta.dtype != ctx.dtypes[1]:
-            dbeta = dbeta.to(ctx.dtypes[1])
-    dsc = None
-    if need_s:
-        dsc = dy if dy.dtype == ctx.dtypes[2] else dy.to(ctx.dtypes[2])
-    return dx if need_x else None, dgamma if need_g else None, dbeta if need_b else None, dsc, None, None
-
-
-_group_norm_backward_once = torch.autograd.function.once_differentiable(_group_norm_backward)
-
-
-class _GroupNormAct(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, gamma, beta, shortcut, state, cfg):
-        y, xc, ga, be, stats, ctx.geo = _group_norm_forward(x, gamma, beta, shortcut, state, cfg, True)
-        ctx.save_for_backward(xc, ga, be, stats, state)
-        ctx.dtypes = (gamma.dtype, beta.dtype, None if shortcut is None else shortcut.dtype)
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        # with create_graph=True the results carry an error for whoever differentiates them
-        return _group_norm_backward_once(ctx, dy) if torch.is_grad_enabled() else _group_norm_backward(ctx, dy)
-
-
 def group_norm_act(x, gamma, beta, groups, activation=None, shortcut=None, epsilon=1e-3, rate=0.0, state=None):
     """``dropout(act(gamma * (x - mean) / sqrt(var + epsilon) + beta)) + shortcut`` over x [B, ..., C] (a
     GPU tensor, bfloat16 or float32), the statistics of every (sample, group of C / groups
@@ -616,43 +539,7 @@ def group_norm_act(x, gamma, beta, groups, activation=None, shortcut=None, epsil
     _check_shortcut(x, shortcut, "group_norm_act")
     rate = _check_dropout(x, rate, state, "group_norm_act")
     state = state if rate > 0.0 else None
-    if _records(x, gamma, beta, shortcut):
-        return _GroupNormAct.apply(x, gamma, beta, shortcut, state, (groups, code, float(epsilon), rate))
-    with torch.no_grad():
-        return _group_norm_forward(x, gamma, beta, shortcut, state, (groups, code, float(epsilon), rate), False)[0]
-
-
-def _dropout_launch(x, shortcut, rate, state):
-    x = x if x.is_contiguous() else x.contiguous()
-    y = torch.empty_like(x)
-    sc = None if shortcut is None else _dense(shortcut, x.dtype)
-    _lib.launch("ymx_dropout", x, x.data_ptr(), _lib.ptr(sc), y.data_ptr(), x.numel(), _lib.dtype_code(x.dtype), rate, state.data_ptr())
-    return y
-
-
-def _dropout_backward(ctx, dy):
-    (state,) = ctx.saved_tensors
-    need_x, need_s = ctx.needs_input_grad[:2]
-    rate, x_dtype, shortcut_dtype = ctx.args
-    if dy.dtype != x_dtype:
-        dy = dy.to(x_dtype)
-    dx = _dropout_launch(dy, None, rate, state) if need_x else None
-    return dx, (dy if dy.dtype == shortcut_dtype else dy.to(shortcut_dtype)) if need_s else None, None, None
-
-
-_dropout_backward_once = torch.autograd.function.once_differentiable(_dropout_backward)
-
-
-class _DropoutFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, shortcut, rate, state):
-        ctx.save_for_backward(state)
-        ctx.args = (rate, x.dtype, None if shortcut is None else shortcut.dtype)
-        return _dropout_launch(x, shortcut, rate, state)
-
-    @staticmethod
-    def backward(ctx, dy):
-        return _dropout_backward_once(ctx, dy) if torch.is_grad_enabled() else _dropout_backward(ctx, dy)
+    return _lib.native().group_norm_act(x, gamma, beta, shortcut, state, groups, code, epsilon, rate)
 
 
 def dropout(x, rate, state, shortcut=None):
@@ -670,7 +557,4 @@ def dropout(x, rate, state, shortcut=None):
         return x if shortcut is None else x + shortcut.to(x.dtype)
     if x.numel() == 0:
         return x.clone()
-    if _records(x, shortcut):
-        return _DropoutFn.apply(x, shortcut, rate, state)
-    with torch.no_grad():
-        return _dropout_launch(x, shortcut, rate, state)
+    return _lib.native().dropout(x, shortcut, state, rate)
