@@ -123,7 +123,7 @@ int ymx_conv2d_fused_ex(const void *x, const void *w, const void *scale, const v
  * shift and act as above, y and residual have the type out_dtype (fp32 or bf16; both 0-dense or
  * with pixel strides), products are accumulated in fp32.  ymx_packed_weight_bytes gives the size.
  *
- * Layers for which ymx_conv2d_quantizes(output pixels, Cout, k) returns 1 also take x_dtype = YMX_BF16, a bf16 map with pixel
+ * Layers for which ymx_conv2d_quantizes(output pixels, Cout, k, out_dtype) returns 1 also take x_dtype = YMX_BF16, a bf16 map with pixel
  * stride x_ld, and quantise it themselves: the same result in one launch.
  *
  * Values are e4m3 numbers times 2^k, one k for each block of up to 128 input channels: of one
@@ -135,7 +135,7 @@ int ymx_conv2d_fused_ex(const void *x, const void *w, const void *scale, const v
  * bytes [n_pix][C], padding to a multiple of 256 bytes, then a plane of exponent bytes k + 127 for
  * each block of channels, [ceil(C / 128)][n_pix rounded up to 4], the padding zero.  x of
  * ymx_quantize_blocks is fp32 or bf16 with pixel stride x_ld (elements, a multiple of 8; 0 = dense). */
-int ymx_conv2d_quantizes(long long n_pix, int Cout, int k);
+int ymx_conv2d_quantizes(long long n_pix, int Cout, int k, int out_dtype);
 size_t ymx_quantized_bytes(long long n_pix, int C);
 int ymx_quantize_blocks(const void *x, void *q, long long n_pix, int C, int dtype, int x_ld, void *stream);
 

@@ -50,7 +50,8 @@ def test_plain_maps_are_for_small_1x1_layers():
 
     def conv(B=1, H=8, W=8, cin=32, cout=32, k=1, xd=_lib.BF16, x_ld=0, x=one):
         return L.ymx_conv2d_fused_ex(x, one, None, None, None, one, B, H, W, cin, cout, k, 1, 0, _lib.F8E4M3, xd, _lib.BF16, x_ld, 0, 0, None)
-    assert [L.ymx_conv2d_quantizes(n, c, k) for n, c, k in ((169, 512, 1), (11264, 64, 1), (11265, 64, 1), (169, 512, 3), (0, 64, 1), (1, 0, 1))] == [1, 1, 0, 0, 0, 0]
+    assert [L.ymx_conv2d_quantizes(n, c, k, _lib.BF16) for n, c, k in ((169, 512, 1), (11264, 64, 1), (11265, 64, 1), (169, 512, 3), (0, 64, 1), (1, 0, 1))] == [1, 1, 0, 0, 0, 0]
+    assert [L.ymx_conv2d_quantizes(n, 64, 1, _lib.F32) for n in (11265, 49152, 49153)] == [1, 1, 0]
     for call, text in ((lambda: conv(B=200), b"quantised map"), (lambda: conv(xd=_lib.F32), b"quantised map"), (lambda: conv(x_ld=36), b"stride"),
                        (lambda: conv(x_ld=24), b"stride"), (lambda: conv(x=ctypes.c_void_p(264)), b"aligned")):
         assert call() == -1 and text in L.ymx_last_error(), L.ymx_last_error()

@@ -242,14 +242,15 @@ def test_conv8_capture_needs_a_packed_kernel():
 
 @pytest.mark.parametrize("b,size,cin,cout,stride,out", [(1, 13, 1024, 512, 1, torch.bfloat16), (1, 13, 16, 40, 1, torch.bfloat16),
                                                         (3, 7, 144, 255, 1, torch.float32), (1, 1, 272, 64, 1, torch.bfloat16),
-                                                        (2, 23, 400, 72, 2, torch.bfloat16), (8, 13, 1024, 512, 1, torch.float32)])
+                                                        (2, 23, 400, 72, 2, torch.bfloat16), (8, 13, 1024, 512, 1, torch.float32),
+                                                        (8, 26, 1024, 255, 1, torch.float32), (3, 25, 80, 33, 2, torch.float32)])
 def test_conv8_quantises_small_maps_itself(b, size, cin, cout, stride, out):
     """A 1x1 layer of few pixels takes the plain map in one launch: the bits of quantisation and product one after the other,
     for blocks of any size, zeros, NaN and infinities, fp32 maps and maps that are not 16-byte aligned."""
     from yolo_amd import _lib
     from yolo_amd.layers import YOLOConv, quantize_blocks
     oh = size if stride == 1 else (size + 1 - 1) // 2 + 1
-    assert _lib.lib().ymx_conv2d_quantizes(b * oh * oh, cout, 1) == 1 and _lib.lib().ymx_conv2d_quantizes(b * oh * oh, cout, 3) == 0
+    assert [_lib.lib().ymx_conv2d_quantizes(b * oh * oh, cout, k, _lib.dtype_code(out)) for k in (1, 3)] == [1, 0]
     layer = YOLOConv((1, 1, cout), downsample=stride == 2, dtype=F8, in_channels=cin).to(DEV)
     g = torch.Generator().manual_seed(cin)
     x = torch.randn(b, size, size, cin, generator=g)

@@ -45,7 +45,7 @@ SIGNATURES = {
     "ymx_bn_act_forward": (_i, [_vp, _vp, _vp, _vp, _vp, _ll, _i, _i, _i, _vp]),
     "ymx_bn_act_backward": (_i, [_vp, _vp, _vp, _vp, _vp, _ll, _i, _i, _i, _vp, _vp, _sz, _vp]),
     "ymx_bn_backward_apply": (_i, [_vp] * 6 + [_ll, _i, _i, _vp]),
-    "ymx_conv2d_quantizes": (_i, [_ll, _i, _i]),
+    "ymx_conv2d_quantizes": (_i, [_ll, _i, _i, _i]),
     "ymx_quantized_bytes": (_sz, [_ll, _i]),
     "ymx_quantize_blocks": (_i, [_vp, _vp, _ll, _i, _i, _i, _vp]),
     "ymx_group_norm_workspace_bytes": (_sz, [_ll, _ll, _i, _i]),

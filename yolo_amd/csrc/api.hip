@@ -141,7 +141,7 @@ static int conv_impl(const void *x, const void *w, const void *scale, const void
         // x is a quantised map (ymx_quantize_blocks), the residual has the output's type
         const bool raw = x_dtype == YMX_BF16;
         if (!raw && x_dtype != YMX_F8E4M3) return fail(YMX_EARG, "conv2d: an 8-bit kernel takes a quantised map");
-        if (raw && !conv_f8_raw(a.P, Cout, k)) return fail(YMX_EARG, "conv2d: an 8-bit kernel of this size takes a quantised map");
+        if (raw && !conv_f8_raw(a.P, Cout, k, out_dtype)) return fail(YMX_EARG, "conv2d: an 8-bit kernel of this size takes a quantised map");
         if (out_dtype != YMX_F32 && out_dtype != YMX_BF16) return fail(YMX_EARG, "conv2d: output dtype %d", out_dtype);
         if (z || d2s) return fail(YMX_EUNSUPPORTED, "conv2d: 8-bit kernels are for inference");
         if (Cin % 16 || (k != 1 && k != 3)) return fail(YMX_EUNSUPPORTED, "conv2d: 8-bit kernels take input channels in multiples of 16 and 1x1 or 3x3 windows (%d, %d)", Cin, k);
@@ -312,7 +312,7 @@ int ymx_pack_weights(const float *w_hwio, void *w_packed, int k, int Cin, int Co
     return launch_pack_weights(w_hwio, w_packed, k, Cin, Cout, dtype, (hipStream_t)stream);
 }
 
-int ymx_conv2d_quantizes(long long n_pix, int Cout, int k) { return n_pix > 0 && Cout > 0 && conv_f8_raw(n_pix, Cout, k); }
+int ymx_conv2d_quantizes(long long n_pix, int Cout, int k, int out_dtype) { return n_pix > 0 && Cout > 0 && conv_f8_raw(n_pix, Cout, k, out_dtype); }
 
 size_t ymx_quantized_bytes(long long n_pix, int C) { return (n_pix > 0 && C > 0) ? quant_bytes(n_pix, C) : 0; }
 

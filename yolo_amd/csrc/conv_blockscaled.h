@@ -44,19 +44,22 @@ __device__ __forceinline__ f32x4_t f8_mfma(const i32x8_t &w, const i32x8_t &x, c
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 0, 0, 0, ws, 0, xs);
 }
 
-// A fragment's 32 values times 2^(exponent byte - 127) as bf16: eight at a time, in the order they lie in.  Exact down to
-// 2^-126, bf16 having e4m3's digits and fp32's exponents.
-__device__ __forceinline__ void f8_to_bf16(const i32x8_t &v, int exponent, bf16x8_t (&o)[4]) {
+// Two words of e4m3 numbers times 2^(exponent byte - 127) as eight bf16 ones.  Exact down to 2^-126, bf16 having e4m3's
+// digits and fp32's exponents.
+__device__ __forceinline__ void f8_words_to_bf16(uint32_t a, uint32_t b, int exponent, uint4 &o) {
     const float f = __uint_as_float((uint32_t)exponent << 23);
+    o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, f, false));
+    o.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, f, true));
+    o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, f, false));
+    o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, f, true));
+}
+// A fragment's 32 values, eight at a time, in the order they lie in.
+__device__ __forceinline__ void f8_to_bf16(const i32x8_t &v, int exponent, bf16x8_t (&o)[4]) {
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            w[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)v[2 * h + i], f, false));
-            w[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)v[2 * h + i], f, true));
-        }
-        o[h] = __builtin_bit_cast(bf16x8_t, uint4{w[0], w[1], w[2], w[3]});
+        uint4 w;
+        f8_words_to_bf16((uint32_t)v[2 * h], (uint32_t)v[2 * h + 1], exponent, w);
+        o[h] = __builtin_bit_cast(bf16x8_t, w);
     }
 }
 

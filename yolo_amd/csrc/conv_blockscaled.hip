@@ -208,8 +208,9 @@ __device__ __forceinline__ uint4 f8_quantize16(uint32_t (&w)[8], int &e) {
 // for pixels and channels alike (the order inside a block does not matter: one exponent covers it).
 //
 // RAW: x is a bf16 map, staged as such (256 bytes per pixel and K tile, chunk c of row r in slot c ^ (r & 15)).  While
-// tile kt is multiplied, the threads quantise tile kt + 1, 16 channels each, into one of two further row buffers.
-template <bool RAW, int NWQ, int NWP, int NI, int NJ, int NSTAGE> struct F8Tile {
+// tile kt is multiplied, the threads quantise tile kt + 1, 16 channels each, into one of two further row buffers (32-bit
+// outputs: in place, as the bf16 numbers that their products take).
+template <bool RAW, typename OT, int NWQ, int NWP, int NI, int NJ, int NSTAGE> struct F8Tile {
     static constexpr int NW = NWQ * NWP, TQ = NWQ * NI * 16, TP = NWP * NJ * 16;
     static constexpr int XROW = RAW ? 256 : 128, XPER = 1024 / XROW;                // bytes of a pixel, pixels per instruction
     static constexpr int NXI = TP / XPER / NW, NWI = TQ / 8 / NW;                       // DMA instructions per wave: rows ...
@@ -217,16 +218,16 @@ template <bool RAW, int NWQ, int NWP, int NI, int NJ, int NSTAGE> struct F8Tile 
     static constexpr int NSI = (NS + NW - 1) / NW;                                   // (per wave)
     static constexpr int XB = TP * XROW, WB = TQ * 128, STAGE = XB + WB + NS * 256, PIECES = NXI + NWI + NSI;
     static constexpr int EPI = NW * EpiGeom<NI, 64, 16 * NJ>::LDS_BYTES;
-    static constexpr int XQ = RAW ? TP * 132 : 0, USED = NSTAGE * STAGE + 2 * XQ, LDS = USED > EPI ? USED : EPI;     // (rows and exponents)
+    static constexpr int XQ = RAW && sizeof(OT) == 2 ? TP * 132 : 0, USED = NSTAGE * STAGE + 2 * XQ, LDS = USED > EPI ? USED : EPI;     // (rows and exponents)
     static constexpr int AHEAD = NSTAGE - (RAW ? 3 : 2);                             // K tiles in flight behind the one waited for
     static_assert(TP % (XPER * NW) == 0 && TQ % (8 * NW) == 0, "whole instructions per wave");
 };
 template <bool RAW, typename OT, int NWQ, int NWP, int NI, int NJ, int NSTAGE>
 __global__ void __launch_bounds__(64 * NWQ * NWP, 2)
 conv_f8_kernel(const F8Args g, const int ntile_q) {
-    typedef F8Tile<RAW, NWQ, NWP, NI, NJ, NSTAGE> C;
+    typedef F8Tile<RAW, OT, NWQ, NWP, NI, NJ, NSTAGE> C;
     constexpr int NXI = C::NXI, NWI = C::NWI, NSI = C::NSI, SX = C::SX, XB = C::XB, WB = C::WB, STAGE = C::STAGE;
-    constexpr bool EXACT = sizeof(OT) == 4;
+    constexpr bool EXACT = sizeof(OT) == 4, ROUNDED = RAW && EXACT;
     constexpr unsigned OOB = 0x80000000u;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const ConvArgs &a = g.a;
@@ -309,7 +310,7 @@ conv_f8_kernel(const F8Args g, const int ntile_q) {
 
     const int frow = lane & 15, q = lane >> 4;
     const int s0 = (q ^ (frow & 7)) << 4, s1 = ((q + 4) ^ (frow & 7)) << 4;
-    const int a_off = XB + (wq * NI * 16 + frow) * 128, b_off = (wp * NJ * 16 + frow) * 128;
+    const int a_off = XB + (wq * NI * 16 + frow) * 128, b_off = (wp * NJ * 16 + frow) * (ROUNDED ? 256 : 128);
     const int as_off = XB + WB + (SX * 64 + wq * NI * 16 + frow) * 4, bs_off = (RAW ? C::TP * 128 : XB + WB) + (wp * NJ * 16 + frow) * 4;
 
     auto frag = [&](const char *p) { return f8_frag(*(const int4 *)(p + s0), *(const int4 *)(p + s1)); };
@@ -317,6 +318,7 @@ conv_f8_kernel(const F8Args g, const int ntile_q) {
     // which then runs under the reads' latency.
     constexpr int PRE = NI <= 2 ? NI : 1;
     i32x8_t b[NJ], w[PRE];
+    bf16x8_t bb[EXACT ? NJ : 1][4];                              // 32-bit outputs: the same fragments, scaled, as bf16
     int bs[NJ], ws[PRE];
     auto load_w = [&](const char *base, int i, i32x8_t &f, int &e) {
         f = frag(base + a_off + i * 2048);
@@ -325,29 +327,40 @@ conv_f8_kernel(const F8Args g, const int ntile_q) {
     auto load = [&](const char *base, const char *xbase) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            b[j] = frag(xbase + b_off + j * 2048);
-            bs[j] = *(const int *)(xbase + bs_off + j * 64);
+            if constexpr (ROUNDED) {
+#pragma unroll
+                for (int h = 0; h < 4; ++h) bb[j][h] = *(const bf16x8_t *)(xbase + b_off + j * 4096 + (((2 * q + (h & 1) + (h & 2) * 4) ^ frow) << 4));
+            } else {
+                b[j] = frag(xbase + b_off + j * 2048);
+                bs[j] = *(const int *)(xbase + bs_off + j * 64);
+            }
         }
 #pragma unroll
         for (int i = 0; i < PRE; ++i) load_w(base, i, w[i], ws[i]);
     };
-    // RAW: tile kt's pixels t / 8, t / 8 + 8 NW, ...: 16 channels a thread
+    // RAW: tile kt's pixels t / 8, t / 8 + 8 NW, ...: 16 channels a thread.  For 32-bit outputs the values go back as scaled bf16
+    // numbers to where they were, once for all waves.
     char *xq = smem + NSTAGE * STAGE;
-    auto quantize = [&](const char *base, char *to) {
+    auto quantize = [&](char *base, char *to) {
 #pragma unroll
         for (int n = 0; n < C::TP / (8 * C::NW); ++n) {
             const int row = n * 8 * C::NW + (t >> 3), part = t & 7;
-            const uint4 lo = *(const uint4 *)(base + row * 256 + (((2 * part) ^ (row & 15)) << 4));
-            const uint4 hi = *(const uint4 *)(base + row * 256 + (((2 * part + 1) ^ (row & 15)) << 4));
-            uint32_t v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+            uint4 *lo = (uint4 *)(base + row * 256 + (((2 * part) ^ (row & 15)) << 4)), *hi = (uint4 *)(base + row * 256 + (((2 * part + 1) ^ (row & 15)) << 4));
+            const uint4 l = *lo, h = *hi;
+            uint32_t v[8] = {l.x, l.y, l.z, l.w, h.x, h.y, h.z, h.w};
             int e;
-            *(uint4 *)(to + row * 128 + ((part ^ (row & 7)) << 4)) = f8_quantize16(v, e);
-            if (part == 0) *(int *)(to + C::TP * 128 + row * 4) = e;
+            const uint4 o = f8_quantize16(v, e);
+            if constexpr (ROUNDED) {
+                f8_words_to_bf16(o.x, o.y, e, *lo);
+                f8_words_to_bf16(o.z, o.w, e, *hi);
+            } else {
+                *(uint4 *)(to + row * 128 + ((part ^ (row & 7)) << 4)) = o;
+                if (part == 0) *(int *)(to + C::TP * 128 + row * 4) = e;
+            }
         }
     };
     auto compute = [&](const char *base) {
-        bf16x8_t bb[EXACT ? NJ : 1][4];                          // 32-bit outputs: the same fragments, scaled, as bf16
-        if constexpr (EXACT)
+        if constexpr (EXACT && !RAW)
 #pragma unroll
             for (int j = 0; j < NJ; ++j) f8_to_bf16(b[j], bs[j], bb[j]);
 #pragma unroll
@@ -385,9 +398,9 @@ conv_f8_kernel(const F8Args g, const int ntile_q) {
     }
     int st = 0;
     for (int kt = 0; kt < g.nkt; ++kt) {
-        const char *base = smem + st * STAGE;
+        char *base = smem + st * STAGE;
         const int next = st + 1 == NSTAGE ? 0 : st + 1;
-        load(base, RAW ? xq + (kt & 1) * C::XQ : base);
+        load(base, RAW && !ROUNDED ? xq + (kt & 1) * C::XQ : base);
         dma(st == 0 ? NSTAGE - 1 : st - 1);
         if constexpr (RAW) quantize(smem + next * STAGE, xq + (kt + 1 & 1) * C::XQ);
         compute(base);
@@ -401,7 +414,7 @@ conv_f8_kernel(const F8Args g, const int ntile_q) {
 }
 
 template <typename OT, int NWQ, int NWP, int NI, int NJ, int NSTAGE, bool RAW = false> static int launch_f8_cfg(const F8Args &g, hipStream_t s) {
-    typedef F8Tile<RAW, NWQ, NWP, NI, NJ, NSTAGE> C;
+    typedef F8Tile<RAW, OT, NWQ, NWP, NI, NJ, NSTAGE> C;
     auto kern = conv_f8_kernel<RAW, OT, NWQ, NWP, NI, NJ, NSTAGE>;
     static LdsReserve reserved;
     if (const int rc = reserve_lds(reserved, (const void *)kern, C::LDS, "conv_f8")) return rc;
@@ -435,10 +448,13 @@ template <typename OT> static int launch_f8_shape(const F8Args &g, hipStream_t s
 }
 
 // Whether a layer on a bf16 map quantises it in its own kernel, in tiles of 64 x 32.  Every tile of channels and every tap
-// quantises its pixels again, so where there are few of them: 1x1 windows, up to 176 tiles of 64 x 64.  Measured (us, one
-// launch against two): 13^2 1024 -> 512 11.3, 12.3; 26^2 256 -> 512 8.7, 10.7; 52^2 256 -> 255 to fp32 10.0, 11.9; 8 x 13^2 1024 ->
-// 512 (176 tiles) 13.9, 13.8; 8 x 13^2 1024 -> 1024 (352) 20.4, 15.2; 3x3: 13^2 512 -> 1024 25.8, 20.2.  And 6 us less on the host.
-bool conv_f8_raw(long long P, int Cout, int k) { return k == 1 && (P + 63) / 64 * ((Cout + 63) / 64) <= 176; }
+// quantises its pixels again, so where there are few of them: 1x1 windows, up to 176 tiles of 64 x 64; up to 768 for 32-bit
+// outputs, which save the waves' own conversions.  Measured (us, one launch against two): 13^2 1024 -> 512 11.8, 12.4; 26^2 256 ->
+// 512 8.5, 10.9; 8 x 13^2 1024 -> 512 (176 tiles) 13.2, 13.6; 8 x 13^2 1024 -> 1024 (352) 19.7, 15.0; to fp32: 8 x 26^2 1024 -> 255
+// 17.5, 21.4; 64 x 13^2 1024 -> 255 (676) 30.1, 33.2; 8 x 52^2 256 -> 255 (1352) 27.8, 26.1; 3x3: 13^2 512 -> 1024 25.8, 20.2.
+bool conv_f8_raw(long long P, int Cout, int k, int out_dtype) {
+    return k == 1 && (P + 63) / 64 * ((Cout + 63) / 64) <= (out_dtype == YMX_F32 ? 768 : 176);
+}
 
 // a: geometry of the convolution with x_ld = Cin; x = quantised map, or a bf16 one
 // where conv_f8_raw says so; w = packed kernel.
@@ -466,7 +482,7 @@ int launch_conv_f8(const ConvArgs &args, long long in_pix, hipStream_t s) {
         const long long rb = ((long long)(args.P - 1) * args.res_ld + args.Cout) * 2;
         g.a.res_bytes = rb < 0x80000000LL ? (unsigned)rb : 0u;
     }
-    if (raw) return args.out_dtype == YMX_BF16 ? launch_f8_cfg<bf16_t, 4, 1, 1, 2, 4, true>(g, s) : launch_f8_cfg<float, 4, 1, 1, 2, 4, true>(g, s);
+    if (raw) return args.out_dtype == YMX_BF16 ? launch_f8_cfg<bf16_t, 4, 1, 1, 2, 3, true>(g, s) : launch_f8_cfg<float, 4, 1, 1, 2, 3, true>(g, s);
     return args.out_dtype == YMX_BF16 ? launch_f8_shape<bf16_t>(g, s) : launch_f8_shape<float>(g, s);
 }
 

@@ -199,7 +199,7 @@ Tensor conv8(const Tensor &t, bool quantised, int64_t B, int64_t H, int64_t W, i
     int x_type = YMX_F8E4M3;
     if (!quantised) {
         x = aligned(t.contiguous());
-        if (x.scalar_type() == at::kBFloat16 && api.ymx_conv2d_quantizes(B * oh * ow, (int)cout, (int)k)) {
+        if (x.scalar_type() == at::kBFloat16 && api.ymx_conv2d_quantizes(B * oh * ow, (int)cout, (int)k, fp32 ? YMX_F32 : YMX_BF16)) {
             x_type = YMX_BF16;                                   // few pixels: by the layer's own kernel
         } else {
             const Tensor q = workspace(api.ymx_quantized_bytes(B * H * W, (int)cin), x);
