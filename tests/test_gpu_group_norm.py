@@ -477,6 +477,39 @@ def test_training_step_in_a_graph():
         torch.ones(1000, device=DEV).sum().item()                    # eager work between the replays
 
 
+def test_gradients_share_no_memory():
+    """backward() into leaves, the shortcut among them: no .grad lies in the caller's dy or in another one, and a second
+    backward() over the kept graph adds the same again."""
+    from yolo_amd import training as T
+    for use in (lambda x, s: T.group_norm_act(x, ga, be, 4, "mish", s), lambda x, s: T.dropout(x, 0.25, torch.tensor([1, 2], device=DEV), s)):
+        ga, be = torch.ones(32, device=DEV, requires_grad=True), torch.zeros(32, device=DEV, requires_grad=True)
+        x, s = (torch.randn(2, 5, 5, 32, device=DEV).requires_grad_() for _ in range(2))
+        dy = torch.randn(2, 5, 5, 32, device=DEV)
+        kept = dy.clone()
+        y = use(x, s)
+        y.backward(dy, retain_graph=True)
+        assert len({t.data_ptr() for t in (dy, x.grad, s.grad, x, s, y)}) == 6 and torch.equal(s.grad, dy)
+        first = x.grad.clone()
+        s.grad.mul_(3.0)
+        assert torch.equal(dy, kept)
+        y.backward(dy)
+        assert torch.equal(x.grad, first + first) and torch.equal(s.grad, 3.0 * kept + kept)
+        with pytest.raises(RuntimeError, match="second time"):
+            y.backward(dy)
+
+
+def test_a_changed_state_is_noticed():
+    """The backward pass computes the mask from the state again: autograd refuses one that was written to in between."""
+    from yolo_amd import training as T
+    x = torch.randn(2, 4, 4, 32, device=DEV, requires_grad=True)
+    ga, be = torch.ones(32, device=DEV), torch.zeros(32, device=DEV)
+    state = torch.tensor([1, 2], device=DEV)
+    for y in (T.group_norm_act(x, ga, be, 4, None, rate=0.5, state=state), T.dropout(x, 0.5, state)):
+        state.add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+
+
 def test_second_derivatives_are_refused():
     from yolo_amd import training as T
     x = torch.randn(2, 4, 4, 32, device=DEV, requires_grad=True)

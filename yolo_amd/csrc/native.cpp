@@ -51,8 +51,8 @@ Tensor empty_as(const Tensor &t) { return at::empty(t.sizes(), t.options()); }
 Tensor workspace(size_t bytes, const Tensor &like) { return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)); }
 
 // The gradients of a step that is itself being recorded (create_graph=True): an error for whoever differentiates them.
-variable_list once(variable_list grads) {
-    if (!at::GradMode::is_enabled()) return grads;
+variable_list once(bool recorded, variable_list grads) {
+    if (!recorded) return grads;
     variable_list in;
     for (const Tensor &g : grads)
         if (g.defined()) in.push_back(g.detach().set_requires_grad(true));
@@ -113,14 +113,17 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
         ctx->saved_data["rate"] = rate;
         return o.y;
     }
+    // (The gradient of the shortcut is dy itself, not an alias of it: whoever accumulates it sees who else holds it.)
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        const bool recorded = at::GradMode::is_enabled();
+        const at::AutoGradMode off(false);
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &gamma = saved[1], &beta = saved[2], &stats = saved[3], &state = saved[4];
         const std::vector<int64_t> c = ctx->saved_data["call"].toIntVector();
         const bool need_x = ctx->needs_input_grad(0), need_g = ctx->needs_input_grad(1), need_b = ctx->needs_input_grad(2);
         const bool need_s = c[9] >= 0 && ctx->needs_input_grad(3);
         variable_list out(9);
-        const Tensor dy = dense(grads[0].detach(), x.scalar_type());
+        const Tensor dy = dense(grads[0], x.scalar_type());
         if (need_x || need_g || need_b) {
             Tensor dx = empty_as(x), dgamma = empty_as(gamma), dbeta = empty_as(beta);
             if (c[1] > 0) {
@@ -138,8 +141,8 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
             if (need_g) out[1] = cast(dgamma, (at::ScalarType)c[7]);
             if (need_b) out[2] = cast(dbeta, (at::ScalarType)c[8]);
         }
-        if (need_s) out[3] = cast(dy, (at::ScalarType)c[9]);
-        return once(std::move(out));
+        if (need_s) out[3] = cast(grads[0], (at::ScalarType)c[9]);
+        return once(recorded, std::move(out));
     }
 };
 
@@ -167,13 +170,14 @@ struct Dropout : torch::autograd::Function<Dropout> {
         return dropout_run(x, shortcut, state, rate);
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        const bool recorded = at::GradMode::is_enabled();
+        const at::AutoGradMode off(false);
         const variable_list saved = ctx->get_saved_variables();
         const std::vector<int64_t> types = ctx->saved_data["types"].toIntVector();
-        const Tensor dy = cast(grads[0].detach(), (at::ScalarType)types[0]);
         variable_list out(4);
-        if (ctx->needs_input_grad(0)) out[0] = dropout_run(dy, std::nullopt, saved[0], ctx->saved_data["rate"].toDouble());
-        if (types[1] >= 0 && ctx->needs_input_grad(1)) out[1] = cast(dy, (at::ScalarType)types[1]);
-        return once(std::move(out));
+        if (ctx->needs_input_grad(0)) out[0] = dropout_run(cast(grads[0], (at::ScalarType)types[0]), std::nullopt, saved[0], ctx->saved_data["rate"].toDouble());
+        if (types[1] >= 0 && ctx->needs_input_grad(1)) out[1] = cast(grads[0], (at::ScalarType)types[1]);
+        return once(recorded, std::move(out));
     }
 };
 
