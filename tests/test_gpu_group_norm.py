@@ -68,6 +68,11 @@ CASES = [   # shape, groups, activation, shortcut, rate, type
     ((1, 4, 4, 6168), 8, "leaky", True, 0.0, "bf16"),           # 771 channels a group: no whole vectors
     ((1, 5, 5, 2400), 300, "mish", False, 0.1, "bf16"),         # more than 256 groups
     ((1, 77, 77, 1024), 1, "mish", True, 0.0, "bf16"),          # one wide group over many chunks
+    ((2, 40, 41, 260), 13, "mish", True, 0.1, "bf16"),          # vectors of four
+    ((3, 9, 11, 68), 17, "leaky", False, 0.3, "bf16"),
+    ((2, 21, 20, 2052), 27, None, True, 0.0, "bf16"),           # ... in several blocks
+    ((1, 30, 30, 1028), 1, "mish", True, 0.1, "bf16"),          # ... a group in parts of them
+    ((5, 33, 31, 129), 43, "mish", True, 0.4, "f32"),           # single elements with dropout over several chunks
 ]
 
 

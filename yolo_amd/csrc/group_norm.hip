@@ -266,9 +266,24 @@ template <int V> struct GnChannels {
     __device__ __forceinline__ float t(int i, float x) const { return __builtin_fmaf(x - mean[i], ta[i], be[i]); }
 };
 
+// Single elements (V = 1) would compute four random words each for one: their bits come from a pass of its own over the flat
+// map, byte j those of elements 8 j ... 8 j + 7 (16 x 52^2 x 255, rate 0.1: forward/backward 36.4/44.7 us, 50.6/77.5 without).
+__global__ void __launch_bounds__(256) gn_mask_kernel(const DropArgs drop, unsigned long long n, unsigned char *__restrict__ mask) {
+    const unsigned long long j = (unsigned long long)blockIdx.x * 256 + threadIdx.x;
+    if (j * 8 >= n) return;
+    bool keep[8];
+    drop_keep<8>(drop, uint4{drop.state[0], drop.state[1], drop.state[2], drop.state[3]}, j * 8, keep);
+    unsigned m = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m |= keep[i] ? 1u << i : 0u;
+    mask[j] = (unsigned char)m;
+}
+__device__ __forceinline__ unsigned gn_mask_bit(const unsigned char *mask, size_t i) { return mask[i >> 3] >> (i & 7) & 1u; }
+
 // Pass 2, forward.
 template <typename T, int V, int ACT, bool DROP>
-__global__ void __launch_bounds__(256) gn_apply_kernel(const GnArgs a, const GnWork w, const float2 *__restrict__ part) {
+__global__ void __launch_bounds__(256) gn_apply_kernel(const GnArgs a, const GnWork w, const float2 *__restrict__ part,
+                                                       const unsigned char *__restrict__ mask) {
     extern __shared__ __attribute__((aligned(16))) float2 joined[];      // [G], then 256 of scratch
     const GnPos<V> g(a, w);
     gn_join<false, V>(a, w, g.b, g.chunk == 0 && g.cb == 0, part, joined, joined + a.G);
@@ -282,11 +297,12 @@ __global__ void __launch_bounds__(256) gn_apply_kernel(const GnArgs a, const GnW
     const bool has_res = a.res != nullptr;
     const DropArgs drop = {a.state, a.threshold, a.keep_scale};
     uint4 key = {};
-    if constexpr (DROP) key = uint4{a.state[0], a.state[1], a.state[2], a.state[3]};
-    struct Row { typename IO::raw x, s; };
-    gn_rows<2>(g.p, g.p1, w.R, [&](int p) {
+    if constexpr (DROP && V > 1) key = uint4{a.state[0], a.state[1], a.state[2], a.state[3]};
+    struct Row { typename IO::raw x, s; unsigned keep; };
+    gn_rows<V == 1 ? 4 : 2>(g.p, g.p1, w.R, [&](int p) {
                    Row q;
                    q.x = IO::load(x + (size_t)p * a.C);
+                   if constexpr (DROP && V == 1) q.keep = gn_mask_bit(mask, base + (size_t)p * a.C);
                    if (has_res) q.s = IO::load(res + (size_t)p * a.C);
                    return q;
                },
@@ -294,7 +310,8 @@ __global__ void __launch_bounds__(256) gn_apply_kernel(const GnArgs a, const GnW
                    float v[V], s[V];
                    bool keep[V];
                    IO::unpack(q.x, v);
-                   if constexpr (DROP) drop_keep<V>(drop, key, base + (size_t)p * a.C, keep);
+                   if constexpr (DROP && V == 1) keep[0] = q.keep;
+                   else if constexpr (DROP) drop_keep<V>(drop, key, base + (size_t)p * a.C, keep);
 #pragma unroll
                    for (int i = 0; i < V; ++i) {
                        v[i] = act_c<ACT>(ch.t(i, v[i]));
@@ -363,17 +380,22 @@ __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const GnArgs a, const 
         float s1[V], s2[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.0f;
-        struct Row { typename IO::raw x, d; };
-        gn_rows<4>(g.p, g.p1, w.R, [&](int p) { return Row{IO::load(x + (size_t)p * a.C), IO::load(dy + (size_t)p * a.C)}; },
+        struct Row { typename IO::raw x, d; unsigned keep; };
+        gn_rows<4>(g.p, g.p1, w.R, [&](int p) {
+                       Row q = {IO::load(x + (size_t)p * a.C), IO::load(dy + (size_t)p * a.C), 0u};
+                       if constexpr (DROP && V == 1) q.keep = gn_mask_bit(mask, base + (size_t)p * a.C);
+                       return q;
+                   },
                    [&](int p, const Row &q) {
                        float v[V], d[V], dt[V];
                        IO::unpack(q.x, v);
                        IO::unpack(q.d, d);
                        unsigned keep = 0u;
-                       if constexpr (DROP) {
+                       if constexpr (DROP && V == 1) keep = q.keep;
+                       else if constexpr (DROP) {
                            const size_t at = base + (size_t)p * a.C;
                            keep = gn_keep_bits<V>(drop, key, at);
-                           if constexpr (V > 1) mask[at / V] = (unsigned char)keep;
+                           mask[at / V] = (unsigned char)keep;
                        }
                        gn_dt<V, ACT, DROP>(ch, drop.keep_scale, keep, v, d, dt);
 #pragma unroll
@@ -469,22 +491,18 @@ __global__ void __launch_bounds__(256) gn_bwd_apply_kernel(const GnArgs a, const
     const size_t base = (size_t)g.b * a.P * a.C + g.c0;
     const T *__restrict__ x = (const T *)a.x + base, *__restrict__ dy = (const T *)a.dy + base;
     T *__restrict__ dx = (T *)a.dx + base;
-    const DropArgs drop = {a.state, a.threshold, a.keep_scale};
-    uint4 key = {};
-    if constexpr (DROP && V == 1) key = uint4{a.state[0], a.state[1], a.state[2], a.state[3]};
     struct Row { typename IO::raw x, d; unsigned keep; };
     gn_rows<4>(g.p, g.p1, w.R, [&](int p) {
                    Row q = {IO::load(x + (size_t)p * a.C), IO::load(dy + (size_t)p * a.C), 0u};
-                   if constexpr (DROP && V > 1) q.keep = mask[(base + (size_t)p * a.C) / V];
+                   if constexpr (DROP && V == 1) q.keep = gn_mask_bit(mask, base + (size_t)p * a.C);
+                   else if constexpr (DROP) q.keep = mask[(base + (size_t)p * a.C) / V];
                    return q;
                },
                [&](int p, const Row &q) {
                    float v[V], d[V], dt[V];
                    IO::unpack(q.x, v);
                    IO::unpack(q.d, d);
-                   unsigned keep = q.keep;
-                   if constexpr (DROP && V == 1) keep = gn_keep_bits<V>(drop, key, base + (size_t)p * a.C);
-                   gn_dt<V, ACT, DROP>(ch, drop.keep_scale, keep, v, d, dt);
+                   gn_dt<V, ACT, DROP>(ch, a.keep_scale, q.keep, v, d, dt);
 #pragma unroll
                    for (int i = 0; i < V; ++i) v[i] = gr.dx(ch, i, v[i], dt[i]);
                    IO::store(dx + (size_t)p * a.C, v);
@@ -717,11 +735,20 @@ template <int V> static GnWork gn_work(const GnArgs &a) {
     w.nchunk = (a.P + w.per - 1) / w.per;
     return w;
 }
-// Pairs: one per (chunk, channel) and one per (chunk, group or part of one).  Behind them the backward pass's bytes of kept
-// elements, one for four or eight.
+// Pairs: one per (chunk, channel) and one per (chunk, group or part of one).  Behind them the bytes of kept elements, one for
+// four or eight.
 static size_t gn_pairs(int G, int C) { return (size_t)G * ((C / G + 255) / 256); }
+static size_t gn_pair_bytes(int B, int P, int C, int G) { return (size_t)B * gn_chunks(B, P, C) * (C + gn_pairs(G, C)) * sizeof(float2); }
 size_t group_norm_workspace_bytes(int B, int P, int C, int G) {
-    return (size_t)B * gn_chunks(B, P, C) * (C + gn_pairs(G, C)) * sizeof(float2) + (size_t)B * P * C / 4;
+    return gn_pair_bytes(B, P, C, G) + (size_t)B * P * C / 4 + 8;
+}
+template <int V> static unsigned char *gn_mask(const GnArgs &a, void *ws, hipStream_t s) {
+    unsigned char *mask = (unsigned char *)ws + gn_pair_bytes(a.B, a.P, a.C, a.G);
+    if (V == 1 && a.state) {
+        const unsigned long long n = (unsigned long long)a.B * a.P * a.C;
+        hipLaunchKernelGGL(gn_mask_kernel, dim3((unsigned)((n + 2047) / 2048)), dim3(256), 0, s, DropArgs{a.state, a.threshold, a.keep_scale}, n, mask);
+    }
+    return mask;
 }
 
 // The one-pass form's slabs, or sv = 0 where the chunked form runs: groups of a power of two of at most 64
@@ -753,16 +780,21 @@ template <int V, typename F> static void gn_pick_act(const GnArgs &a, F f) {
     else if (a.act == YMX_ACT_LEAKY) drop(std::integral_constant<int, YMX_ACT_LEAKY>{});
     else drop(std::integral_constant<int, YMX_ACT_NONE>{});
 }
-// 16-byte vectors where the channel count and every map's address allow them and blocks of whole groups, or parts of
-// a group, are whole vectors; else one element at a time.
-template <typename T, typename F> static void gn_pick(const GnArgs &a, F f) {
-    constexpr int V = 16 / sizeof(T);
-    auto ok = [](const void *p) { return p == nullptr || aligned16(p); };
+// Vectors of V elements where the channel count and every map's address allow them and blocks of whole groups, or parts of
+// a group, are whole vectors: 16 bytes, else 8 of bf16 (16 x 52^2 x 260 forward/backward 24.8/35.2 us, in single elements
+// 35.9/50.8), else one element at a time.
+template <int V, typename T> static bool gn_vectors(const GnArgs &a) {
+    auto ok = [](const void *p) { return ((uintptr_t)p & (V * sizeof(T) - 1)) == 0; };
     int unit = a.D;
     for (int v = V; v > 1 && unit % 2 == 0; v /= 2) unit /= 2;   // vectors in the least run of whole groups
     const bool blocks = a.C <= 256 * V || unit <= 256 || a.D % V == 0;
-    if (a.C % V == 0 && blocks && ok(a.x) && ok(a.res) && ok(a.dy) && ok(a.y) && ok(a.dx)) gn_pick_act<V>(a, f);
-    else gn_pick_act<1>(a, f);
+    return a.C % V == 0 && blocks && ok(a.x) && ok(a.res) && ok(a.dy) && ok(a.y) && ok(a.dx);
+}
+template <typename T, typename F> static void gn_pick(const GnArgs &a, F f) {
+    if (gn_vectors<16 / sizeof(T), T>(a)) return gn_pick_act<16 / sizeof(T)>(a, f);
+    if constexpr (sizeof(T) == 2)
+        if (gn_vectors<4, T>(a)) return gn_pick_act<4>(a, f);
+    gn_pick_act<1>(a, f);
 }
 
 template <typename T> static int gn_forward(const GnArgs &a, void *ws, hipStream_t s) {
@@ -770,7 +802,7 @@ template <typename T> static int gn_forward(const GnArgs &a, void *ws, hipStream
     gn_pick<T>(a, [&](auto v, auto act, auto drop) {
         constexpr int V = decltype(v)::value, ACT = decltype(act)::value;
         constexpr bool DROP = decltype(drop)::value;
-        if constexpr (V > 1) {
+        if constexpr (V * sizeof(T) == 16) {
             const GnSlab sl = gn_slab<V>(a, 16);
             if (sl.sv) {
                 const int nv = (a.P * sl.sv + 511) / 512, lds = 9 * sl.sv * V * 4;
@@ -785,8 +817,9 @@ template <typename T> static int gn_forward(const GnArgs &a, void *ws, hipStream
         }
         const GnWork w = gn_work<V>(a);
         const dim3 grid((unsigned)(a.B * w.nchunk * w.nzb));
+        const unsigned char *mask = gn_mask<V>(a, ws, s);
         hipLaunchKernelGGL((gn_stats_kernel<T, V>), grid, dim3(256), 0, s, a, w, part);
-        hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, DROP>), grid, dim3(256), (a.G + 256) * sizeof(float2), s, a, w, part);
+        hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, DROP>), grid, dim3(256), (a.G + 256) * sizeof(float2), s, a, w, part, mask);
     });
     return check_launch("group_norm_forward");
 }
@@ -794,7 +827,7 @@ template <typename T> static int gn_backward(const GnArgs &a, void *ws, hipStrea
     gn_pick<T>(a, [&](auto v, auto act, auto drop) {
         constexpr int V = decltype(v)::value, ACT = decltype(act)::value;
         constexpr bool DROP = decltype(drop)::value;
-        if constexpr (V > 1) {
+        if constexpr (V * sizeof(T) == 16) {
             const GnSlab sl = gn_slab<V>(a, 12);
             if (sl.sv) {
                 const int nv = (a.P * sl.sv + 511) / 512, lds = 10 * sl.sv * V * 4;
@@ -811,7 +844,7 @@ template <typename T> static int gn_backward(const GnArgs &a, void *ws, hipStrea
         const GnWork w = gn_work<V>(a);
         const dim3 grid((unsigned)(a.B * w.nchunk * w.nzb));
         float2 *gpart = (float2 *)ws, *part = gpart + (size_t)a.B * w.nchunk * w.nsub * a.G;
-        unsigned char *mask = (unsigned char *)(part + (size_t)a.B * w.nchunk * a.C);
+        unsigned char *mask = gn_mask<V>(a, ws, s);
         const int nparam = (a.C + 127) / 128 * 8;                // whole eights: a chunk stays on the XCD that pass 1 read it on
         hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT, DROP>), grid, dim3(256), 0, s, a, w, part, gpart, mask);
         hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, DROP>), dim3(grid.x + nparam), dim3(256),

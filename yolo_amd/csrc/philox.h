@@ -75,6 +75,19 @@ template <> struct vec_io<bf16_t, 8> {
         store_stream16(p, pack(v[0], v[1]), pack(v[2], v[3]), pack(v[4], v[5]), pack(v[6], v[7]));
     }
 };
+template <> struct vec_io<bf16_t, 4> {
+    typedef uint2 raw;
+    __device__ static __forceinline__ raw load(const bf16_t *p) { return *(const uint2 *)p; }
+    __device__ static __forceinline__ void unpack(const raw &r, float (&v)[4]) {
+        v[0] = __uint_as_float(r.x << 16);
+        v[1] = __uint_as_float(r.x & 0xffff0000u);
+        v[2] = __uint_as_float(r.y << 16);
+        v[3] = __uint_as_float(r.y & 0xffff0000u);
+    }
+    __device__ static __forceinline__ void store(bf16_t *p, const float (&v)[4]) {
+        *(uint2 *)p = uint2{vec_io<bf16_t, 8>::pack(v[0], v[1]), vec_io<bf16_t, 8>::pack(v[2], v[3])};
+    }
+};
 template <> struct vec_io<float, 4> {
     typedef float4 raw;
     __device__ static __forceinline__ raw load(const float *p) { return *(const float4 *)p; }
