@@ -266,17 +266,22 @@ template <int V> struct GnChannels {
     __device__ __forceinline__ float t(int i, float x) const { return __builtin_fmaf(x - mean[i], ta[i], be[i]); }
 };
 
+// Bit i: element i0 + i is kept.
+template <int V> __device__ __forceinline__ unsigned gn_keep_bits(const DropArgs &drop, const uint4 &key, unsigned long long i0) {
+    bool keep[V];
+    drop_keep<V>(drop, key, i0, keep);
+    unsigned m = 0u;
+#pragma unroll
+    for (int i = 0; i < V; ++i) m |= keep[i] ? 1u << i : 0u;
+    return m;
+}
+
 // Single elements (V = 1) would compute four random words each for one: their bits come from a pass of its own over the flat
 // map, byte j those of elements 8 j ... 8 j + 7 (16 x 52^2 x 255, rate 0.1: forward/backward 36.4/44.7 us, 50.6/77.5 without).
 __global__ void __launch_bounds__(256) gn_mask_kernel(const DropArgs drop, unsigned long long n, unsigned char *__restrict__ mask) {
-    const unsigned long long j = (unsigned long long)blockIdx.x * 256 + threadIdx.x;
-    if (j * 8 >= n) return;
-    bool keep[8];
-    drop_keep<8>(drop, uint4{drop.state[0], drop.state[1], drop.state[2], drop.state[3]}, j * 8, keep);
-    unsigned m = 0u;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m |= keep[i] ? 1u << i : 0u;
-    mask[j] = (unsigned char)m;
+    const uint4 key = {drop.state[0], drop.state[1], drop.state[2], drop.state[3]};
+    for (unsigned long long j = (unsigned long long)blockIdx.x * 256 + threadIdx.x; j * 8 < n; j += (unsigned long long)gridDim.x * 256)
+        mask[j] = (unsigned char)gn_keep_bits<8>(drop, key, j * 8);
 }
 __device__ __forceinline__ unsigned gn_mask_bit(const unsigned char *mask, size_t i) { return mask[i >> 3] >> (i & 7) & 1u; }
 
@@ -336,14 +341,6 @@ __device__ __forceinline__ void gn_dt(const GnChannels<V> &ch, float keep_scale,
         if constexpr (DROP) d = (keep >> i & 1u) ? d * keep_scale : 0.0f;
         dt[i] = d * act_grad_c<ACT>(ch.t(i, x[i]));
     }
-}
-template <int V> __device__ __forceinline__ unsigned gn_keep_bits(const DropArgs &drop, const uint4 &key, unsigned long long i0) {
-    bool keep[V];
-    drop_keep<V>(drop, key, i0, keep);
-    unsigned m = 0u;
-#pragma unroll
-    for (int i = 0; i < V; ++i) m |= keep[i] ? 1u << i : 0u;
-    return m;
 }
 
 // dx of V values: r (gamma dt - (m1 + h m2)) = ta dt + d b + c with the group's m1 = S1 / N, m2 = S2 / N.
@@ -746,7 +743,7 @@ template <int V> static unsigned char *gn_mask(const GnArgs &a, void *ws, hipStr
     unsigned char *mask = (unsigned char *)ws + gn_pair_bytes(a.B, a.P, a.C, a.G);
     if (V == 1 && a.state) {
         const unsigned long long n = (unsigned long long)a.B * a.P * a.C;
-        hipLaunchKernelGGL(gn_mask_kernel, dim3((unsigned)((n + 2047) / 2048)), dim3(256), 0, s, DropArgs{a.state, a.threshold, a.keep_scale}, n, mask);
+        hipLaunchKernelGGL(gn_mask_kernel, dim3((unsigned)std::min<unsigned long long>((n + 2047) / 2048, 16384)), dim3(256), 0, s, DropArgs{a.state, a.threshold, a.keep_scale}, n, mask);
     }
     return mask;
 }
