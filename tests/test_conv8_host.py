@@ -80,3 +80,18 @@ def test_layers_check_before_the_device():
         c(q, residual=q)
     with pytest.raises(ValueError, match="input channels"):
         YOLOConv((3, 3, 32), dtype=F8, in_channels=64)(q)
+
+
+def test_the_planned_program_refuses_what_it_has_no_kernels_for():
+    import yolo_amd
+    from yolo_amd.backbones import Darknet53
+    with pytest.raises(ValueError, match="float32 and bfloat16"):
+        yolo_amd.Detector(num_classes=2, dtype=F8)
+    for kw in (dict(groupNormalization=8), dict(dtype=F8)):
+        det = yolo_amd.Detector(num_classes=2, dtype=torch.bfloat16)
+        det.backbone = Darknet53(seed=0, **kw)
+        for m in det.backbone.conv_layers():
+            if m.in_channels is None:
+                m.build(3)
+        with pytest.raises(ValueError, match="run by module"):
+            det._build_plan((1,), 64, torch.bfloat16, torch.device("cpu"))

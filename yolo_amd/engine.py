@@ -53,6 +53,7 @@ class Detector(nn.Module):
         self.fuse_stem = bool(fuse_stem)
         self._side_streams = {}             # device -> streams of the sub-batches after the first
         self.num_classes = num_classes
+        _lib.dtype_code(dtype)              # the planned program runs bf16 and fp32 kernels; 8-bit networks run by module
         self.dtype = dtype
         self.backbone = Darknet53(dtype=dtype, seed=seed)
         self.head = YoloV3(num_classes, dtype=dtype, seed=None if seed is None else seed + 1)
@@ -153,6 +154,8 @@ class Detector(nn.Module):
             return 0 if t is None or t.stride(2) == t.shape[3] else t.stride(2)
 
         def conv(layer, x, h, w, residual=None, x_code=code, out_dtype=cdt, head=None, out=None):
+            if layer.group_normalization or layer.is_8bit():
+                raise ValueError("Detector: layers with group normalisation and 8-bit layers run by module, not in a planned program")
             oh, ow = layer.output_hw(h, w)
             cout = layer.filters
             if head is not None and cout % 8:
