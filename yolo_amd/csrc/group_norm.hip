@@ -626,7 +626,7 @@ __global__ void __launch_bounds__(512) gn_slab_kernel(const GnArgs a, const GnSl
 }
 
 // Backward: x stays as it was read, dt as computed (fp32); the sums over a sample of each channel go to
-// part[b C + c] for the parameters' gradients.
+// part[b C + c] for the parameters' gradients; those of a single sample are the gradients (13^2 x 1024: 9.3 -> 6.4 us).
 template <typename T, int V, int NV, int ACT, bool DROP>
 __global__ void __launch_bounds__(512) gn_slab_bwd_kernel(const GnArgs a, const GnSlab w, float2 *__restrict__ part) {
     extern __shared__ float red[];                               // [8][sv V], then two of [sv V]
@@ -675,7 +675,13 @@ __global__ void __launch_bounds__(512) gn_slab_bwd_kernel(const GnArgs a, const 
     const float inv_n = 1.0f / ((float)a.P * (float)a.D);
     float ga = 0.0f;
     if ((int)threadIdx.x < W) {
-        part[(size_t)b * a.C + slab * W + threadIdx.x] = float2{t1, t2};
+        const int c = slab * W + threadIdx.x;
+        if (a.B == 1) {                                          // the sums over all samples: no second launch
+            a.dbeta[c] = t1;
+            a.dgamma[c] = t2;
+        } else {
+            part[(size_t)b * a.C + c] = float2{t1, t2};
+        }
         ga = a.gamma[slab * W + threadIdx.x] * inv_n;
     }
     const float u1 = gn_group_sum(ga * t1, a.D), u2 = gn_group_sum(ga * t2, a.D);
@@ -834,7 +840,7 @@ template <typename T> static int gn_backward(const GnArgs &a, void *ws, hipStrea
                 else if (nv <= 4) hipLaunchKernelGGL((gn_slab_bwd_kernel<T, V, 4, ACT, DROP>), grid, dim3(512), lds, s, a, sl, part);
                 else if (nv <= 6) hipLaunchKernelGGL((gn_slab_bwd_kernel<T, V, 6, ACT, DROP>), grid, dim3(512), lds, s, a, sl, part);
                 else hipLaunchKernelGGL((gn_slab_bwd_kernel<T, V, 12, ACT, DROP>), grid, dim3(512), lds, s, a, sl, part);
-                hipLaunchKernelGGL(gn_param_grads_kernel, dim3((unsigned)((a.C + 15) / 16)), dim3(1024), 0, s, a, a.B, part);
+                if (a.B > 1) hipLaunchKernelGGL(gn_param_grads_kernel, dim3((unsigned)((a.C + 15) / 16)), dim3(1024), 0, s, a, a.B, part);
                 return;
             }
         }
