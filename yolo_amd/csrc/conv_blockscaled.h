@@ -65,7 +65,7 @@ __device__ __forceinline__ void f8_to_bf16(const i32x8_t &v, int exponent, bf16x
 
 // Rows of the fp32 accumulator image in LDS (see conv_epilogue.h for the layout) with 32-bit outputs, whose residual is
 // 32-bit too, and of any output whose channel count or pixel stride is no multiple of 8 (the 255 channels
-// of the logits): there a lane takes one channel and the wave 64 neighbouring ones of a pixel at a time.
+// of the logits): there a lane takes a few neighbouring channels of a pixel, whose address need not be aligned.
 template <typename OT, int NI, int NJ>
 __device__ __forceinline__ void f8_epilogue_rows(const ConvArgs &a, f32x4_t (&acc)[NI][NJ], char *tbase, int cbase, int pbase, int lane) {
     constexpr int HQ = NI * 16 < 64 ? NI * 16 : 64, NH = NI * 16 / HQ, SLOTS = HQ / 4, LPP = SLOTS / 2, PPI = 64 / LPP, NPASS = 16 * NJ / PPI;
@@ -95,37 +95,86 @@ __device__ __forceinline__ void f8_epilogue_rows(const ConvArgs &a, f32x4_t (&ac
                     sc[r] = in ? (a.scale ? a.scale[co + r] : 1.0f) : 0.0f;
                     sh[r] = (in && a.shift) ? a.shift[co + r] : 0.0f;
                 }
-#pragma unroll 2
-                for (int n = 0; n < NPASS; ++n) {
-                    const int px = n * PPI + lane / LPP, p = pbase + px, sw = px & (SLOTS - 1);
-                    const char *row = tbase + px * (HQ * 4);
-                    const float4 v0 = *(const float4 *)(row + (((2 * sl) ^ sw) << 4));
-                    const float4 v1 = *(const float4 *)(row + (((2 * sl + 1) ^ sw) << 4));
-                    float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-                    if (p >= a.P || co >= a.Cout) continue;
+                constexpr int U = NPASS < 4 ? NPASS : 4;             // residuals of U passes in flight
+                for (int n0 = 0; n0 < NPASS; n0 += U) {
+                    float4 q[U][2];
+                    if (res)
 #pragma unroll
-                    for (int r = 0; r < 8; ++r) v[r] = act_c<ACT>(affine_f(v[r], sc[r], sh[r]));
-                    if (res) {
-                        const float4 q0 = *(const float4 *)(res + (size_t)p * a.res_ld + co), q1 = *(const float4 *)(res + (size_t)p * a.res_ld + co + 4);
-                        v[0] = __fadd_rn(v[0], q0.x); v[1] = __fadd_rn(v[1], q0.y); v[2] = __fadd_rn(v[2], q0.z); v[3] = __fadd_rn(v[3], q0.w);
-                        v[4] = __fadd_rn(v[4], q1.x); v[5] = __fadd_rn(v[5], q1.y); v[6] = __fadd_rn(v[6], q1.z); v[7] = __fadd_rn(v[7], q1.w);
+                        for (int u = 0; u < U; ++u) {
+                            const int p = pbase + (n0 + u) * PPI + lane / LPP;
+                            const float *rp = (const float *)res + (size_t)p * a.res_ld + co;
+                            if (p < a.P && co < a.Cout) { q[u][0] = *(const float4 *)rp; q[u][1] = *(const float4 *)(rp + 4); }
+                        }
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const int px = (n0 + u) * PPI + lane / LPP, p = pbase + px, sw = px & (SLOTS - 1);
+                        const char *row = tbase + px * (HQ * 4);
+                        const float4 v0 = *(const float4 *)(row + (((2 * sl) ^ sw) << 4));
+                        const float4 v1 = *(const float4 *)(row + (((2 * sl + 1) ^ sw) << 4));
+                        float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+                        if (p >= a.P || co >= a.Cout) continue;
+#pragma unroll
+                        for (int r = 0; r < 8; ++r) v[r] = act_c<ACT>(affine_f(v[r], sc[r], sh[r]));
+                        if (res) {
+                            const float4 q0 = q[u][0], q1 = q[u][1];
+                            v[0] = __fadd_rn(v[0], q0.x); v[1] = __fadd_rn(v[1], q0.y); v[2] = __fadd_rn(v[2], q0.z); v[3] = __fadd_rn(v[3], q0.w);
+                            v[4] = __fadd_rn(v[4], q1.x); v[5] = __fadd_rn(v[5], q1.y); v[6] = __fadd_rn(v[6], q1.z); v[7] = __fadd_rn(v[7], q1.w);
+                        }
+                        float *yp = (float *)y + (size_t)p * a.y_ld + co;
+                        store_stream16(yp, v[0], v[1], v[2], v[3]);
+                        store_stream16(yp + 4, v[4], v[5], v[6], v[7]);
                     }
-                    float *yp = (float *)y + (size_t)p * a.y_ld + co;
-                    store_stream16(yp, v[0], v[1], v[2], v[3]);
-                    store_stream16(yp + 4, v[4], v[5], v[6], v[7]);
                 }
             } else {
-                const int cl = lane % HQ, co = c0 + cl;              // HQ lanes per pixel, 64 / HQ pixels at a time
-                const bool in = co < a.Cout;
-                const float sc = in && a.scale ? a.scale[co] : 1.0f, sh = in && a.shift ? a.shift[co] : 0.0f;
-#pragma unroll 4
-                for (int n = 0; n < 16 * NJ / (64 / HQ); ++n) {
-                    const int px = n * (64 / HQ) + lane / HQ, p = pbase + px;
-                    float v = *(const float *)(tbase + px * (HQ * 4) + (((cl >> 2) ^ (px & (SLOTS - 1))) << 4) + (cl & 3) * 4);
-                    if (p >= a.P || !in) continue;
-                    v = act_c<ACT>(affine_f(v, sc, sh));
-                    if (res) v = __fadd_rn(v, elem<OT>::load(res + (size_t)p * a.res_ld + co));
-                    elem<OT>::store(y + (size_t)p * a.y_ld + co, v);
+                // two bf16 or four fp32 channels a lane, one access at any address; the last ones of a pixel one by one (6 x 122^2
+                // 128 -> 959 3x3 with shortcut 287 us, a channel a lane 514, 960 channels 190; 64 x 52^2 1024 -> 255 to fp32 161, 184)
+                constexpr int CH = sizeof(OT) == 4 ? 4 : 2, HL = HQ / CH, PP = 64 / HL, N = 16 * NJ / PP;
+                constexpr int B = N % (16 / CH) == 0 ? 16 / CH : N % 4 == 0 ? 4 : N % 2 == 0 ? 2 : 1;
+                struct __attribute__((packed, aligned(sizeof(OT)))) few_t { OT v[CH]; };
+                typedef float tvec_t __attribute__((ext_vector_type(CH)));
+                typedef std::conditional_t<sizeof(OT) == 4, tvec_t, uint32_t> word_t;
+                typedef word_t any_word_t __attribute__((aligned(sizeof(OT))));
+                const int cl = lane % HL * CH, co = c0 + cl, nc = min(a.Cout - co, CH);
+                float sc[CH], sh[CH];
+#pragma unroll
+                for (int r = 0; r < CH; ++r) {
+                    sc[r] = r < nc && a.scale ? a.scale[co + r] : 1.0f;
+                    sh[r] = r < nc && a.shift ? a.shift[co + r] : 0.0f;
+                }
+                for (int n0 = 0; n0 < N; n0 += B) {
+                    few_t q[B];                                          // residuals of B passes in flight
+                    if (res)
+#pragma unroll
+                        for (int u = 0; u < B; ++u) {
+                            const int p = pbase + (n0 + u) * PP + lane / HL;
+                            const OT *rp = res + (size_t)p * a.res_ld + co;
+                            if (p >= a.P) continue;
+                            if (nc >= CH) q[u] = *(const few_t *)rp;
+                            else
+#pragma unroll
+                                for (int r = 0; r < CH - 1; ++r)
+                                    if (r < nc) q[u].v[r] = rp[r];
+                        }
+#pragma unroll
+                    for (int u = 0; u < B; ++u) {
+                        const int px = (n0 + u) * PP + lane / HL, p = pbase + px;
+                        const tvec_t t = *(const tvec_t *)(tbase + px * (HQ * 4) + (((cl >> 2) ^ (px & (SLOTS - 1))) << 4) + (cl & 3) * 4);
+                        if (p >= a.P || nc <= 0) continue;
+                        tvec_t v;
+#pragma unroll
+                        for (int r = 0; r < CH; ++r) {
+                            v[r] = act_c<ACT>(affine_f(t[r], sc[r], sh[r]));
+                            if (res) v[r] = __fadd_rn(v[r], elem<OT>::load(&q[u].v[r]));
+                        }
+                        OT *yp = y + (size_t)p * a.y_ld + co;
+                        if (nc >= CH) {
+                            if constexpr (sizeof(OT) == 4) *(any_word_t *)yp = v;
+                            else *(any_word_t *)yp = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, epi_bf16x2_t));
+                        } else
+#pragma unroll
+                            for (int r = 0; r < CH - 1; ++r)
+                                if (r < nc) elem<OT>::store(yp + r, v[r]);
+                    }
                 }
             }
         }
