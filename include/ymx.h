@@ -428,7 +428,7 @@ int ymx_bn_backward_apply(const void *dz, const void *u, const float *a, const f
  * stored: the backward pass is given the same rate and the same two words.
  *   dx, dgamma, dbeta = gradients for dy = d loss / d y; the shortcut's gradient is dy itself.
  * gamma, beta, stats, dgamma, dbeta are fp32; x, residual, y, dy, dx have the type dtype.  Sums are
- * fp32 in a fixed order (reproducible).  workspace: ymx_group_norm_workspace_bytes(B, n_pix, C, G)
+ * fp32 or wider in a fixed order (reproducible).  B <= 2^20, n_pix <= 2^30, max(B, 2048) C <= 2^30.  workspace: ymx_group_norm_workspace_bytes(B, n_pix, C, G)
  * bytes, 16-byte aligned, nothing of it is kept between calls. */
 size_t ymx_group_norm_workspace_bytes(long long B, long long n_pix, int C, int G);
 int ymx_group_norm_forward(const void *x, const float *gamma, const float *beta, const void *residual, void *y, float *stats,

@@ -2,7 +2,7 @@
 // launch and, where they are differentiable, the node of torch's autograd.  At small maps such a call is
 // bound by the host.  A training step's node in Python costs it more than the kernels cost the GPU: its backward step runs on
 // autograd's own thread, which has to take the interpreter's lock from the caller first.  Host time per call, in Python
-// and here: group norm + Mish 13^2 x 1024 11.3 -> 6.0 us; with shortcut over 13^2 x 512, forward and backward, 116 -> 78; dropout
+// and here: group norm + Mish 13^2 x 1024 11.3 -> 6.0 us; with shortcut over 13^2 x 512, forward and backward, 116 -> 75; dropout
 // with shortcut, forward and backward, 80 -> 54; 8-bit convolution 13^2 1024 -> 512 (one launch) 10.6 -> 8.1,
 // 3x3 256 -> 512 (two) 17 -> 12.
 //

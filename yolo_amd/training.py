@@ -521,7 +521,7 @@ def group_norm_act(x, gamma, beta, groups, activation=None, shortcut=None, epsil
     GPU tensor, bfloat16 or float32), the statistics of every (sample, group of C / groups
     neighbouring channels) over its pixels.  gamma, beta: [C].  activation: "mish", "leaky" or None.
     rate, state: dropout before the shortcut, see ``dropout``.  Differentiable in x, gamma, beta and
-    shortcut (once; the gradients of gamma and beta are summed in fp32); with gradients disabled, or if
+    shortcut (once; the gradients of gamma and beta are summed in fp32 or wider); with gradients disabled, or if
     none of them requires one, no graph is recorded."""
     _lib.require_gpu(x, gamma, beta, shortcut)
     code = _activation_code(activation, "group_norm_act")
