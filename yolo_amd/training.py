@@ -503,7 +503,7 @@ def _check_rate(rate, who):
 def _check_dropout(x, rate, state, who):
     rate = _check_rate(rate, who)
     if rate > 0.0:
-        if not torch.is_tensor(state) or state.dtype != torch.int64 or tuple(state.shape) != (2,) or not state.is_contiguous():
+        if not torch.is_tensor(state) or state.dtype != torch.int64 or state.shape != (2,) or not state.is_contiguous():
             raise ValueError("%s: state must be an int64 tensor (seed, call number)" % who)
         if state.device != x.device:
             raise ValueError("%s: state on %s, input on %s" % (who, state.device, x.device))
@@ -523,22 +523,25 @@ def group_norm_act(x, gamma, beta, groups, activation=None, shortcut=None, epsil
     rate, state: dropout before the shortcut, see ``dropout``.  Differentiable in x, gamma, beta and
     shortcut (once; the gradients of gamma and beta are summed in fp32 or wider); with gradients disabled, or if
     none of them requires one, no graph is recorded."""
-    _lib.require_gpu(x, gamma, beta, shortcut)
+    _lib.require_gpu(x)                          # the others have to be where x is
     code = _activation_code(activation, "group_norm_act")
     if x.dim() < 2:
         raise ValueError("group_norm_act: expected [B, ..., C], got shape %s" % (tuple(x.shape),))
     _lib.dtype_code(x.dtype)
-    c, groups = x.shape[-1], int(groups)
+    c, groups, device = x.shape[-1], int(groups), x.device
     if groups <= 0 or c % groups:
         raise ValueError("group_norm_act: %d channels do not split into %d groups" % (c, groups))
     for name, t in (("gamma", gamma), ("beta", beta)):
-        if tuple(t.shape) != (c,) or t.device != x.device:
-            raise ValueError("group_norm_act: %s %s on %s, expected (%d,) on %s" % (name, tuple(t.shape), t.device, c, x.device))
+        if t.shape != (c,) or t.device != device:
+            raise ValueError("group_norm_act: %s %s on %s, expected (%d,) on %s" % (name, tuple(t.shape), t.device, c, device))
     if not epsilon > 0:
         raise ValueError("group_norm_act: epsilon %g" % epsilon)
-    _check_shortcut(x, shortcut, "group_norm_act")
-    rate = _check_dropout(x, rate, state, "group_norm_act")
-    state = state if rate > 0.0 else None
+    if shortcut is not None:
+        _check_shortcut(x, shortcut, "group_norm_act")
+    if rate != 0.0:
+        rate = _check_dropout(x, rate, state, "group_norm_act")
+    else:
+        rate, state = 0.0, None
     return _lib.native().group_norm_act(x, gamma, beta, shortcut, state, groups, code, epsilon, rate)
 
 
@@ -549,9 +552,10 @@ def dropout(x, rate, state, shortcut=None):
     equal states give equal masks and the backward pass computes the mask again from the state: leave
     its values alone until then (autograd notices an in-place change), and give every call of a step
     another call number (layers.Dropout does).  Differentiable in x and shortcut."""
-    _lib.require_gpu(x, shortcut)
+    _lib.require_gpu(x)
     _lib.dtype_code(x.dtype)
-    _check_shortcut(x, shortcut, "dropout")
+    if shortcut is not None:
+        _check_shortcut(x, shortcut, "dropout")
     rate = _check_dropout(x, rate, state, "dropout")
     if rate == 0.0:
         return x if shortcut is None else x + shortcut.to(x.dtype)
