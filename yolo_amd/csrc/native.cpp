@@ -2,8 +2,8 @@
 // launch and, where they are differentiable, the node of torch's autograd.  At small maps such a call is
 // bound by the host.  A training step's node in Python costs it more than the kernels cost the GPU: its backward step runs on
 // autograd's own thread, which has to take the interpreter's lock from the caller first.  Host time per call, in Python
-// and here: group norm + Mish 13^2 x 1024 11.3 -> 6.0 us; with shortcut over 13^2 x 512, forward and backward, 116 -> 75; dropout
-// with shortcut, forward and backward, 80 -> 54; 8-bit convolution 13^2 1024 -> 512 (one launch) 10.6 -> 8.1,
+// and here: group norm + Mish 13^2 x 1024 11.3 -> 6.0 us; with shortcut over 13^2 x 512, forward and backward, 116 -> 64-72; dropout
+// with shortcut, forward and backward, 80 -> 50; 8-bit convolution 13^2 1024 -> 512 (one launch) 10.6 -> 8.1,
 // 3x3 256 -> 512 (two) 17 -> 12.
 //
 // Arguments are checked by yolo_amd.training and yolo_amd.layers; the kernels are reached through the C entry points of
@@ -11,8 +11,9 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
-#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "../../include/ymx.h"
@@ -21,7 +22,8 @@ namespace {
 
 using at::Tensor;
 using std::optional;
-using torch::autograd::AutogradContext;
+using torch::autograd::Node;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
 #define YMX_ENTRY_POINTS(X)                                                                                   \
@@ -46,9 +48,22 @@ Tensor dense(const Tensor &t, at::ScalarType type) { return (t.scalar_type() == 
 Tensor cast(const Tensor &t, at::ScalarType type) { return t.scalar_type() == type ? t : t.to(type); }
 void *address(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 bool wants(const Tensor &t) { return t.defined() && t.requires_grad(); }
-bool wants(const optional<Tensor> &t) { return t && wants(*t); }
+Tensor given(const optional<Tensor> &t) { return t ? *t : Tensor(); }
 Tensor empty_as(const Tensor &t) { return at::empty(t.sizes(), t.options()); }
 Tensor workspace(size_t bytes, const Tensor &like) { return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)); }
+
+// Whether a call over these tensors is recorded for back-propagation.
+template <typename... Ts> bool records(const Ts &...t) {
+    if (!at::GradMode::is_enabled() || !(wants(t) || ...)) return false;
+    TORCH_CHECK(!(torch::autograd::isFwGradDefined(t) || ...), "yolo_amd.training: these operators have no forward-mode derivative");
+    return true;
+}
+// A node whose gradients go to these tensors, in this order.
+template <typename N, typename... Ts> std::shared_ptr<N> new_node(const Ts &...t) {
+    std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(t...));
+    return node;
+}
 
 // The gradients of a step that is itself being recorded (create_graph=True): an error for whoever differentiates them.
 variable_list once(bool recorded, variable_list grads) {
@@ -102,56 +117,70 @@ GroupNormOut gn_forward(const Tensor &x_in, const Tensor &gamma, const Tensor &b
     return o;
 }
 
-struct GroupNorm : torch::autograd::Function<GroupNorm> {
-    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &gamma, const Tensor &beta, const optional<Tensor> &shortcut,
-                          const optional<Tensor> &state, int64_t groups, int64_t act, double eps, double rate) {
-        GroupNormOut o = gn_forward(x, gamma, beta, shortcut, state, groups, act, eps, rate, true);
-        const GroupNormCall &c = o.call;
-        ctx->save_for_backward({o.x, o.gamma, o.beta, o.stats, state ? *state : Tensor()});
-        ctx->saved_data["call"] = std::vector<int64_t>{c.B, c.pix, c.C, c.G, c.act, c.dtype, (int64_t)c.ws, (int64_t)gamma.scalar_type(),
-                                                       (int64_t)beta.scalar_type(), shortcut ? (int64_t)shortcut->scalar_type() : -1};
-        ctx->saved_data["rate"] = rate;
-        return o.y;
+struct GroupNormBackward : Node {
+    SavedVariable x_, gamma_, beta_, stats_, state_;
+    GroupNormCall call;
+    at::ScalarType gamma_type, beta_type, shortcut_type;
+
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable *v : {&x_, &gamma_, &beta_, &stats_, &state_}) v->reset_data();
     }
     // (The gradient of the shortcut is dy itself, not an alias of it: whoever accumulates it sees who else holds it.)
-    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    variable_list apply(variable_list &&grads) override {
+        const std::lock_guard<std::mutex> lock(mutex_);
         const bool recorded = at::GradMode::is_enabled();
         const at::AutoGradMode off(false);
-        const variable_list saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &gamma = saved[1], &beta = saved[2], &stats = saved[3], &state = saved[4];
-        const std::vector<int64_t> c = ctx->saved_data["call"].toIntVector();
-        const bool need_x = ctx->needs_input_grad(0), need_g = ctx->needs_input_grad(1), need_b = ctx->needs_input_grad(2);
-        const bool need_s = c[9] >= 0 && ctx->needs_input_grad(3);
-        variable_list out(9);
-        const Tensor dy = dense(grads[0], x.scalar_type());
+        const Tensor x = x_.unpack(), gamma = gamma_.unpack(), beta = beta_.unpack(), stats = stats_.unpack(), state = state_.unpack();
+        const bool need_x = task_should_compute_output(0), need_g = task_should_compute_output(1), need_b = task_should_compute_output(2);
+        variable_list out(4);
+        if (!grads[0].defined()) return out;
         if (need_x || need_g || need_b) {
+            const Tensor dy = dense(grads[0], x.scalar_type());
             Tensor dx = empty_as(x), dgamma = empty_as(gamma), dbeta = empty_as(beta);
-            if (c[1] > 0) {
+            if (call.pix > 0) {
                 const c10::DeviceGuard guard(x.device());
-                const Tensor ws = workspace((size_t)c[6], x);
+                const Tensor ws = workspace(call.ws, x);
                 check(api.ymx_group_norm_backward(x.data_ptr(), dy.data_ptr(), (const float *)gamma.data_ptr(), (const float *)beta.data_ptr(),
-                                      (const float *)stats.data_ptr(), dx.data_ptr(), (float *)dgamma.data_ptr(), (float *)dbeta.data_ptr(), c[0], c[1],
-                                      (int)c[2], (int)c[3], (int)c[4], (int)c[5], ctx->saved_data["rate"].toDouble(), address(state), ws.data_ptr(),
-                                      (size_t)c[6], stream_of(x)));
+                                                  (const float *)stats.data_ptr(), dx.data_ptr(), (float *)dgamma.data_ptr(), (float *)dbeta.data_ptr(),
+                                                  call.B, call.pix, call.C, call.G, call.act, call.dtype, call.rate, address(state), ws.data_ptr(),
+                                                  call.ws, stream_of(x)));
             } else {
                 dgamma.zero_();
                 dbeta.zero_();
             }
             if (need_x) out[0] = dx;
-            if (need_g) out[1] = cast(dgamma, (at::ScalarType)c[7]);
-            if (need_b) out[2] = cast(dbeta, (at::ScalarType)c[8]);
+            if (need_g) out[1] = cast(dgamma, gamma_type);
+            if (need_b) out[2] = cast(dbeta, beta_type);
         }
-        if (need_s) out[3] = cast(grads[0], (at::ScalarType)c[9]);
+        if (task_should_compute_output(3)) out[3] = cast(grads[0], shortcut_type);
         return once(recorded, std::move(out));
     }
 };
 
 Tensor group_norm_act(const Tensor &x, const Tensor &gamma, const Tensor &beta, const optional<Tensor> &shortcut, const optional<Tensor> &state,
                       int64_t groups, int64_t act, double eps, double rate) {
-    if (at::GradMode::is_enabled() && (wants(x) || wants(gamma) || wants(beta) || wants(shortcut)))
-        return GroupNorm::apply(x, gamma, beta, shortcut, state, groups, act, eps, rate);
-    const at::AutoGradMode off(false);
-    return gn_forward(x, gamma, beta, shortcut, state, groups, act, eps, rate, false).y;
+    const Tensor sc = given(shortcut);
+    const bool recorded = records(x, gamma, beta, sc);
+    GroupNormOut o;
+    {
+        const at::AutoGradMode off(false);
+        o = gn_forward(x, gamma, beta, shortcut, state, groups, act, eps, rate, recorded);
+    }
+    if (recorded) {
+        auto node = new_node<GroupNormBackward>(x, gamma, beta, sc);
+        node->x_ = SavedVariable(o.x, false);
+        node->gamma_ = SavedVariable(o.gamma, false);
+        node->beta_ = SavedVariable(o.beta, false);
+        node->stats_ = SavedVariable(o.stats, false);
+        node->state_ = SavedVariable(given(state), false);
+        node->call = o.call;
+        node->gamma_type = gamma.scalar_type();
+        node->beta_type = beta.scalar_type();
+        node->shortcut_type = sc.defined() ? sc.scalar_type() : at::kFloat;
+        torch::autograd::set_history(o.y, node);
+    }
+    return o.y;
 }
 
 // ---- dropout + shortcut ----------------------------------------------------------------------------------
@@ -162,29 +191,45 @@ Tensor dropout_run(const Tensor &x_in, const optional<Tensor> &shortcut, const T
     return y;
 }
 
-struct Dropout : torch::autograd::Function<Dropout> {
-    static Tensor forward(AutogradContext *ctx, const Tensor &x, const optional<Tensor> &shortcut, const Tensor &state, double rate) {
-        ctx->save_for_backward({state});
-        ctx->saved_data["types"] = std::vector<int64_t>{(int64_t)x.scalar_type(), shortcut ? (int64_t)shortcut->scalar_type() : -1};
-        ctx->saved_data["rate"] = rate;
-        return dropout_run(x, shortcut, state, rate);
+struct DropoutBackward : Node {
+    SavedVariable state_;
+    at::ScalarType x_type, shortcut_type;
+    double rate;
+
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        state_.reset_data();
     }
-    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    variable_list apply(variable_list &&grads) override {
+        const std::lock_guard<std::mutex> lock(mutex_);
         const bool recorded = at::GradMode::is_enabled();
         const at::AutoGradMode off(false);
-        const variable_list saved = ctx->get_saved_variables();
-        const std::vector<int64_t> types = ctx->saved_data["types"].toIntVector();
-        variable_list out(4);
-        if (ctx->needs_input_grad(0)) out[0] = dropout_run(cast(grads[0], (at::ScalarType)types[0]), std::nullopt, saved[0], ctx->saved_data["rate"].toDouble());
-        if (types[1] >= 0 && ctx->needs_input_grad(1)) out[1] = cast(grads[0], (at::ScalarType)types[1]);
+        const Tensor state = state_.unpack();
+        variable_list out(2);
+        if (!grads[0].defined()) return out;
+        if (task_should_compute_output(0)) out[0] = dropout_run(cast(grads[0], x_type), std::nullopt, state, rate);
+        if (task_should_compute_output(1)) out[1] = cast(grads[0], shortcut_type);
         return once(recorded, std::move(out));
     }
 };
 
 Tensor dropout(const Tensor &x, const optional<Tensor> &shortcut, const Tensor &state, double rate) {
-    if (at::GradMode::is_enabled() && (wants(x) || wants(shortcut))) return Dropout::apply(x, shortcut, state, rate);
-    const at::AutoGradMode off(false);
-    return dropout_run(x, shortcut, state, rate);
+    const Tensor sc = given(shortcut);
+    const bool recorded = records(x, sc);
+    Tensor y;
+    {
+        const at::AutoGradMode off(false);
+        y = dropout_run(x, shortcut, state, rate);
+    }
+    if (recorded) {
+        auto node = new_node<DropoutBackward>(x, sc);
+        node->state_ = SavedVariable(state, false);
+        node->x_type = x.scalar_type();
+        node->shortcut_type = sc.defined() ? sc.scalar_type() : at::kFloat;
+        node->rate = rate;
+        torch::autograd::set_history(y, node);
+    }
+    return y;
 }
 
 // ---- convolution block in 8 bits ----------------------------------------------------------------------------
