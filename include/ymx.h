@@ -420,8 +420,8 @@ int ymx_bn_backward_apply(const void *dz, const void *u, const float *a, const f
  * group) over its pixels and channels (biased variance):
  *   h = (x - mean) / sqrt(var + eps),  t = gamma h + beta
  *   y = keep * act(t) / (1 - rate) + residual            (residual may be NULL)
- * stats [B][G] receives the pairs (mean, 1 / sqrt(var + eps)) that the backward pass takes (NULL: they are
- * not kept).
+ * stats [B][G][4] receives (mean, 1 / sqrt(var + eps), what rounding to fp32 left out of each), which the backward
+ * pass takes (NULL: not kept; 16-byte aligned).
  * rate 0: no dropout, state may be NULL.  0 < rate < 1: state points to two 64-bit words on the
  * device, (seed, call); element i of the map (linear index) is kept iff word i % 4 of
  * Philox4x32-10 with counter (i / 4, call) and key seed is >= floor(rate * 2^32).  The mask is not

@@ -482,6 +482,27 @@ def test_training_step_in_a_graph():
         torch.ones(1000, device=DEV).sum().item()                    # eager work between the replays
 
 
+@pytest.mark.parametrize("shape,groups,dt", [((1, 207, 207, 593), 1, "f32"), ((64, 26, 26, 512), 32, "f32"), ((16, 104, 104, 128), 32, "bf16"),
+                                             ((4, 150, 150, 260), 13, "bf16")])
+def test_leaky_derivative_is_taken_on_the_right_side_of_zero(shape, groups, dt):
+    """dbeta for dy = 1 counts the elements on each side of t = 0 (weights 1 and 0.1): against 64-bit signs no channel of
+    millions of elements is off by one of them, 0.9 (the sum of 43 thousand rounds to 0.004 at most)."""
+    from yolo_amd import training as T
+    c = shape[-1]
+    g = torch.Generator().manual_seed(c)
+    x = (torch.randn(shape, generator=g) + 0.25).to(DT[dt]).to(DEV)
+    ga, be = torch.randn(c, generator=g).to(DEV), torch.randn(c, generator=g).to(DEV).requires_grad_()
+    dbeta, = torch.autograd.grad(T.group_norm_act(x, ga, be, groups, "leaky").float().sum(), [be]) if dt == "f32" else \
+        torch.autograd.grad(T.group_norm_act(x, ga, be, groups, "leaky"), [be], torch.ones_like(x))
+    want = torch.zeros(c, dtype=torch.float64, device=DEV)
+    for b in range(shape[0]):
+        z = x[b].double().reshape(-1, groups, c // groups)
+        mean, var = z.mean((0, 2), keepdim=True), z.var((0, 2), unbiased=False, keepdim=True)
+        t = ((z - mean) / torch.sqrt(var + 1e-3)).reshape(-1, c) * ga.double() + be.detach().double()
+        want += torch.where(t > 0, 1.0, 0.1).sum(0, dtype=torch.float64)
+    assert float((dbeta.double() - want).abs().max()) < 0.45
+
+
 def test_gradients_share_no_memory():
     """backward() into leaves, the shortcut among them: no .grad lies in the caller's dy or in another one, and a second
     backward() over the kept graph adds the same again."""

@@ -61,6 +61,15 @@ def test_sizes_beyond_a_grid_are_refused():
     assert fwd(2, 8, 64, 8, None) == -1 and b"null" in L.ymx_last_error()
 
 
+def test_statistics_are_quadruples():
+    from yolo_amd import _lib
+    L, one, odd = _lib.lib(), ctypes.c_void_p(256), ctypes.c_void_p(264)
+    assert L.ymx_group_norm_forward(one, one, one, None, one, odd, 2, 16, 64, 8, 0, 1e-3, _lib.BF16, 0.0, None, one, 1 << 30, None) == -1
+    assert b"stats" in L.ymx_last_error()
+    assert L.ymx_group_norm_backward(one, one, one, one, odd, one, one, one, 2, 16, 64, 8, 0, _lib.BF16, 0.0, None, one, 1 << 30, None) == -1
+    assert b"stats" in L.ymx_last_error()
+
+
 def test_functions_refuse_before_the_device():
     from yolo_amd import training as T
     x, v = torch.zeros(1, 2, 2, 8), torch.zeros(8)

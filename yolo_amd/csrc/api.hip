@@ -942,6 +942,7 @@ int ymx_group_norm_forward(const void *x, const float *gamma, const float *beta,
     if (!(eps > 0.0f)) return fail(YMX_EARG, "group_norm_forward: epsilon %g", (double)eps);
     GnArgs a = {};
     if (const int rc = gn_args("group_norm_forward", a, B, n_pix, C, G, act, dtype, rate, state, workspace, ws_bytes)) return rc;
+    if (!aligned16(stats)) return fail(YMX_EARG, "group_norm_forward: stats must be 16-byte aligned");
     a.x = x; a.gamma = gamma; a.beta = beta; a.res = residual; a.y = y; a.stats = stats; a.eps = eps;
     return launch_group_norm_forward(a, workspace, (hipStream_t)stream);
 }
@@ -953,6 +954,7 @@ int ymx_group_norm_backward(const void *x, const void *dy, const float *gamma, c
         return fail(YMX_EARG, "group_norm_backward: null pointer");
     GnArgs a = {};
     if (const int rc = gn_args("group_norm_backward", a, B, n_pix, C, G, act, dtype, rate, state, workspace, ws_bytes)) return rc;
+    if (!aligned16(stats)) return fail(YMX_EARG, "group_norm_backward: stats must be 16-byte aligned");
     a.x = x; a.dy = dy; a.gamma = gamma; a.beta = beta; a.stats = (float *)stats; a.dx = dx; a.dgamma = dgamma; a.dbeta = dbeta;
     return launch_group_norm_backward(a, workspace, (hipStream_t)stream);
 }

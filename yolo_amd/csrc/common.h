@@ -316,7 +316,7 @@ struct GnArgs {
     const void *x, *res, *dy;        // [B][P][C] dense; res: shortcut added after activation and dropout, or null
     void *y, *dx;
     const float *gamma, *beta;
-    float *stats;                    // [B][G] pairs (mean, 1 / sqrt(var + eps))
+    float *stats;                    // [B][G][4]: mean, 1 / sqrt(var + eps), what their rounding left out
     float *dgamma, *dbeta;
     int B, P, C, G, D;               // samples, pixels per sample, channels, groups, channels per group
     int act, dtype;

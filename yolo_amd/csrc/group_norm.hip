@@ -67,7 +67,13 @@ template <int V> struct GnPos {
 };
 
 // A sum of squares that rounding may have taken below zero; NaN stays NaN (an infinity in the map makes the variance one).
-__device__ __forceinline__ float gn_squares(float v) { return v < 0.0f ? 0.0f : v; }
+template <typename F> __device__ __forceinline__ F gn_squares(F v) { return v < (F)0 ? (F)0 : v; }
+__device__ __forceinline__ double gn_rstd(double var, float eps) { return 1.0 / sqrt(gn_squares(var) + (double)eps); }
+// Statistics for the backward pass: mean, 1 / sqrt(var + eps) and what their rounding left out.
+__device__ __forceinline__ void gn_keep_stats(const GnArgs &a, int b, int g, double mean, double rstd) {
+    const float m = (float)mean, r = (float)rstd;
+    ((float4 *)a.stats)[(size_t)b * a.G + g] = float4{m, r, (float)(mean - m), (float)(rstd - r)};
+}
 
 // Calls use(p, load(p)) for p, p + R, ... < p1, U loads in flight at a time.
 template <int U, typename L, typename F> __device__ __forceinline__ void gn_rows(int p, int p1, int R, L load, F use) {
@@ -190,10 +196,10 @@ __global__ void __launch_bounds__(256) gn_stats_kernel(const GnArgs a, const GnW
 //   backward  (S1, S2) / N
 template <bool BWD, int V>
 __device__ __forceinline__ void gn_join(const GnArgs &a, const GnWork &w, int b, bool keep, const float2 *__restrict__ part,
-                                        float2 *__restrict__ out, float2 *__restrict__ scratch) {
+                                        float2 *__restrict__ out, double2 *__restrict__ scratch) {
     const int gl = min(a.G, 256), cl = 256 / gl, lane = threadIdx.x % gl, row = threadIdx.x / gl, blocks = w.nchunk * w.nsub;
     const float2 *__restrict__ src = part + (size_t)b * blocks * a.G;
-    const float inv_n = 1.0f / ((float)a.P * (float)a.D);
+    const double inv_n = 1.0 / ((double)a.P * a.D);
     auto values = [&](int k) {                                   // how many block k holds of a group
         const int chunk = w.nsub == 1 ? k : k / w.nsub, sub = k - chunk * w.nsub;
         const int pix = min(w.per, a.P - chunk * w.per), wid = w.nsub == 1 ? a.D : min(w.cvb * V, a.D - sub * w.cvb * V);
@@ -202,7 +208,7 @@ __device__ __forceinline__ void gn_join(const GnArgs &a, const GnWork &w, int b,
     for (int g0 = 0; g0 < a.G; g0 += gl) {
         const int g = g0 + lane;
         const bool on = row < cl && g < a.G;
-        float2 s = {0.0f, 0.0f};
+        double2 s = {0.0, 0.0};
         float piv = 0.0f;                                        // forward: sums about the first block's mean
         if (on) {
             if (!BWD) piv = src[g].x;
@@ -211,7 +217,7 @@ __device__ __forceinline__ void gn_join(const GnArgs &a, const GnWork &w, int b,
                     s.x += v.x;
                     s.y += v.y;
                 } else {
-                    const float n = values(k), d = v.x - piv;
+                    const double n = values(k), d = (double)v.x - piv;
                     s.x += n * d;
                     s.y += v.y + n * d * d;
                 }
@@ -235,11 +241,11 @@ __device__ __forceinline__ void gn_join(const GnArgs &a, const GnWork &w, int b,
                 s.y += scratch[r * gl + lane].y;
             }
             if (BWD) {
-                out[g] = float2{s.x * inv_n, s.y * inv_n};
+                out[g] = float2{(float)(s.x * inv_n), (float)(s.y * inv_n)};
             } else {
-                const float shift = s.x * inv_n;
-                out[g] = float2{piv + shift, 1.0f / sqrtf(gn_squares(s.y * inv_n - shift * shift) + a.eps)};
-                if (keep && a.stats) ((float2 *)a.stats)[(size_t)b * a.G + g] = out[g];
+                const double shift = s.x * inv_n, mean = piv + shift, rstd = gn_rstd(s.y * inv_n - shift * shift, a.eps);
+                out[g] = float2{(float)mean, (float)rstd};
+                if (keep && a.stats) gn_keep_stats(a, b, g, mean, rstd);
             }
         }
     }
@@ -256,12 +262,20 @@ template <int V> struct GnChannels {
         ta[i] = gamma * rstd;
         be[i] = beta;
     }
-    __device__ __forceinline__ void load(const GnArgs &a, const float2 *st, int c0) {      // st: of the sample's groups
+    template <typename S> __device__ __forceinline__ void load(const GnArgs &a, const S *st, int c0) {      // st: of the sample's groups
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const float2 m = st[(c0 + i) / a.D];
+            const S m = st[(c0 + i) / a.D];
             set(i, m.x, m.y, a.gamma[c0 + i], a.beta[c0 + i]);
         }
+    }
+    // a t no larger than this may have the wrong sign
+    __device__ __forceinline__ float near(int i) const { return 4e-7f * (fabsf(be[i]) + fabsf(mean[i] * ta[i])); }
+    __device__ __forceinline__ bool doubtful(float low) const {
+        float n = near(0);
+#pragma unroll
+        for (int i = 1; i < V; ++i) n = fmaxf(n, near(i));
+        return low <= n;
     }
     __device__ __forceinline__ float t(int i, float x) const { return __builtin_fmaf(x - mean[i], ta[i], be[i]); }
 };
@@ -289,9 +303,9 @@ __device__ __forceinline__ unsigned gn_mask_bit(const unsigned char *mask, size_
 template <typename T, int V, int ACT, bool DROP>
 __global__ void __launch_bounds__(256) gn_apply_kernel(const GnArgs a, const GnWork w, const float2 *__restrict__ part,
                                                        const unsigned char *__restrict__ mask) {
-    extern __shared__ __attribute__((aligned(16))) float2 joined[];      // [G], then 256 of scratch
+    extern __shared__ __attribute__((aligned(16))) float2 joined[];      // [G, even], then 256 pairs of doubles
     const GnPos<V> g(a, w);
-    gn_join<false, V>(a, w, g.b, g.chunk == 0 && g.cb == 0, part, joined, joined + a.G);
+    gn_join<false, V>(a, w, g.b, g.chunk == 0 && g.cb == 0, part, joined, (double2 *)(joined + (a.G + 1 & ~1)));
     if (!g.on) return;
     typedef vec_io<T, V> IO;
     GnChannels<V> ch;
@@ -331,15 +345,17 @@ __global__ void __launch_bounds__(256) gn_apply_kernel(const GnArgs a, const GnW
                });
 }
 
-// dt of one vector of a map and its gradient; bit i of keep: element i is kept.
+// dt of one vector of a map and its gradient; bit i of keep: element i is kept.  low (leaky): the least |t| so far.
 template <int V, int ACT, bool DROP>
 __device__ __forceinline__ void gn_dt(const GnChannels<V> &ch, float keep_scale, unsigned keep, const float (&x)[V], const float (&dy)[V],
-                                      float (&dt)[V]) {
+                                      float (&dt)[V], float &low) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         float d = dy[i];
         if constexpr (DROP) d = (keep >> i & 1u) ? d * keep_scale : 0.0f;
-        dt[i] = d * act_grad_c<ACT>(ch.t(i, x[i]));
+        const float t = ch.t(i, x[i]);
+        if constexpr (ACT == YMX_ACT_LEAKY) low = fminf(low, fabsf(t));
+        dt[i] = d * act_grad_c<ACT>(t);
     }
 }
 
@@ -355,6 +371,46 @@ template <int V> struct GnGradient {
     }
 };
 
+// The leaky derivative jumps at t = 0, and one element in ten million has a t whose fp32 sign is not that of the formula: off
+// by the whole jump.  So a thread that met a doubtful t (one in tens of thousands) goes over its rows once more: for each
+// of its elements whose sign 64-bit arithmetic turns round, use(i, p, x, right dt - wrong dt, right dt, its channel).
+template <typename T, int V, bool DROP, typename F>
+__device__ __forceinline__ void gn_mend(const GnArgs &a, const GnChannels<V> &ch, int b, int c0, int p, int p1, int R, F use) {
+    // everything is computed and loaded again: not to cost the rest registers
+    asm volatile("" : "+v"(c0), "+v"(p)::"memory");
+    typedef vec_io<T, V> IO;
+    const size_t base = (size_t)b * a.P * a.C + c0;
+    const T *__restrict__ x = (const T *)a.x + base, *__restrict__ dy = (const T *)a.dy + base;
+    gn_rows<8>(p, p1, R, [&](int q) { return IO::load(x + (size_t)q * a.C); }, [&](int q, const typename IO::raw &r) {
+        float v[V];
+        IO::unpack(r, v);
+        unsigned doubt = 0u;
+#pragma unroll
+        for (int i = 0; i < V; ++i) doubt |= fabsf(ch.t(i, v[i])) <= ch.near(i) ? 1u << i : 0u;
+        while (doubt) {
+            const int i = __builtin_ctz(doubt), c = c0 + i;
+            doubt &= doubt - 1u;
+            const float4 *st = (const float4 *)a.stats + (size_t)b * a.G;
+            const float4 own = st[c / a.D];
+            GnChannels<1> one;
+            one.load(a, st, c);
+            const size_t at = (size_t)q * a.C + i;
+            const float w = elem<T>::load(x + at);
+            const double h = ((double)w - own.x - own.z) * ((double)own.y + own.w), exact = a.gamma[c] * h + a.beta[c];
+            if ((exact > 0.0) == (one.t(0, w) > 0.0f)) continue;
+            float d = elem<T>::load(dy + at);
+            if constexpr (DROP) {
+                bool keep[1];
+                const DropArgs drop = {a.state, a.threshold, a.keep_scale};
+                drop_keep<1>(drop, uint4{a.state[0], a.state[1], a.state[2], a.state[3]}, base + at, keep);
+                d = keep[0] ? d * a.keep_scale : 0.0f;
+            }
+            const float right = d * (exact > 0.0 ? 1.0f : 0.1f), wrong = d * (exact > 0.0 ? 0.1f : 1.0f);
+            use(i, q, w, right - wrong, right, one);
+        }
+    });
+}
+
 // Pass 1, backward: part[(b nchunk + chunk) C + c] = (sum dt, sum dt h) of the chunk's pixels, and
 // gpart[((b nchunk + chunk) nsub + sub) G + g] = (S1, S2) of the block's values.  With dropout, mask (V > 1) receives a byte
 // of kept elements per vector for pass 2: the random words are a fifth of this pass (16 x 208^2 x 64, rate 0.1: backward
@@ -368,13 +424,14 @@ __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const GnArgs a, const 
     const int W = w.cvb * V;
     if (g.on) {
         GnChannels<V> ch;
-        ch.load(a, (const float2 *)a.stats + (size_t)g.b * a.G, g.c0);
+        ch.load(a, (const float4 *)a.stats + (size_t)g.b * a.G, g.c0);
         const size_t base = (size_t)g.b * a.P * a.C + g.c0;
         const T *__restrict__ x = (const T *)a.x + base, *__restrict__ dy = (const T *)a.dy + base;
         const DropArgs drop = {a.state, a.threshold, a.keep_scale};
         uint4 key = {};
         if constexpr (DROP) key = uint4{a.state[0], a.state[1], a.state[2], a.state[3]};
         float s1[V], s2[V];
+        float low = __builtin_inff();
 #pragma unroll
         for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.0f;
         struct Row { typename IO::raw x, d; unsigned keep; };
@@ -394,13 +451,22 @@ __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const GnArgs a, const 
                            keep = gn_keep_bits<V>(drop, key, at);
                            mask[at / V] = (unsigned char)keep;
                        }
-                       gn_dt<V, ACT, DROP>(ch, drop.keep_scale, keep, v, d, dt);
+                       gn_dt<V, ACT, DROP>(ch, drop.keep_scale, keep, v, d, dt, low);
 #pragma unroll
                        for (int i = 0; i < V; ++i) {
                            s1[i] += dt[i];
                            s2[i] += dt[i] * (v[i] - ch.mean[i]);
                        }
                    });
+        if constexpr (ACT == YMX_ACT_LEAKY)
+            if (ch.doubtful(low))
+                gn_mend<T, V, DROP>(a, ch, g.b, g.c0, g.p, g.p1, w.R, [&](int i, int, float v, float more, float, const GnChannels<1> &c) {
+#pragma unroll
+                    for (int k = 0; k < V; ++k) {
+                        s1[k] += k == i ? more : 0.0f;
+                        s2[k] += k == i ? more * (v - c.mean[0]) : 0.0f;
+                    }
+                });
 #pragma unroll
         for (int i = 0; i < V; ++i) red[g.r * W + g.cv * V + i] = float2{s1[i], s2[i] * ch.r[i]};
     }
@@ -468,18 +534,18 @@ __global__ void __launch_bounds__(1024) gn_param_grads_kernel(const GnArgs a, in
 template <typename T, int V, int ACT, bool DROP>
 __global__ void __launch_bounds__(256) gn_bwd_apply_kernel(const GnArgs a, const GnWork w, const float2 *__restrict__ part,
                                                            const float2 *__restrict__ gpart, const unsigned char *__restrict__ mask, int nparam) {
-    extern __shared__ __attribute__((aligned(16))) float2 joined[];      // [G], then 256 of scratch; or 16 * 17 pairs of doubles
+    extern __shared__ __attribute__((aligned(16))) float2 joined[];      // [G, even], then 256 pairs of doubles; or 16 * 17 of them
     if ((int)blockIdx.x < nparam) {                              // the first workgroups: parameter gradients, 16 channels each
         gn_param_grads<16>(a, blockIdx.x, a.B * w.nchunk, part, (double2 *)joined);
         return;
     }
     const GnPos<V> g(a, w, nparam);
-    gn_join<true, V>(a, w, g.b, false, gpart, joined, joined + a.G);
+    gn_join<true, V>(a, w, g.b, false, gpart, joined, (double2 *)(joined + (a.G + 1 & ~1)));
     if (!g.on) return;
     typedef vec_io<T, V> IO;
     GnChannels<V> ch;
     GnGradient<V> gr;
-    ch.load(a, (const float2 *)a.stats + (size_t)g.b * a.G, g.c0);
+    ch.load(a, (const float4 *)a.stats + (size_t)g.b * a.G, g.c0);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const float2 m = joined[(g.c0 + i) / a.D];
@@ -488,6 +554,7 @@ __global__ void __launch_bounds__(256) gn_bwd_apply_kernel(const GnArgs a, const
     const size_t base = (size_t)g.b * a.P * a.C + g.c0;
     const T *__restrict__ x = (const T *)a.x + base, *__restrict__ dy = (const T *)a.dy + base;
     T *__restrict__ dx = (T *)a.dx + base;
+    float low = __builtin_inff();
     struct Row { typename IO::raw x, d; unsigned keep; };
     gn_rows<4>(g.p, g.p1, w.R, [&](int p) {
                    Row q = {IO::load(x + (size_t)p * a.C), IO::load(dy + (size_t)p * a.C), 0u};
@@ -499,11 +566,19 @@ __global__ void __launch_bounds__(256) gn_bwd_apply_kernel(const GnArgs a, const
                    float v[V], d[V], dt[V];
                    IO::unpack(q.x, v);
                    IO::unpack(q.d, d);
-                   gn_dt<V, ACT, DROP>(ch, a.keep_scale, q.keep, v, d, dt);
+                   gn_dt<V, ACT, DROP>(ch, a.keep_scale, q.keep, v, d, dt, low);
 #pragma unroll
                    for (int i = 0; i < V; ++i) v[i] = gr.dx(ch, i, v[i], dt[i]);
                    IO::store(dx + (size_t)p * a.C, v);
                });
+    if constexpr (ACT == YMX_ACT_LEAKY)
+        if (ch.doubtful(low))
+            gn_mend<T, V, DROP>(a, ch, g.b, g.c0, g.p, g.p1, w.R, [&](int i, int p, float v, float, float right, const GnChannels<1> &c) {
+                const float2 m = joined[(g.c0 + i) / a.D];
+                GnGradient<1> one;
+                one.set(c, 0, m.x, m.y);
+                elem<T>::store(dx + (size_t)p * a.C + i, one.dx(c, 0, v, right));
+            });
 }
 
 // ---- one pass: the pixels of a sample's channel slab stay in registers ------------------------------
@@ -514,7 +589,7 @@ __global__ void __launch_bounds__(256) gn_bwd_apply_kernel(const GnArgs a, const
 struct GnSlab { int sv, nslab; };
 
 // sum[i] (channel cv V + i of this thread) -> totals over the workgroup's rows; tot[c] for thread c < sv V.
-template <int V> __device__ __forceinline__ float gn_slab_total(const float (&v)[V], int sv, float *red) {
+template <int V> __device__ __forceinline__ double gn_slab_total(const float (&v)[V], int sv, float *red) {
     float s[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) s[i] = v[i];
@@ -527,13 +602,13 @@ template <int V> __device__ __forceinline__ float gn_slab_total(const float (&v)
 #pragma unroll
         for (int i = 0; i < V; ++i) red[wave * W + lane * V + i] = s[i];
     __syncthreads();
-    float t = 0.0f;
+    double t = 0.0;
     if ((int)threadIdx.x < W)
         for (int w = 0; w < 8; ++w) t += red[w * W + threadIdx.x];
     return t;
 }
 // Sum over the D neighbouring threads of a group.
-__device__ __forceinline__ float gn_group_sum(float t, int D) {
+__device__ __forceinline__ double gn_group_sum(double t, int D) {
     for (int o = 1; o < D; o <<= 1) t += __shfl_xor(t, o);
     return t;
 }
@@ -552,7 +627,7 @@ __global__ void __launch_bounds__(512) gn_slab_kernel(const GnArgs a, const GnSl
 #pragma unroll
     for (int n = 0; n < NV; ++n)
         if (row + n * R < a.P) q[n] = IO::load(x + (size_t)(row + n * R) * a.C);
-    const float inv_n = 1.0f / ((float)a.P * (float)a.D);
+    const double inv_n = 1.0 / ((double)a.P * a.D);
     float s[V], mean[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) s[i] = 0.0f;
@@ -564,9 +639,8 @@ __global__ void __launch_bounds__(512) gn_slab_kernel(const GnArgs a, const GnSl
 #pragma unroll
             for (int i = 0; i < V; ++i) s[i] += v[i];
     }
-    float t = gn_group_sum(gn_slab_total<V>(s, w.sv, red), a.D) * inv_n;
-    if ((int)threadIdx.x < W) grp[threadIdx.x] = t;
-    const float m_keep = t;
+    const double m = gn_group_sum(gn_slab_total<V>(s, w.sv, red), a.D) * inv_n;
+    if ((int)threadIdx.x < W) grp[threadIdx.x] = (float)m;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -584,11 +658,10 @@ __global__ void __launch_bounds__(512) gn_slab_kernel(const GnArgs a, const GnSl
                 s[i] += d * d;
             }
     }
-    t = gn_group_sum(gn_slab_total<V>(s, w.sv, red), a.D) * inv_n;
-    t = 1.0f / sqrtf(t + a.eps);
+    const double rstd = gn_rstd(gn_group_sum(gn_slab_total<V>(s, w.sv, red), a.D) * inv_n, a.eps);
     if ((int)threadIdx.x < W) {
-        grp[threadIdx.x] = t;
-        if (a.stats && threadIdx.x % a.D == 0) ((float2 *)a.stats)[(size_t)b * a.G + (slab * W + threadIdx.x) / a.D] = float2{m_keep, t};
+        grp[threadIdx.x] = (float)rstd;
+        if (a.stats && threadIdx.x % a.D == 0) gn_keep_stats(a, b, (slab * W + threadIdx.x) / a.D, m, rstd);
     }
     __syncthreads();
     GnChannels<V> ch;
@@ -645,11 +718,12 @@ __global__ void __launch_bounds__(512) gn_slab_bwd_kernel(const GnArgs a, const 
             qd[n] = IO::load(dy + (size_t)(row + n * R) * a.C);
         }
     GnChannels<V> ch;
-    ch.load(a, (const float2 *)a.stats + (size_t)b * a.G, slab * W + cv * V);
+    ch.load(a, (const float4 *)a.stats + (size_t)b * a.G, slab * W + cv * V);
     const DropArgs drop = {a.state, a.threshold, a.keep_scale};
     uint4 key = {};
     if constexpr (DROP) key = uint4{a.state[0], a.state[1], a.state[2], a.state[3]};
     float dt[NV][V], s1[V], s2[V];
+    float low = __builtin_inff();
 #pragma unroll
     for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.0f;
 #pragma unroll
@@ -661,7 +735,7 @@ __global__ void __launch_bounds__(512) gn_slab_bwd_kernel(const GnArgs a, const 
             IO::unpack(qd[n], d);
             unsigned keep = 0u;
             if constexpr (DROP) keep = gn_keep_bits<V>(drop, key, base + (size_t)p * a.C);
-            gn_dt<V, ACT, DROP>(ch, drop.keep_scale, keep, v, d, dt[n]);
+            gn_dt<V, ACT, DROP>(ch, drop.keep_scale, keep, v, d, dt[n], low);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 s1[i] += dt[n][i];
@@ -669,25 +743,34 @@ __global__ void __launch_bounds__(512) gn_slab_bwd_kernel(const GnArgs a, const 
             }
         }
     }
+    if constexpr (ACT == YMX_ACT_LEAKY)
+        if (ch.doubtful(low))
+            gn_mend<T, V, DROP>(a, ch, b, slab * W + cv * V, row, a.P, R, [&](int i, int, float v, float more, float, const GnChannels<1> &c) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    s1[k] += k == i ? more : 0.0f;
+                    s2[k] += k == i ? more * (v - c.mean[0]) : 0.0f;
+                }
+            });
 #pragma unroll
     for (int i = 0; i < V; ++i) s2[i] *= ch.r[i];
-    const float t1 = gn_slab_total<V>(s1, w.sv, red), t2 = gn_slab_total<V>(s2, w.sv, red);
-    const float inv_n = 1.0f / ((float)a.P * (float)a.D);
-    float ga = 0.0f;
+    const double t1 = gn_slab_total<V>(s1, w.sv, red), t2 = gn_slab_total<V>(s2, w.sv, red);
+    const double inv_n = 1.0 / ((double)a.P * a.D);
+    double ga = 0.0;
     if ((int)threadIdx.x < W) {
         const int c = slab * W + threadIdx.x;
         if (a.B == 1) {                                          // the sums over all samples: no second launch
-            a.dbeta[c] = t1;
-            a.dgamma[c] = t2;
+            a.dbeta[c] = (float)t1;
+            a.dgamma[c] = (float)t2;
         } else {
-            part[(size_t)b * a.C + c] = float2{t1, t2};
+            part[(size_t)b * a.C + c] = float2{(float)t1, (float)t2};
         }
         ga = a.gamma[slab * W + threadIdx.x] * inv_n;
     }
-    const float u1 = gn_group_sum(ga * t1, a.D), u2 = gn_group_sum(ga * t2, a.D);
+    const double u1 = gn_group_sum(ga * t1, a.D), u2 = gn_group_sum(ga * t2, a.D);
     if ((int)threadIdx.x < W) {
-        g1[threadIdx.x] = u1;
-        g2[threadIdx.x] = u2;
+        g1[threadIdx.x] = (float)u1;
+        g2[threadIdx.x] = (float)u2;
     }
     __syncthreads();
     GnGradient<V> gr;
@@ -703,6 +786,13 @@ __global__ void __launch_bounds__(512) gn_slab_bwd_kernel(const GnArgs a, const 
         for (int i = 0; i < V; ++i) v[i] = gr.dx(ch, i, v[i], dt[n][i]);
         IO::store(dx + (size_t)p * a.C, v);
     }
+    if constexpr (ACT == YMX_ACT_LEAKY)
+        if (ch.doubtful(low))
+            gn_mend<T, V, DROP>(a, ch, b, slab * W + cv * V, row, a.P, R, [&](int i, int p, float v, float, float right, const GnChannels<1> &c) {
+                GnGradient<1> one;
+                one.set(c, 0, g1[cv * V + i], g2[cv * V + i]);
+                elem<T>::store(dx + (size_t)p * a.C + i, one.dx(c, 0, v, right));
+            });
 }
 
 // ---- host side -----------------------------------------------------------------------------------
@@ -800,6 +890,8 @@ template <typename T, typename F> static void gn_pick(const GnArgs &a, F f) {
     gn_pick_act<1>(a, f);
 }
 
+static size_t gn_join_lds(int G) { return (G + 1 & ~1) * sizeof(float2) + 256 * sizeof(double2); }
+
 template <typename T> static int gn_forward(const GnArgs &a, void *ws, hipStream_t s) {
     float2 *part = (float2 *)ws;
     gn_pick<T>(a, [&](auto v, auto act, auto drop) {
@@ -822,7 +914,7 @@ template <typename T> static int gn_forward(const GnArgs &a, void *ws, hipStream
         const dim3 grid((unsigned)(a.B * w.nchunk * w.nzb));
         const unsigned char *mask = gn_mask<V>(a, ws, s);
         hipLaunchKernelGGL((gn_stats_kernel<T, V>), grid, dim3(256), 0, s, a, w, part);
-        hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, DROP>), grid, dim3(256), (a.G + 256) * sizeof(float2), s, a, w, part, mask);
+        hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, DROP>), grid, dim3(256), gn_join_lds(a.G), s, a, w, part, mask);
     });
     return check_launch("group_norm_forward");
 }
@@ -851,7 +943,7 @@ template <typename T> static int gn_backward(const GnArgs &a, void *ws, hipStrea
         const int nparam = (a.C + 127) / 128 * 8;                // whole eights: a chunk stays on the XCD that pass 1 read it on
         hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT, DROP>), grid, dim3(256), 0, s, a, w, part, gpart, mask);
         hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, DROP>), dim3(grid.x + nparam), dim3(256),
-                           std::max((a.G + 256) * sizeof(float2), 16 * 17 * sizeof(double2)), s, a, w,
+                           std::max(gn_join_lds(a.G), 16 * 17 * sizeof(double2)), s, a, w,
                            part, gpart, mask, nparam);
     });
     return check_launch("group_norm_backward");

@@ -105,7 +105,7 @@ GroupNormOut gn_forward(const Tensor &x_in, const Tensor &gamma, const Tensor &b
     c.act = (int)act;
     c.dtype = dtype_of(o.x);
     c.rate = rate;
-    if (keep) o.stats = at::empty({c.B, groups, 2}, o.gamma.options());
+    if (keep) o.stats = at::empty({c.B, groups, 4}, o.gamma.options());
     if (o.x.numel() == 0) return o;                              // pix = 0: nothing is launched, here and backward
     c.pix = o.x.numel() / (c.B * c.C);
     c.ws = api.ymx_group_norm_workspace_bytes(c.B, c.pix, c.C, c.G);
