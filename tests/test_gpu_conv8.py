@@ -294,6 +294,40 @@ def test_conv8_graph_follows_a_repacked_kernel(norm):
         assert torch.equal(y, want)
 
 
+@pytest.mark.parametrize("replayed", [False, True])
+def test_conv8_repacking_waits_for_other_streams(replayed):
+    """A call (or a replay of a graph) queued on another stream before the kernel changes computes with the kernel it was
+    called with: its stream is kept busy, so that the call still waits when the main stream packs the new one in the same place."""
+    from yolo_amd.layers import YOLOConv
+    torch.manual_seed(6)
+    layer = YOLOConv((3, 3, 128), dtype=F8, in_channels=128).to(DEV)
+    x = torch.randn(2, 20, 20, 128, device=DEV).bfloat16()
+    a = torch.randn(8192, 8192, device=DEV).bfloat16()
+    b = torch.empty_like(a)
+    before = layer(x).clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = layer(x)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(30):
+            torch.mm(a, a, out=b)                             # 30 ms and more
+        if replayed:
+            g.replay()
+        else:
+            y = layer(x)
+    with torch.no_grad():
+        layer.kernel.mul_(-2.0)
+        layer.bias.fill_(1.0)
+    after = layer(x)
+    torch.cuda.synchronize()
+    assert torch.equal(y, before)
+    fresh = YOLOConv((3, 3, 128), dtype=F8, in_channels=128).to(DEV)
+    fresh.load_reference_params({"kernel": layer.kernel.detach(), "bias": layer.bias.detach()})
+    assert torch.equal(after, fresh(x)) and not torch.equal(after, before)
+
+
 def test_conv8_group_norm_output_view_is_checked():
     from yolo_amd.layers import YOLOConv
     layer = YOLOConv((1, 1, 64), dtype=F8, in_channels=64, groupNormalization=8).to(DEV)

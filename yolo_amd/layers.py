@@ -373,6 +373,8 @@ class YOLOConv(nn.Module):
         k, cin, cout = self.kernel_size, self.in_channels, self.filters
         nbytes = _lib.lib().ymx_packed_weight_bytes(k, cin, cout, code)
         old = hit[1] if f8 and hit is not None and hit[0][:2] == key[:2] else None       # graphs hold its addresses
+        if old is not None:                  # calls and replays queued on any stream still read what is overwritten here
+            torch.cuda.synchronize(dev)
         wp = torch.empty(nbytes, dtype=torch.uint8, device=dev) if old is None else old[0]
         src = self.kernel.detach().float().contiguous()
         _lib.launch("ymx_pack_weights", wp, _lib.ptr(src), _lib.ptr(wp), k, cin, cout, code)
