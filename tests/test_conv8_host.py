@@ -82,6 +82,23 @@ def test_layers_check_before_the_device():
         YOLOConv((3, 3, 32), dtype=F8, in_channels=64)(q)
 
 
+def test_quantised_maps_are_checked_against_their_buffer():
+    """The kernels take a map's extent from its shape: a buffer that does not hold it is refused before the device is used."""
+    from yolo_amd.layers import BlockQuantized, YOLOConv
+    c = YOLOConv((3, 3, 32), dtype=F8, in_channels=32)
+    need = 2 * 256 + 16                                       # 16 pixels of 32 bytes, one exponent each
+    whole = torch.zeros(need + 16, dtype=torch.uint8)
+    whole = whole[-whole.data_ptr() % 16:][:need]
+    for buf in (whole[:-1], whole.view(2, -1), torch.zeros(2 * need, dtype=torch.uint8)[::2], whole.view(torch.int8),
+                torch.zeros(need + 32, dtype=torch.uint8)[-whole.data_ptr() % 16 + 8:][:need]):
+        with pytest.raises(ValueError, match="needs a flat"):
+            c(BlockQuantized(buf, (1, 4, 4, 32)))
+    with pytest.raises(ValueError, match="needs a flat"):
+        c(BlockQuantized(whole, (2, 4, 4, 32)))
+    with pytest.raises(RuntimeError, match="GPU"):            # the right one passes this check
+        c(BlockQuantized(whole, (1, 4, 4, 32)))
+
+
 def test_the_planned_program_refuses_what_it_has_no_kernels_for():
     import yolo_amd
     from yolo_amd.backbones import Darknet53

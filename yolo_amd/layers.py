@@ -53,6 +53,14 @@ class BlockQuantized(object):
     def device(self):
         return self.buffer.device
 
+    def check(self):
+        """ValueError unless buffer is laid out and large enough for shape (the kernels read all of it)."""
+        b, n = self.buffer, self.shape.numel()
+        need = _lib.lib().ymx_quantized_bytes(n // self.shape[-1], self.shape[-1])
+        if b.dtype != torch.uint8 or b.dim() != 1 or not b.is_contiguous() or b.numel() < need or b.data_ptr() % 16:
+            raise ValueError("BlockQuantized: a map %s needs a flat, 16-byte aligned uint8 buffer of %d bytes, got %s %s" %
+                             (tuple(self.shape), need, b.dtype, tuple(b.shape)))
+
     @property
     def values(self):
         return self.buffer[:self.shape.numel()].view(torch.float8_e4m3fn).view(self.shape)
@@ -453,6 +461,8 @@ class YOLOConv(nn.Module):
             _lib.dtype_code(x.dtype)
         if b * h * w == 0:
             raise ValueError("YOLOConv: expected a non-empty map, got shape %s" % (tuple(x.shape),))
+        if quantised:
+            x.check()
         if x.device != self.kernel.device:
             raise ValueError("YOLOConv: input on %s, kernel on %s" % (x.device, self.kernel.device))
         wp, scale, shift, _ = self.packed(torch.float8_e4m3fn)
