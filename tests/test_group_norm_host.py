@@ -115,3 +115,26 @@ def test_layers_construct_and_refuse():
     assert sum(conv.drop is not None for conv in net.conv_layers()) == 23
     plain = Darknet53(seed=1)
     assert all(torch.equal(a.kernel, b.kernel) for a, b in zip(net.conv_layers(), plain.conv_layers()))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("needs", [False, True])
+def test_tangents_are_refused(grad, needs):
+    """Forward mode: an error, whether or not the input requires a gradient and gradients are enabled.  (An empty map launches
+    nothing; without a tangent the same call succeeds.)"""
+    from torch.autograd import forward_ad
+    from yolo_amd import _lib
+    native = _lib.native()
+    empty, v = torch.zeros(0, 2, 2, 8), torch.ones(8)
+    state = torch.zeros(2, dtype=torch.int64)
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t.clone().requires_grad_(needs), torch.ones_like(t))
+        assert native.group_norm_act(empty, v, v, None, None, 2, 0, 1e-3, 0.0).shape == empty.shape
+        for args in ((empty, dual(v), v, None), (empty, v, dual(v), None), (dual(empty), v, v, None), (empty, v, v, dual(empty))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                native.group_norm_act(*args, None, 2, 0, 1e-3, 0.0)
+        x = torch.ones(4)
+        for args in ((dual(x), None), (x, dual(x))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                native.dropout(*args, state, 0.5)

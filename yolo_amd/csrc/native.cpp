@@ -52,11 +52,11 @@ Tensor given(const optional<Tensor> &t) { return t ? *t : Tensor(); }
 Tensor empty_as(const Tensor &t) { return at::empty(t.sizes(), t.options()); }
 Tensor workspace(size_t bytes, const Tensor &like) { return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)); }
 
-// Whether a call over these tensors is recorded for back-propagation.
+// Whether a call over these tensors is recorded for back-propagation.  (Tangents are refused whether or not it is: a dual tensor
+// need not require a gradient, and no_grad does not switch forward mode off.)
 template <typename... Ts> bool records(const Ts &...t) {
-    if (!at::GradMode::is_enabled() || !(wants(t) || ...)) return false;
     TORCH_CHECK(!(torch::autograd::isFwGradDefined(t) || ...), "yolo_amd.training: these operators have no forward-mode derivative");
-    return true;
+    return at::GradMode::is_enabled() && (wants(t) || ...);
 }
 // A node whose gradients go to these tensors, in this order.
 template <typename N, typename... Ts> std::shared_ptr<N> new_node(const Ts &...t) {

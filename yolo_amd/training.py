@@ -522,7 +522,7 @@ def group_norm_act(x, gamma, beta, groups, activation=None, shortcut=None, epsil
     neighbouring channels) over its pixels.  gamma, beta: [C].  activation: "mish", "leaky" or None.
     rate, state: dropout before the shortcut, see ``dropout``.  Differentiable in x, gamma, beta and
     shortcut (once; the gradients of gamma and beta are summed in fp32 or wider); with gradients disabled, or if
-    none of them requires one, no graph is recorded."""
+    none of them requires one, no graph is recorded.  Forward-mode tangents are refused."""
     _lib.require_gpu(x)                          # the others have to be where x is
     code = _activation_code(activation, "group_norm_act")
     if x.dim() < 2:
@@ -551,7 +551,7 @@ def dropout(x, rate, state, shortcut=None):
     i % 4 of Philox4x32-10 with counter (i // 4, call) and key seed is >= floor(rate * 2**32), so
     equal states give equal masks and the backward pass computes the mask again from the state: leave
     its values alone until then (autograd notices an in-place change), and give every call of a step
-    another call number (layers.Dropout does).  Differentiable in x and shortcut."""
+    another call number (layers.Dropout does).  Differentiable in x and shortcut (backward mode)."""
     _lib.require_gpu(x)
     _lib.dtype_code(x.dtype)
     if shortcut is not None:
