@@ -503,6 +503,52 @@ def test_leaky_derivative_is_taken_on_the_right_side_of_zero(shape, groups, dt):
     assert float((dbeta.double() - want).abs().max()) < 0.45
 
 
+def _zero_leaky(shape, kind, dtype):
+    """Leaves with t = 0 in every element: gamma = beta = 0 (a residual branch that starts as zero), or an empty map with beta = 0."""
+    c = shape[-1]
+    g = torch.Generator(device=DEV).manual_seed(c)
+    x = torch.zeros(shape, device=DEV) if kind == "map" else torch.randn(shape, device=DEV, generator=g)
+    ga = torch.zeros(c, device=DEV) if kind == "parameters" else torch.randn(c, device=DEV, generator=g)
+    return [x.to(dtype).requires_grad_(), ga.requires_grad_(), torch.zeros(c, device=DEV, requires_grad=True)]
+
+
+@pytest.mark.parametrize("kind", ["parameters", "map"])
+@pytest.mark.parametrize("shape,groups,dt", [((2, 13, 13, 256), 32, "bf16"), ((2, 104, 104, 64), 8, "bf16"), ((3, 19, 19, 255), 5, "f32")])
+def test_leaky_derivative_at_zero(shape, groups, dt, kind):
+    from yolo_amd import training as T
+    leaves = _zero_leaky(shape, kind, DT[dt])
+    dy = torch.randn(shape, generator=torch.Generator().manual_seed(1)).to(DT[dt])
+    want = O.group_norm(*(t.detach().cpu() for t in leaves), groups, "leaky", 1e-3, dy=dy)
+    got = torch.autograd.grad(T.group_norm_act(*leaves, groups, "leaky"), leaves, dy.to(DEV))
+    for name, v in zip(("dx", "dgamma", "dbeta"), got):
+        _within(name, v, want[name], want[name + "_mag"], DT[dt] if name == "dx" else torch.float32)
+
+
+@pytest.mark.parametrize("kind", ["parameters", "map"])
+def test_leaky_backward_at_zero_is_as_fast(kind):
+    """Signs of t = 0 need no second look: the backward step over such a map takes the time of any other (a factor of two
+    leaves room for the clock)."""
+    from yolo_amd import training as T
+    shape = (16, 208, 208, 64)
+    dy = torch.randn(shape, device=DEV).bfloat16()
+
+    def micros(leaves):
+        y = T.group_norm_act(*leaves, 32, "leaky")
+        times = []
+        for _ in range(12):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            torch.autograd.grad(y, leaves, dy, retain_graph=True)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b) * 1e3)
+        return sorted(times)[4]
+    plain = [torch.randn(shape, device=DEV).bfloat16().requires_grad_()] + [torch.randn(64, device=DEV, requires_grad=True) for _ in range(2)]
+    usual, zero = micros(plain), micros(_zero_leaky(shape, kind, torch.bfloat16))
+    print("us: usual %.0f, t = 0 %.0f" % (usual, zero))
+    assert zero < 2 * usual
+
+
 def test_gradients_share_no_memory():
     """backward() into leaves, the shortcut among them: no .grad lies in the caller's dy or in another one, and a second
     backward() over the kept graph adds the same again."""

@@ -269,13 +269,14 @@ template <int V> struct GnChannels {
             set(i, m.x, m.y, a.gamma[c0 + i], a.beta[c0 + i]);
         }
     }
-    // a t no larger than this may have the wrong sign
+    // a t smaller than this may have the wrong sign (0 where nothing has been rounded: gamma = beta = 0, or a mean and a beta
+    // of 0; such a channel may hold nothing but t = 0, and has no doubtful one)
     __device__ __forceinline__ float near(int i) const { return 4e-7f * (fabsf(be[i]) + fabsf(mean[i] * ta[i])); }
     __device__ __forceinline__ bool doubtful(float low) const {
         float n = near(0);
 #pragma unroll
         for (int i = 1; i < V; ++i) n = fmaxf(n, near(i));
-        return low <= n;
+        return low < n;
     }
     __device__ __forceinline__ float t(int i, float x) const { return __builtin_fmaf(x - mean[i], ta[i], be[i]); }
 };
@@ -386,7 +387,7 @@ __device__ __forceinline__ void gn_mend(const GnArgs &a, const GnChannels<V> &ch
         IO::unpack(r, v);
         unsigned doubt = 0u;
 #pragma unroll
-        for (int i = 0; i < V; ++i) doubt |= fabsf(ch.t(i, v[i])) <= ch.near(i) ? 1u << i : 0u;
+        for (int i = 0; i < V; ++i) doubt |= fabsf(ch.t(i, v[i])) < ch.near(i) ? 1u << i : 0u;
         while (doubt) {
             const int i = __builtin_ctz(doubt), c = c0 + i;
             doubt &= doubt - 1u;
