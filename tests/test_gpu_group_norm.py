@@ -503,6 +503,47 @@ def test_leaky_derivative_is_taken_on_the_right_side_of_zero(shape, groups, dt):
     assert float((dbeta.double() - want).abs().max()) < 0.45
 
 
+@pytest.mark.parametrize("far", [1.0, 100.0, 1000.0])
+@pytest.mark.parametrize("shape,groups,dt", [((2, 26, 26, 256), 16, "bf16"), ((2, 26, 26, 256), 16, "f32"), ((2, 104, 104, 64), 4, "bf16"),
+                                             ((2, 40, 41, 260), 13, "bf16"), ((2, 52, 52, 128), 2, "f32"), ((2, 40, 41, 255), 5, "f32")])
+def test_leaky_derivative_with_a_mean_far_from_zero(shape, groups, dt, far):
+    """The sign of t where the mean is `far` spreads from zero.  beta is chosen, channel by channel, so that one value of the map
+    has a t of about 1e-7: above what the kept statistics may be off by, below what fp32 ones would be off by (2^-24 far / sqrt 3
+    a rounding: 3e-6 at 100).
+    Their error, at its largest here (26^2, 16 channels a group): fp32 sums of a wave's 85 pixels of a channel about the first
+    pixel's value, which is one spread off the mean, so that k values add up to k spreads and each addition rounds by 2^-24 /
+    sqrt 3 of that: eleven in a row in each of eight lanes, then their tree, sqrt(8 * 11^3 / 3 + 4 * 22^2 + 2 * 44^2 + 88^2) = 131,
+    4.5e-6 spreads.  128 of those sums make a group of 10816 values: 4.5e-6 sqrt(128) / 10816 = 5e-9 of a spread; the
+    squares' sum is off by the same part of itself.  Eight times that, 4e-8 (|gamma| + |beta|), is not asked about."""
+    from yolo_amd import training as T
+    c, d = shape[-1], shape[-1] // groups
+    g = torch.Generator().manual_seed(int(far) + c)
+    x = (torch.randn(shape, generator=g) + far).to(DT[dt])
+    ga = (0.5 + torch.rand(c, generator=g)) * torch.where(torch.rand(c, generator=g) < 0.5, -1.0, 1.0)
+    xd = x.double().reshape(shape[0], -1, groups, d)
+    mean = xd.mean((1, 3), keepdim=True)
+    r = 1.0 / torch.sqrt((xd - mean).square().mean((1, 3), keepdim=True) + 1e-3)
+    h = ((xd - mean) * r).reshape(shape[0], -1, c)
+    near = h[0].abs().argmin(0)                                # one pixel a channel: the value of sample 0 next to the mean
+    aim = -ga.double() * h[0, near, torch.arange(c)]
+    be = (aim + (1.0 + aim.abs()) * 1e-7 * torch.where(torch.arange(c) % 2 == 0, 1.0, -1.0)).float()
+    t = ga.double() * h + be.double()
+    asked = t.abs() > 4e-8 * (ga.double().abs() + be.double().abs())
+    assert int((asked & (t.abs() < 3e-7)).sum()) >= c // 2      # what the test is about
+    leaves = [v.to(DEV).requires_grad_() for v in (x, ga, be)]
+    y = T.group_norm_act(*leaves, groups, "leaky")
+    dx, _, dbeta = torch.autograd.grad(y, leaves, torch.ones_like(y))
+    dt_ = torch.where(t > 0, 1.0, 0.1).double()
+    gd = (ga.double() * dt_).reshape(xd.shape)
+    hg = h.reshape(xd.shape)
+    want = r * (gd - gd.mean((1, 3), keepdim=True) - hg * (gd * hg).mean((1, 3), keepdim=True))
+    off = ((dx.double().cpu().reshape(xd.shape) - want) / (r * ga.double().abs().reshape(1, 1, groups, d))).abs().reshape(t.shape)
+    wrong = int((asked & (off > 0.45)).sum())                  # a wrong sign: 0.9
+    assert wrong == 0, wrong
+    whole = asked.all((0, 1))
+    assert float((dbeta.double().cpu() - dt_.sum((0, 1)))[whole].abs().max()) < 0.45
+
+
 def _zero_leaky(shape, kind, dtype):
     """Leaves with t = 0 in every element: gamma = beta = 0 (a residual branch that starts as zero), or an empty map with beta = 0."""
     c = shape[-1]

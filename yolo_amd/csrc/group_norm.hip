@@ -13,7 +13,7 @@
 // needed instead of being stored.
 //
 // Chunked form: the pixels of a sample are cut into chunks, a workgroup per chunk.  Pass 1 leaves one
-// pair of numbers per (chunk, group) -- mean and centred sum of squares, or S1 and S2 -- and, backward,
+// pair of numbers per (chunk, group) -- mean and centred sum of squares (in 64 bits), or S1 and S2 -- and, backward,
 // one per (chunk, channel); every workgroup of pass 2 first joins the pairs of its sample (a few
 // hundred, from L2), then reads the map again and writes.  Slab form: see gn_slab_kernel.  All sums
 // are fp32 or wider, added in a fixed order: no result depends on the order workgroups run in.
@@ -121,19 +121,24 @@ template <typename F, typename D2> __device__ __forceinline__ void gn_over_group
 }
 
 // Pass 1, forward: part[((b nchunk + chunk) nsub + sub) G + g] = (mean, sum of squares about it) of the block's values.
-// A thread sums about its own first value, so what cancels in s2 - s1^2 / n is at most n eps of the result.
+// A thread sums about its own first value, so what cancels in s2 - s1^2 / n is at most n eps of the result; the threads' means
+// stay (first value, rest) until they are joined in 64 bits, so that what is lost is small against the spread, wherever the
+// mean lies (rounded to fp32 each: 3e-6 of the spread at a mean of 100 spreads; the leaky derivative shows that, see gn_mend).
 template <typename T, int V>
-__global__ void __launch_bounds__(256) gn_stats_kernel(const GnArgs a, const GnWork w, float2 *__restrict__ part) {
-    __shared__ float2 red[256 * V];                              // [R][W]; row 0 then holds the channels' pairs
+__global__ void __launch_bounds__(256) gn_stats_kernel(const GnArgs a, const GnWork w, double2 *__restrict__ part) {
+    __shared__ float2 red[256 * V];                              // [R][W] (mean - first value, squares); row 0 then holds the channels' pairs
+    __shared__ __attribute__((aligned(16))) T first[256 * V];    // [R][W]; row 0 then holds what is missing from the channels' means
     const GnPos<V> g(a, w);
     typedef vec_io<T, V> IO;
     const T *__restrict__ x = (const T *)a.x + (size_t)g.b * a.P * a.C + g.c0;
     const int W = w.cvb * V;
     if (g.on) {
         float piv[V], s1[V], s2[V];
+        typename IO::raw q0 = {};
 #pragma unroll
-        for (int i = 0; i < V; ++i) piv[i] = s1[i] = s2[i] = 0.0f;
-        if (g.p < g.p1) IO::unpack(IO::load(x + (size_t)g.p * a.C), piv);
+        for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.0f;
+        if (g.p < g.p1) q0 = IO::load(x + (size_t)g.p * a.C);
+        IO::unpack(q0, piv);
         gn_rows<4>(g.p, g.p1, w.R, [&](int p) { return IO::load(x + (size_t)p * a.C); },
                    [&](int, const typename IO::raw &q) {
                        float v[V];
@@ -148,29 +153,42 @@ __global__ void __launch_bounds__(256) gn_stats_kernel(const GnArgs a, const GnW
         const int n = g.p < g.p1 ? (g.p1 - g.p + w.R - 1) / w.R : 0;
         const float inv = n > 0 ? 1.0f / (float)n : 0.0f;
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            red[g.r * W + g.cv * V + i] = float2{piv[i] + s1[i] * inv, gn_squares(s2[i] - s1[i] * s1[i] * inv)};
+        for (int i = 0; i < V; ++i) red[g.r * W + g.cv * V + i] = float2{s1[i] * inv, gn_squares(s2[i] - s1[i] * s1[i] * inv)};
+        *(typename IO::raw *)&first[g.r * W + g.cv * V] = q0;
     }
     __syncthreads();
     const int np = g.p1 - g.chunk * w.per;                       // pixels of the chunk
     const int rows = min(w.R, np);
+    // The n values of row r: the chunk's pixels r, r + R, ...
+    const int each = np / w.R, more = np - each * w.R;
+    auto row = [&](int r, int c, double &n, double &m, float &m2) {
+        const float2 q = red[r * W + c];
+        n = each + (r < more ? 1 : 0);
+        m = (double)elem<T>::load(&first[r * W + c]) + q.x;
+        m2 = q.y;
+    };
     for (int c = threadIdx.x; c < g.wc; c += 256) {
-        float mean = 0.0f, m2 = 0.0f;
-        for (int r = 0; r < rows; ++r) mean += (float)((np - r + w.R - 1) / w.R) * red[r * W + c].x;
-        mean /= (float)np;
+        double mean = 0.0, sq = 0.0, n, m;
+        float m2;
         for (int r = 0; r < rows; ++r) {
-            const float2 q = red[r * W + c];
-            const float d = q.x - mean;
-            m2 += q.y + (float)((np - r + w.R - 1) / w.R) * d * d;
+            row(r, c, n, m, m2);
+            mean += n * m;
         }
-        red[c] = float2{mean, m2};
+        mean /= np;
+        for (int r = 0; r < rows; ++r) {
+            row(r, c, n, m, m2);
+            sq += m2 + n * ((m - mean) * (m - mean));
+        }
+        const float hi = (float)mean;
+        red[c] = float2{hi, (float)sq};
+        elem<T>::store(&first[c], (float)(mean - hi));
     }
     __syncthreads();
-    const float inv_d = 1.0f / (float)g.D;
-    float2 *dst = part + g.pair(a, w);
+    const double inv_d = 1.0 / g.D;
+    double2 *dst = part + g.pair(a, w);
     const int ng = g.wc / g.D, lane = threadIdx.x & 63;
-    const int first = g.D <= 16 ? 0 : lane, step = g.D <= 16 ? 1 : 64;       // a thread per narrow group, a wave per wide one
-    auto group_sum = [&](float v) {
+    const int c0 = g.D <= 16 ? 0 : lane, step = g.D <= 16 ? 1 : 64;       // a thread per narrow group, a wave per wide one
+    auto group_sum = [&](double v) {
         if (step == 64)
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
@@ -178,15 +196,16 @@ __global__ void __launch_bounds__(256) gn_stats_kernel(const GnArgs a, const GnW
     };
     for (int gr = step == 1 ? threadIdx.x : threadIdx.x >> 6; gr < ng; gr += step == 1 ? 256 : 4) {
         const float2 *ch = red + gr * g.D;
-        float mean = 0.0f, m2 = 0.0f;
-        for (int c = first; c < g.D; c += step) mean += ch[c].x;
+        const T *rest = first + gr * g.D;
+        double mean = 0.0, sq = 0.0;
+        for (int c = c0; c < g.D; c += step) mean += (double)ch[c].x + elem<T>::load(&rest[c]);
         mean = group_sum(mean) * inv_d;
-        for (int c = first; c < g.D; c += step) {
-            const float d = ch[c].x - mean;
-            m2 += ch[c].y + (float)np * d * d;
+        for (int c = c0; c < g.D; c += step) {
+            const double d = (double)ch[c].x + elem<T>::load(&rest[c]) - mean;
+            sq += ch[c].y + np * (d * d);
         }
-        m2 = group_sum(m2);
-        if (step == 1 || lane == 0) dst[gr] = float2{mean, m2};
+        sq = group_sum(sq);
+        if (step == 1 || lane == 0) dst[gr] = double2{mean, sq};
     }
 }
 
@@ -194,37 +213,37 @@ __global__ void __launch_bounds__(256) gn_stats_kernel(const GnArgs a, const GnW
 // part (256: group lanes x block lanes).  out[g] in LDS; scratch holds 256 pairs.
 //   forward   (mean, 1 / sqrt(var + eps)); one workgroup of the sample keeps it in stats
 //   backward  (S1, S2) / N
-template <bool BWD, int V>
-__device__ __forceinline__ void gn_join(const GnArgs &a, const GnWork &w, int b, bool keep, const float2 *__restrict__ part,
+template <bool BWD, int V, typename Pair>
+__device__ __forceinline__ void gn_join(const GnArgs &a, const GnWork &w, int b, bool keep, const Pair *__restrict__ part,
                                         float2 *__restrict__ out, double2 *__restrict__ scratch) {
     const int gl = min(a.G, 256), cl = 256 / gl, lane = threadIdx.x % gl, row = threadIdx.x / gl, blocks = w.nchunk * w.nsub;
-    const float2 *__restrict__ src = part + (size_t)b * blocks * a.G;
+    const Pair *__restrict__ src = part + (size_t)b * blocks * a.G;
     const double inv_n = 1.0 / ((double)a.P * a.D);
     auto values = [&](int k) {                                   // how many block k holds of a group
         const int chunk = w.nsub == 1 ? k : k / w.nsub, sub = k - chunk * w.nsub;
         const int pix = min(w.per, a.P - chunk * w.per), wid = w.nsub == 1 ? a.D : min(w.cvb * V, a.D - sub * w.cvb * V);
-        return (float)pix * (float)wid;
+        return (double)pix * wid;
     };
     for (int g0 = 0; g0 < a.G; g0 += gl) {
         const int g = g0 + lane;
         const bool on = row < cl && g < a.G;
         double2 s = {0.0, 0.0};
-        float piv = 0.0f;                                        // forward: sums about the first block's mean
+        double piv = 0.0;                                        // forward: sums about the first block's mean
         if (on) {
             if (!BWD) piv = src[g].x;
-            auto add = [&](int k, float2 v) {
+            auto add = [&](int k, const Pair &v) {
                 if (BWD) {
                     s.x += v.x;
                     s.y += v.y;
                 } else {
-                    const double n = values(k), d = (double)v.x - piv;
+                    const double n = values(k), d = v.x - piv;
                     s.x += n * d;
                     s.y += v.y + n * d * d;
                 }
             };
             int k = row;
             for (; k + 7 * cl < blocks; k += 8 * cl) {
-                float2 v[8];
+                Pair v[8];
 #pragma unroll
                 for (int u = 0; u < 8; ++u) v[u] = src[(size_t)(k + u * cl) * a.G + g];
 #pragma unroll
@@ -302,7 +321,7 @@ __device__ __forceinline__ unsigned gn_mask_bit(const unsigned char *mask, size_
 
 // Pass 2, forward.
 template <typename T, int V, int ACT, bool DROP>
-__global__ void __launch_bounds__(256) gn_apply_kernel(const GnArgs a, const GnWork w, const float2 *__restrict__ part,
+__global__ void __launch_bounds__(256) gn_apply_kernel(const GnArgs a, const GnWork w, const double2 *__restrict__ part,
                                                        const unsigned char *__restrict__ mask) {
     extern __shared__ __attribute__((aligned(16))) float2 joined[];      // [G, even], then 256 pairs of doubles
     const GnPos<V> g(a, w);
@@ -372,9 +391,12 @@ template <int V> struct GnGradient {
     }
 };
 
-// The leaky derivative jumps at t = 0, and one element in ten million has a t whose fp32 sign is not that of the formula: off
-// by the whole jump.  So a thread that met a doubtful t (one in tens of thousands) goes over its rows once more: for each
-// of its elements whose sign 64-bit arithmetic turns round, use(i, p, x, right dt - wrong dt, right dt, its channel).
+// The leaky derivative jumps at t = 0, and one element in ten million (mean and spread alike; in proportion to the mean) has a t
+// whose fp32 sign is not that of the formula: off by the whole jump.  So a thread that met a doubtful t (one element in a
+// million has one, or more where |beta| + |gamma mean| r is above 1) goes over its rows once more: for each of its elements
+// whose sign 64-bit arithmetic on the kept statistics turns round, use(i, p, x, right dt - wrong dt, right dt, its channel).
+// Those are off by about 5e-9 of the spread (fp32 sums of differences from a value of the map, joined in 64 bits), wherever
+// the mean lies; one sign in a hundred million elements stays undecided.
 template <typename T, int V, bool DROP, typename F>
 __device__ __forceinline__ void gn_mend(const GnArgs &a, const GnChannels<V> &ch, int b, int c0, int p, int p1, int R, F use) {
     // everything is computed and loaded again: not to cost the rest registers
@@ -624,6 +646,9 @@ __global__ void __launch_bounds__(512) gn_slab_kernel(const GnArgs a, const GnSl
     const T *__restrict__ x = (const T *)a.x + base, *__restrict__ res = (const T *)a.res + base;
     T *__restrict__ y = (T *)a.y + base;
     float *grp = red + 8 * W;
+    // sums about the first pixel's values, so that what they lose is small against the spread
+    const typename IO::raw q0 = IO::load(x);
+    const float c0 = (int)threadIdx.x < W ? elem<T>::load((const T *)a.x + (size_t)b * a.P * a.C + slab * W + threadIdx.x) : 0.0f;
     typename IO::raw q[NV];
 #pragma unroll
     for (int n = 0; n < NV; ++n)
@@ -632,15 +657,16 @@ __global__ void __launch_bounds__(512) gn_slab_kernel(const GnArgs a, const GnSl
     float s[V], mean[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) s[i] = 0.0f;
+    IO::unpack(q0, mean);
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
         float v[V];
         IO::unpack(q[n], v);
         if (row + n * R < a.P)
 #pragma unroll
-            for (int i = 0; i < V; ++i) s[i] += v[i];
+            for (int i = 0; i < V; ++i) s[i] += v[i] - mean[i];
     }
-    const double m = gn_group_sum(gn_slab_total<V>(s, w.sv, red), a.D) * inv_n;
+    const double m = gn_group_sum(gn_slab_total<V>(s, w.sv, red) + (double)a.P * c0, a.D) * inv_n, off = m - (float)m;
     if ((int)threadIdx.x < W) grp[threadIdx.x] = (float)m;
     __syncthreads();
 #pragma unroll
@@ -659,7 +685,7 @@ __global__ void __launch_bounds__(512) gn_slab_kernel(const GnArgs a, const GnSl
                 s[i] += d * d;
             }
     }
-    const double rstd = gn_rstd(gn_group_sum(gn_slab_total<V>(s, w.sv, red), a.D) * inv_n, a.eps);
+    const double rstd = gn_rstd(gn_group_sum(gn_slab_total<V>(s, w.sv, red), a.D) * inv_n - off * off, a.eps);
     if ((int)threadIdx.x < W) {
         grp[threadIdx.x] = (float)rstd;
         if (a.stats && threadIdx.x % a.D == 0) gn_keep_stats(a, b, (slab * W + threadIdx.x) / a.D, m, rstd);
@@ -829,7 +855,8 @@ template <int V> static GnWork gn_work(const GnArgs &a) {
     w.nchunk = (a.P + w.per - 1) / w.per;
     return w;
 }
-// Pairs: one per (chunk, channel) and one per (chunk, group or part of one).  Behind them the bytes of kept elements, one for
+// Pairs: one per (chunk, channel) and one per (chunk, group or part of one); the forward pass has the latter alone, of twice
+// the size, and there are no more groups' parts than channels.  Behind them the bytes of kept elements, one for
 // four or eight.
 static size_t gn_pairs(int G, int C) { return (size_t)G * ((C / G + 255) / 256); }
 static size_t gn_pair_bytes(int B, int P, int C, int G) { return (size_t)B * gn_chunks(B, P, C) * (C + gn_pairs(G, C)) * sizeof(float2); }
@@ -894,7 +921,6 @@ template <typename T, typename F> static void gn_pick(const GnArgs &a, F f) {
 static size_t gn_join_lds(int G) { return (G + 1 & ~1) * sizeof(float2) + 256 * sizeof(double2); }
 
 template <typename T> static int gn_forward(const GnArgs &a, void *ws, hipStream_t s) {
-    float2 *part = (float2 *)ws;
     gn_pick<T>(a, [&](auto v, auto act, auto drop) {
         constexpr int V = decltype(v)::value, ACT = decltype(act)::value;
         constexpr bool DROP = decltype(drop)::value;
@@ -913,6 +939,7 @@ template <typename T> static int gn_forward(const GnArgs &a, void *ws, hipStream
         }
         const GnWork w = gn_work<V>(a);
         const dim3 grid((unsigned)(a.B * w.nchunk * w.nzb));
+        double2 *part = (double2 *)ws;                           // (the room of the channels' pairs, which only the backward pass has)
         const unsigned char *mask = gn_mask<V>(a, ws, s);
         hipLaunchKernelGGL((gn_stats_kernel<T, V>), grid, dim3(256), 0, s, a, w, part);
         hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, DROP>), grid, dim3(256), gn_join_lds(a.G), s, a, w, part, mask);
