@@ -411,6 +411,31 @@ def test_dropout_after_plain_and_batch_norm_blocks():
         assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1]) and torch.equal(got[2], dy)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("shape,cin,cout,k", [((2, 12, 10), 64, 96, 3), ((1, 40, 41), 32, 64, 1)])
+def test_group_norm_layer_with_a_32_bit_result(dtype, shape, cin, cout, k):
+    """out_dtype=torch.float32: the normalisation of the convolution's own 32-bit result, not of one rounded to bf16 on the way."""
+    from yolo_amd.layers import YOLOConv
+    torch.manual_seed(3)
+    conv = YOLOConv((k, k, cout), groupNormalization=8, activation="mish", in_channels=cin, dtype=dtype).to(DEV)
+    linear = YOLOConv((k, k, cout), activation=None, in_channels=cin, dtype=dtype).to(DEV)
+    with torch.no_grad():
+        conv.kernel.mul_(8.0)
+        conv.gn.gamma.add_(0.3 * torch.randn(cout, device=DEV))
+        conv.gn.beta.add_(0.3 * torch.randn(cout, device=DEV))
+        linear.kernel.copy_(conv.kernel)
+    x = torch.randn(*shape, cin, device=DEV).bfloat16()
+    sc = torch.randn(*shape, cout, device=DEV)
+    u = linear(x, out_dtype=torch.float32)
+    want = O.group_norm(u.cpu(), conv.gn.gamma.detach().cpu(), conv.gn.beta.detach().cpu(), 8, "mish", 1e-3, sc.cpu())
+    y = conv(x, residual=sc, out_dtype=torch.float32)
+    assert y.dtype == torch.float32
+    _within("y", y, want["y"], want["t_mag"] + want["y"].abs() + sc.cpu().double().abs(), torch.float32)
+    buf = torch.zeros(*shape, cout + 8, device=DEV)
+    assert torch.equal(conv(x, residual=sc, out_dtype=torch.float32, out=buf[..., :cout]), y) and not buf[..., cout:].any()
+    assert conv(x).dtype == torch.bfloat16                       # the default stays the map's type
+
+
 def test_backbone_with_group_norm_and_dropout():
     """Darknet53(groupNormalization=, dropout=): one training step reaches every parameter, inference runs."""
     from yolo_amd import training as T

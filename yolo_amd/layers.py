@@ -522,7 +522,8 @@ class YOLOConv(nn.Module):
             y = _training.conv_block(self, x, residual, _grad_link)
             return y if out_dtype in (None, y.dtype) else y.to(out_dtype)
         if self.group_normalization and not _linear:
-            u = self.forward(x, _linear=True)
+            # (a 32-bit result comes from 32-bit sums, as that of any other layer)
+            u = self.forward(x, out_dtype=torch.float32 if out_dtype == torch.float32 else None, _linear=True)
             if out is not None:
                 self._check_out(out, *u.shape[:3], out_dtype or u.dtype, u.device)
             y = self.gn.apply_act(u, self.act_code, residual, training=False)
