@@ -379,7 +379,7 @@ conv_f8_wide_kernel(const F8Args g, const int ntq, const int ncb, const int np4,
 
 static int slab_pieces(int W, int tp) { return (tp + 2 * W + 2 + 7) / 8; }
 static int slab_lds(int pieces) { return 2 * pieces * 1024 + 4 * F8_PIECE + 1024 + 1024 + 1024; }
-// Slabs of 192-pixel tiles fit for rows up to 91 pixels, of 256-pixel tiles up to 59.
+// Slabs of 192-pixel tiles fit for rows up to 87 pixels, of 256-pixel tiles up to 55.
 static bool slab_fits(const F8Args &g) { return g.taps == 9 && g.a.stride == 1 && slab_lds(slab_pieces(g.a.W, 192)) <= 160 * 1024; }
 
 // Layers for these kernels: bf16 outputs, 160 tiles and more, 256-channel tiles no more than a quarter wider than
