@@ -203,10 +203,13 @@ int ymx_run_program(const ymx_op *ops /* host */, int n_ops, void *stream);
 
 /* Diagnostic (no counterpart in the reference): the kernel family ymx_run_program would
  * launch for a convolution op with the calling thread's options -- "halo", "halo192", "dma", "dma4",
- * "dma2", "slab2", "igemm", "first_rows" or "direct" (a static string) -- or NULL with
+ * "dma2", "slab2", "igemm", "first_rows", "direct" or "f8" (a static string) -- or NULL with
  * ymx_last_error() set when the op is invalid.  Nothing is launched.  Benchmarks use it to
  * attribute measured launch times to kernels without mirroring the selection rules. */
 const char *ymx_conv_kernel_label(const ymx_op *op /* host */);
+/* The same for an op of dtype YMX_F8E4M3: the tile its kernel works in, channels x pixels ("64x32 raw" where it quantises a bf16
+ * map itself, "256x192 slab" where the input stays in LDS over the taps). */
+const char *ymx_conv8_tile_label(const ymx_op *op /* host */);
 
 /* ---- decode (+ score filter) ------------------------------------------------
  * Replaces decode / decode_predict (utils.py:107-126, 133-140) for all scales at

@@ -63,6 +63,7 @@ SIGNATURES = {
     "ymx_conv_resblock_fused": (_i, [_vp] * 8 + [_i] * 7 + [_vp]),
     "ymx_run_program": (_i, [ctypes.POINTER(ymx_op), _i, _vp]),
     "ymx_conv_kernel_label": (ctypes.c_char_p, [ctypes.POINTER(ymx_op)]),
+    "ymx_conv8_tile_label": (ctypes.c_char_p, [ctypes.POINTER(ymx_op)]),
     "ymx_decode_workspace_bytes": (_sz, [_i, _i, ctypes.POINTER(_i)]),
     "ymx_decode_filter": (_i, [ctypes.POINTER(_vp), _i, ctypes.POINTER(_i), _i, _i, _i,
                                ctypes.POINTER(_f), ctypes.POINTER(_f), ctypes.POINTER(_f),

@@ -81,8 +81,8 @@ static int conv_impl(const void *x, const void *w, const void *scale, const void
                      const void *residual, void *y, int B, int H, int W, int Cin, int Cout, int k,
                      int stride, int act, int dtype, int x_dtype, int out_dtype, int x_ld, int res_ld,
                      int y_ld, hipStream_t s, int op_min_tiles = 0, const char **label = nullptr, void *z = nullptr,
-                     const int *d2s = nullptr) {
-    // label != nullptr: validate and select only; *label names the kernel family, nothing is launched
+                     const int *d2s = nullptr, const char **tile = nullptr) {
+    // label != nullptr: validate and select only; *label names the kernel family, nothing is launched (8 bits: *tile its tile)
     // z != nullptr: the value before the activation is stored too (bf16, dense); kernels without
     // that second output run as two launches, convolution into z and then y = act(z) + residual
     // d2s = {H', W', C}: a 2x2 window (taps at +0 / +1, zeros beyond the bottom / right edge) whose Cout = 4 C
@@ -149,7 +149,11 @@ static int conv_impl(const void *x, const void *w, const void *scale, const void
         if (a.x_ld % 8) return fail(YMX_EARG, "conv2d: pixel stride %d of an 8-bit layer's map (a multiple of 8)", a.x_ld);
         if (!aligned16(x) || !aligned16(w)) return fail(YMX_EARG, "conv2d: x and w must be 16-byte aligned");
         if (!aligned16(y) || (residual && !aligned16(residual))) return fail(YMX_EARG, "conv2d: y/residual must be 16-byte aligned");
-        if (label) { *label = "f8"; return YMX_OK; }
+        if (label) {
+            *label = "f8";
+            if (tile && !(*tile = conv_f8_tile(a, (long long)B * H * W))) return YMX_EUNSUPPORTED;
+            return YMX_OK;
+        }
         return launch_conv_f8(a, (long long)B * H * W, s);
     }
     if (x_dtype == YMX_F8E4M3) return fail(YMX_EARG, "conv2d: a quantised map needs an 8-bit kernel");
@@ -486,6 +490,15 @@ const char *ymx_conv_kernel_label(const ymx_op *op) {
     const int rc = conv_impl(o.x, o.w, o.scale, o.shift, o.residual, o.y, o.B, o.H, o.W, o.Cin, o.Cout, o.k, o.stride,
                              o.act, o.dtype, o.x_dtype, o.out_dtype, o.x_ld, o.res_ld, o.y_ld, nullptr, o.min_tiles, &label);
     return rc == YMX_OK ? label : nullptr;
+}
+
+const char *ymx_conv8_tile_label(const ymx_op *op) {
+    if (!op || op->kind != 1 || op->dtype != YMX_F8E4M3) { fail(YMX_EARG, "conv8_tile_label: not an 8-bit convolution op"); return nullptr; }
+    const ymx_op &o = *op;
+    const char *label = nullptr, *tile = nullptr;
+    const int rc = conv_impl(o.x, o.w, o.scale, o.shift, o.residual, o.y, o.B, o.H, o.W, o.Cin, o.Cout, o.k, o.stride, o.act, o.dtype,
+                             o.x_dtype, o.out_dtype, o.x_ld, o.res_ld, o.y_ld, nullptr, o.min_tiles, &label, nullptr, nullptr, &tile);
+    return rc == YMX_OK ? tile : nullptr;
 }
 
 // workspace layout of the decode/filter calls: [err:4 int][ticket: B int, padded to 16 B][state: B*nseg u64]

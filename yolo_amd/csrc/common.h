@@ -282,6 +282,7 @@ int launch_quantize(const void *x, int x_ld, void *q, long long n_pix, int C, in
 size_t packed_f8_bytes(int k, int Cin, int Cout);
 int launch_pack_f8(const float *w_hwio, void *packed, int k, int Cin, int Cout, hipStream_t s);
 int launch_conv_f8(const ConvArgs &a, long long in_pix, hipStream_t s);
+const char *conv_f8_tile(const ConvArgs &a, long long in_pix);
 bool conv_f8_raw(long long P, int Cout, int k, int out_dtype);
 int launch_pack_weights(const float *w_hwio, void *w_packed, int k, int Cin, int Cout, int dtype,
                         hipStream_t s, int src_cout = 0);

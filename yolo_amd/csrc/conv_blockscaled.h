@@ -208,5 +208,6 @@ __device__ __forceinline__ void f8_epilogue(const ConvArgs &a, f32x4_t (&acc)[NI
 
 bool conv_f8_wide(const F8Args &g);
 int launch_conv_f8_wide(const F8Args &g, hipStream_t s);
+const char *conv_f8_wide_tile(const F8Args &g);
 
 }  // namespace ymx

@@ -441,16 +441,28 @@ template <typename OT, int NWQ, int NWP, int NI, int NJ, int NSTAGE, bool RAW = 
 //   64 x 64, four stages: fewer (26^2 512 -> 1024 3x3: 19.2, two stages 27.3)
 //   64 x 32, four stages: where even that leaves half the CUs idle (13^2 512 -> 1024 3x3: 15.1, 64 x 64 18.0), and for
 //       32-bit outputs, whose conversions weigh more, wherever there are few tiles (8 x 26^2 1024 -> 255 1x1: 12.3, 14.4)
-template <typename OT> static int launch_f8_shape(const F8Args &g, hipStream_t s) {
-    if (conv_f8_wide(g)) return launch_conv_f8_wide(g, s);
+enum class F8Shape { WIDE, T128x128, T64x128, T32x128, T64x64_TWO_STAGES, T64x64, T64x32 };
+static F8Shape f8_shape(const F8Args &g) {
+    if (conv_f8_wide(g)) return F8Shape::WIDE;
+    const bool bf16 = g.a.out_dtype == YMX_BF16;
     const long long np = g.a.P, nq = (g.a.Cout + 63) / 64, n128 = (g.a.Cout + 127) / 128;
     const long long tiles = (np + 127) / 128 * nq;
-    if constexpr (sizeof(OT) == 2)
-        if (n128 * 8 <= nq * 5 && (np + 127) / 128 * n128 >= 300) return launch_f8_cfg<OT, 4, 2, 2, 4, 2>(g, s);
-    if (tiles >= 512) return g.a.Cout <= 32 ? launch_f8_cfg<OT, 2, 2, 1, 4, 2>(g, s) : launch_f8_cfg<OT, 2, 2, 2, 4, 2>(g, s);
-    if (tiles >= 200 && sizeof(OT) == 2) return launch_f8_cfg<OT, 4, 1, 1, 4, 2>(g, s);
-    if (sizeof(OT) == 4 || (np + 63) / 64 * nq <= 128) return launch_f8_cfg<OT, 4, 1, 1, 2, 4>(g, s);
-    return launch_f8_cfg<OT, 4, 1, 1, 4, 4>(g, s);
+    if (bf16 && n128 * 8 <= nq * 5 && (np + 127) / 128 * n128 >= 300) return F8Shape::T128x128;
+    if (tiles >= 512) return g.a.Cout <= 32 ? F8Shape::T32x128 : F8Shape::T64x128;
+    if (bf16 && tiles >= 200) return F8Shape::T64x64_TWO_STAGES;
+    return !bf16 || (np + 63) / 64 * nq <= 128 ? F8Shape::T64x32 : F8Shape::T64x64;
+}
+template <typename OT> static int launch_f8_shape(const F8Args &g, hipStream_t s) {
+    const F8Shape shape = f8_shape(g);
+    if constexpr (sizeof(OT) == 2) {                             // (shapes that 32-bit outputs never take)
+        if (shape == F8Shape::WIDE) return launch_conv_f8_wide(g, s);
+        if (shape == F8Shape::T128x128) return launch_f8_cfg<OT, 4, 2, 2, 4, 2>(g, s);
+        if (shape == F8Shape::T64x64_TWO_STAGES) return launch_f8_cfg<OT, 4, 1, 1, 4, 2>(g, s);
+        if (shape == F8Shape::T64x64) return launch_f8_cfg<OT, 4, 1, 1, 4, 4>(g, s);
+    }
+    if (shape == F8Shape::T64x128) return launch_f8_cfg<OT, 2, 2, 2, 4, 2>(g, s);
+    if (shape == F8Shape::T32x128) return launch_f8_cfg<OT, 2, 2, 1, 4, 2>(g, s);
+    return launch_f8_cfg<OT, 4, 1, 1, 2, 4>(g, s);
 }
 
 // Whether a layer on a bf16 map quantises it in its own kernel, in tiles of 64 x 32.  Every tile of channels and every tap
@@ -464,8 +476,7 @@ bool conv_f8_raw(long long P, int Cout, int k, int out_dtype) {
 
 // a: geometry of the convolution with x_ld = Cin; x = quantised map, or a bf16 one
 // where conv_f8_raw says so; w = packed kernel.
-int launch_conv_f8(const ConvArgs &args, long long in_pix, hipStream_t s) {
-    F8Args g;
+static int f8_args(const ConvArgs &args, long long in_pix, F8Args &g) {
     g.a = args;
     g.a.x_ld = 1;
     g.taps = args.k * args.k;
@@ -488,8 +499,27 @@ int launch_conv_f8(const ConvArgs &args, long long in_pix, hipStream_t s) {
         const long long rb = ((long long)(args.P - 1) * args.res_ld + args.Cout) * 2;
         g.a.res_bytes = rb < 0x80000000LL ? (unsigned)rb : 0u;
     }
-    if (raw) return args.out_dtype == YMX_BF16 ? launch_f8_cfg<bf16_t, 4, 1, 1, 2, 3, true>(g, s) : launch_f8_cfg<float, 4, 1, 1, 2, 3, true>(g, s);
+    return YMX_OK;
+}
+int launch_conv_f8(const ConvArgs &args, long long in_pix, hipStream_t s) {
+    F8Args g;
+    if (const int rc = f8_args(args, in_pix, g)) return rc;
+    if (args.x_dtype == YMX_BF16) return args.out_dtype == YMX_BF16 ? launch_f8_cfg<bf16_t, 4, 1, 1, 2, 3, true>(g, s) : launch_f8_cfg<float, 4, 1, 1, 2, 3, true>(g, s);
     return args.out_dtype == YMX_BF16 ? launch_f8_shape<bf16_t>(g, s) : launch_f8_shape<float>(g, s);
+}
+const char *conv_f8_tile(const ConvArgs &args, long long in_pix) {
+    F8Args g;
+    if (f8_args(args, in_pix, g)) return nullptr;
+    if (args.x_dtype == YMX_BF16) return "64x32 raw";
+    switch (f8_shape(g)) {
+        case F8Shape::WIDE: return conv_f8_wide_tile(g);
+        case F8Shape::T128x128: return "128x128";
+        case F8Shape::T64x128: return "64x128";
+        case F8Shape::T32x128: return "32x128";
+        case F8Shape::T64x64_TWO_STAGES: return "64x64, two stages";
+        case F8Shape::T64x64: return "64x64";
+        default: return "64x32";
+    }
 }
 
 }  // namespace ymx

@@ -392,10 +392,20 @@ bool conv_f8_wide(const F8Args &g) {
     return g.a.out_dtype == YMX_BF16 && nq * 16 <= n64 * 5 && tiles >= 160 && g.nkt > 2 && (slab_fits(g) || tiles <= 256 || tiles >= 512);
 }
 
+static TilePlan wide_plan(const F8Args &g, bool slab) {
+    if (slab && slab_lds(slab_pieces(g.a.W, 256)) > 160 * 1024) return TilePlan{192, 0, 0};
+    return plan_wide_tiles(g.a.P, (g.a.Cout + 255) / 256, 0.85, 0, 0);
+}
+const char *conv_f8_wide_tile(const F8Args &g) {
+    const bool slab = slab_fits(g);
+    const int px = wide_plan(g, slab).pixels;
+    if (slab) return px == 256 ? "256x256 slab" : px == 192 ? "256x192 slab" : "256x256 and 256x192 slab";
+    return px == 256 ? "256x256" : px == 192 ? "256x192" : "256x256 and 256x192";
+}
+
 template <bool SLAB> static int launch_wide(const F8Args &g, hipStream_t s) {
     const int ntq = (g.a.Cout + 255) / 256, np4 = slab_pieces(g.a.W, 256), np3 = slab_pieces(g.a.W, 192);
-    const bool big_fits = !SLAB || slab_lds(np4) <= 160 * 1024;
-    TilePlan pl = big_fits ? plan_wide_tiles(g.a.P, ntq, 0.85, 0, 0) : TilePlan{192, 0, 0};
+    const TilePlan pl = wide_plan(g, SLAB);
     const long long t4 = ((long long)g.a.P + 255) / 256;
     int nbig = 0, pbig = 0;
     if (pl.pixels == 256) { nbig = (int)(t4 * ntq); pbig = g.a.P; }
