@@ -648,6 +648,24 @@ def test_a_changed_state_is_noticed():
             y.sum().backward()
 
 
+@pytest.mark.parametrize("size", [13, 60])
+def test_inside_an_activation_checkpoint(size):
+    """A segment run again in the backward pass, its state drawn outside: the gradients of the plain call."""
+    from torch.utils.checkpoint import checkpoint
+    from yolo_amd import training as T
+    from yolo_amd.layers import Dropout
+    x, ga, be, sc, dy = (t.to(DEV) for t in _case((2, size, size, 64), torch.float32, 3))
+    drop = Dropout(0.3, seed=5).to(DEV)
+    leaves = [t.requires_grad_() for t in (x, ga, be, sc)]
+    one, two = drop.draw(), drop.draw()
+
+    def segment(a, b, c, d):
+        return T.dropout(T.group_norm_act(a, b, c, 8, "mish", d, rate=0.2, state=one), 0.3, two)
+    want = torch.autograd.grad(segment(*leaves), leaves, dy)
+    got = torch.autograd.grad(checkpoint(segment, *leaves, use_reentrant=False), leaves, dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and int(drop.state[1]) == 2
+
+
 def test_second_derivatives_are_refused():
     from yolo_amd import training as T
     x = torch.randn(2, 4, 4, 32, device=DEV, requires_grad=True)

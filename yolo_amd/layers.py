@@ -149,7 +149,9 @@ class Dropout(nn.Module):
     step captured into a HIP graph draws another mask at each replay, and a checkpoint of the
     module resumes the sequence.  seed: default one drawn from torch's CPU generator; layers with
     the same seed draw the same masks, and so do the ranks of a data-parallel job that build the
-    model from the same generator state.
+    model from the same generator state.  A second run of a call, as activation checkpointing makes
+    one in the backward pass, draws another mask: there, draw() outside the segment and call
+    yolo_amd.training.dropout with the state inside.
     """
 
     def __init__(self, rate, seed=None):
