@@ -245,6 +245,40 @@ def test_group_norm_beyond_32_bit_offsets():
     assert float(((y - want).abs() / (2.0 ** -8 * want.abs() + UNITS * (1 + want.abs()))).max()) <= 1.0
 
 
+def test_group_norm_backward_beyond_32_bit_offsets():
+    """More than 2^31 elements, with dropout: dx of the last group of the last sample and the parameters' gradients of its channels,
+    against 64-bit arithmetic on those slices (the mask as the forward pass shows it)."""
+    from yolo_amd import training as T
+    P, C, G, rate = 1050000, 1024, 32, 0.5
+    g = torch.Generator(device=DEV).manual_seed(2)
+    x, dy = (torch.empty((2, P, C), device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    for b in range(2):
+        x[b].normal_(generator=g)
+        dy[b].normal_(generator=g)
+    leaves = [x.requires_grad_(), torch.ones(C, device=DEV, requires_grad=True), torch.zeros(C, device=DEV, requires_grad=True)]
+    y = T.group_norm_act(*leaves, G, "mish", rate=rate, state=torch.tensor([7, 8], device=DEV))
+    keep = y.detach()[..., -32:] != 0
+    dx, dgamma, dbeta = torch.autograd.grad(y, leaves, dy)
+    del y
+    sums = [0.0] * 4
+    for b in range(2):
+        h = x.detach()[b, :, -32:].double()
+        h -= h.mean()
+        r = 1.0 / torch.sqrt(h.square().mean() + 1e-3)
+        h *= r
+        m = torch.where(keep[b], dy[b, :, -32:].double() / (1 - rate), 0.0)
+        dt = m * O.act_grad(h, "mish")
+        mag = m.abs() * (1 + h.abs())
+        for i, v in enumerate((dt * h, dt, mag * (1 + h.abs()), mag)):
+            sums[i] = sums[i] + v.sum(0)
+    want = r * (dt - dt.mean() - h * (dt * h).mean())
+    mag = r * (1 + h.abs()) * (mag + mag.mean() + h.abs() * (mag * h.abs()).mean())
+    err = (dx[1, :, -32:].double() - want).abs()
+    assert float((err / (2.0 ** -8 * want.abs() + UNITS * mag)).max()) <= 1.0
+    for got, want, mag in ((dgamma, sums[0], sums[2]), (dbeta, sums[1], sums[3])):
+        assert float(((got[-32:].double() - want).abs() / (2.0 ** -24 * want.abs() + UNITS * mag)).max()) <= 1.0
+
+
 # ---------------------------------------------------------------- dropout
 @pytest.mark.parametrize("n,dt,rate,use_sc", [(1, "f32", 0.5, False), (7, "bf16", 0.3, True), (4099, "bf16", 0.1, False),
                                               (8 * 19 * 19 * 255, "f32", 0.5, True), (1 << 20, "bf16", 0.25, True),
