@@ -121,7 +121,10 @@ int ymx_conv2d_fused_ex(const void *x, const void *w, const void *scale, const v
  * The convolution entry points above with dtype = x_dtype = YMX_F8E4M3: x is a quantised map, w a
  * kernel packed by ymx_pack_weights(..., YMX_F8E4M3), k is 1 or 3, Cin a multiple of 16; scale,
  * shift and act as above, y and residual have the type out_dtype (fp32 or bf16; both 0-dense or
- * with pixel strides), products are accumulated in fp32.  ymx_packed_weight_bytes gives the size.
+ * with pixel strides).  Sums for fp32 outputs: exact products, added in fp32.  For bf16 outputs the 8-bit matrix pipe
+ * adds products in groups of eight aligned to the group's largest, of which it keeps 13 bits below the leading one
+ * (5e-5 of the result on random operands, a thirtieth of bf16's half step; more where large products cancel), and the
+ * groups in fp32.  ymx_packed_weight_bytes gives the size.
  *
  * Layers for which ymx_conv2d_quantizes(output pixels, Cout, k, out_dtype) returns 1 also take x_dtype = YMX_BF16, a bf16 map with pixel
  * stride x_ld, and quantise it themselves: the same result in one launch.
