@@ -624,6 +624,23 @@ def test_leaky_derivative_at_zero(shape, groups, dt, kind):
         _within(name, v, want[name], want[name + "_mag"], DT[dt] if name == "dx" else torch.float32)
 
 
+@pytest.mark.parametrize("shape,groups,dt", [((3, 13, 13, 256), 16, "bf16"), ((3, 13, 13, 128), 8, "f32"), ((2, 40, 41, 96), 32, "f32"),
+                                             ((2, 104, 104, 64), 4, "bf16"), ((2, 19, 19, 255), 5, "f32"), ((1, 77, 77, 1024), 1, "f32")])
+def test_leaky_derivative_of_a_constant_map(shape, groups, dt):
+    """A map without spread is its own mean exactly, whatever the value (1 / n and sums of n values are not exact): with beta = 0 every
+    t is 0, on the side of the slope 0.1."""
+    from yolo_amd import training as T
+    c = shape[-1]
+    g = torch.Generator().manual_seed(c)
+    value = torch.rand(groups, generator=g).repeat_interleave(c // groups)
+    x = (torch.zeros(shape) + 10.0 * value).to(DT[dt]).to(DEV)
+    be = torch.zeros(c, device=DEV, requires_grad=True)
+    ga = torch.randn(c, generator=g).to(DEV)
+    dbeta, = torch.autograd.grad(T.group_norm_act(x, ga, be, groups, "leaky"), [be], torch.ones_like(x))
+    n = x.numel() // c
+    assert torch.allclose(dbeta, torch.full_like(dbeta, 0.1 * n), rtol=1e-5), (dbeta / n)
+
+
 @pytest.mark.parametrize("kind", ["parameters", "map"])
 def test_leaky_backward_at_zero_is_as_fast(kind):
     """Signs of t = 0 need no second look: the backward step over such a map takes the time of any other (a factor of two
